@@ -36,6 +36,11 @@ class CompCacheS(C.Structure):
                 ("bits", vp), ("keep", vp), ("sink", vp), ("recent", vp)]
 
 
+class Q8CacheS(C.Structure):
+    _fields_ = [("codes", vp), ("scale", vp), ("page_table", vp),
+                ("n_pages", C.c_int), ("page_size", C.c_int), ("max_pages", C.c_int)]
+
+
 class DimsS(C.Structure):
     _fields_ = [("n_layers", C.c_int), ("n_kv", C.c_int), ("d", C.c_int), ("batch", C.c_int)]
 
@@ -91,6 +96,14 @@ _SIGS = {
     "dkv_attn_comp": (C.c_int, [C.POINTER(CompCacheS), DimsS, C.c_int, C.c_int, vp, vp, vp, C.c_int, vp,
                                 C.c_size_t, vp]),
     "dkv_attn_work_bytes": (C.c_size_t, [DimsS, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
+    "dkv_q8_append": (C.c_int, [C.POINTER(Q8CacheS), DimsS, C.c_int, vp, vp, C.c_int, C.c_int, C.c_int64, C.c_int64,
+                                C.c_int64, vp, vp, vp, vp, vp, vp]),
+    "dkv_q8_read": (C.c_int, [C.POINTER(Q8CacheS), DimsS, C.c_int, C.c_int, C.c_int, vp, vp]),
+    "dkv_q8_attn_work_bytes": (C.c_size_t, [DimsS, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
+    "dkv_q8_attn": (C.c_int, [C.POINTER(Q8CacheS), DimsS, C.c_int, C.c_int, C.c_int, vp, vp, vp, vp, C.c_int, C.c_int,
+                              vp, vp, C.c_size_t, vp]),
+    "dkv_q8_evict": (C.c_int, [C.POINTER(Q8CacheS), DimsS, C.c_int, vp, vp, C.c_int, C.c_int, vp, vp, vp, C.c_int, vp,
+                               vp, vp, vp]),
     "dkv_pack_weight_bytes": (C.c_size_t, [C.c_int, C.c_int]),
     "dkv_pack_weight": (C.c_int, [vp, C.c_int, C.c_int, vp, vp]),
     "dkv_gemm": (C.c_int, [vp, C.c_int, vp, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(EpilogueS), vp,

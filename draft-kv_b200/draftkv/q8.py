@@ -1,0 +1,385 @@
+"""A paged KV cache held in 8 bits, with the attention that reads it and
+eviction by accumulated attention weight.
+
+Beside PagedKVCache (bf16 / fp32, draftkv/paged.py:76-177 of the reference)
+and CompressedKVCache (the drafter's slot arrays): half the bytes of the bf16
+cache, the same block allocator and rollback, decode / verify / prompt
+attention, and a bound on its length by eviction per KV head.  The reference
+has no counterpart.
+
+K and V are e4m3 codes under one power-of-two scale per block of tokens, KV
+head and side (byte order: include/draftkv_b200.h, dkv_q8_cache).  Entries are
+counted per layer from 0; until the first eviction entry i is position i.
+"""
+
+from __future__ import annotations
+
+import numpy as np
+
+from . import _lib
+from .paged import BlockPool, BlockPoolExhausted, PagedKVCache, dtype_code
+
+try:
+    import torch
+except ImportError:  # pragma: no cover
+    torch = None
+
+BLOCK_SIZES = (16, 32, 64, 128)
+HEAD_DIMS = (64, 128)
+MASS_ROWS = 64          # query rows a KV head up to which attention can add up the mass
+
+
+def tile_bytes(d_head: int):
+    """(K, V) int64 tables [16, d]: the byte of element (token, dim) inside a
+    16-token tile of the pool (the tensor core's operand order)."""
+    tok, dim = np.arange(16)[:, None], np.arange(d_head)[None, :]
+    blk, r, c = dim // 32, dim % 32, dim % 16
+    k = blk * 512 + ((tok % 8) * 4 + (c % 8) // 2) * 16 + ((r // 16) * 2 + tok // 8) * 4 + (c // 8) * 2 + c % 2
+    v = blk * 512 + ((c % 8) * 4 + (tok % 8) // 2) * 16 + ((r // 16) * 2 + c // 8) * 4 + (tok // 8) * 2 + tok % 2
+    return k, v
+
+
+def _check_i32(name: str, t, shape, device) -> None:
+    if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)} on {device}")
+
+
+class Q8KVCache(PagedKVCache):
+    """The 8-bit paged cache: block tables and rollback of PagedKVCache, the
+    pool in e4m3.  `track_mass` keeps per entry the softmax weight it has
+    received (per layer [batch][n_kv][capacity], added to by attention calls
+    and model forwards) and its position, which `evict` goes by."""
+
+    def __init__(self, n_layers: int, n_heads: int, d_head: int, block_size: int = 16, n_blocks: int = 512,
+                 batch: int = 1, max_blocks_per_seq: int | None = None, device: str = "cuda",
+                 track_mass: bool = False) -> None:
+        self._check_shape(d_head, block_size)
+        self.track_mass = track_mass
+        super().__init__(n_layers, n_heads, d_head, block_size=block_size, n_blocks=n_blocks, dtype=np.float32,
+                         batch=batch, max_blocks_per_seq=max_blocks_per_seq, device=device)
+        self.next_pos = [0] * batch          # position of the next token (entries + evicted)
+
+    @staticmethod
+    def _check_shape(d_head: int, block_size: int) -> None:
+        if d_head not in HEAD_DIMS:
+            raise ValueError(f"the 8-bit cache holds heads of {HEAD_DIMS} (got {d_head})")
+        if block_size not in BLOCK_SIZES:
+            raise ValueError(f"the 8-bit cache has blocks of {BLOCK_SIZES} tokens (got {block_size})")
+
+    @classmethod
+    def from_storage(cls, codes, scale, page_table, block_size: int = 16) -> "Q8KVCache":
+        """A cache over storage the caller owns and allocates: codes uint8
+        [n_pages, n_kv, 2, block_size * d], scale f32 [n_pages, n_kv, 2] and
+        page_table int32 [batch, n_layers, max_pages], all contiguous on one
+        CUDA device.  The device calls (write, attention, evict_rows, read_rows)
+        work; the block allocator's methods do not."""
+        if codes.dtype != torch.uint8 or codes.dim() != 4 or codes.shape[2] != 2 or not codes.is_contiguous():
+            raise ValueError("codes must be a contiguous uint8 tensor [n_pages, n_kv, 2, block_size * d]")
+        if codes.shape[3] % block_size:
+            raise ValueError(f"codes rows of {codes.shape[3]} bytes are no whole block of {block_size} tokens")
+        self = cls.__new__(cls)
+        self.n_heads, self.d_head = codes.shape[1], codes.shape[3] // block_size
+        cls._check_shape(self.d_head, block_size)
+        if scale.dtype != torch.float32 or tuple(scale.shape) != tuple(codes.shape[:3]) or not scale.is_contiguous():
+            raise ValueError("scale must be a contiguous float32 tensor [n_pages, n_kv, 2]")
+        if page_table.dtype != torch.int32 or page_table.dim() != 3 or not page_table.is_contiguous():
+            raise ValueError("page_table must be a contiguous int32 tensor [batch, n_layers, max_pages]")
+        if not (codes.is_cuda and scale.device == codes.device and page_table.device == codes.device):
+            raise ValueError("codes, scale and page_table must be on one CUDA device")
+        self.batch, self.n_layers, self.max_pages = page_table.shape
+        self.block_size, self.device, self.track_mass = block_size, codes.device, False
+        self.pool, self.mass, self.pos_t = None, None, None
+        self.codes, self.scale, self.table_dev = codes, scale, page_table
+        self._dirty = False
+        self._finish_struct()
+        return self
+
+    # ------------------------------------------------------------ device
+    def _alloc_device(self, n_blocks: int) -> None:
+        _lib.load()
+        dev = self.device
+        self.codes = torch.zeros((n_blocks, self.n_heads, 2, self.block_size * self.d_head), dtype=torch.uint8, device=dev)
+        self.scale = torch.ones((n_blocks, self.n_heads, 2), dtype=torch.float32, device=dev)
+        self.table_host = torch.zeros((self.batch, self.n_layers, self.max_pages), dtype=torch.int32, pin_memory=True)
+        self.table_dev = torch.zeros((self.batch, self.n_layers, self.max_pages), dtype=torch.int32, device=dev)
+        self.device = self.codes.device
+        self._dirty = False
+        shape = (self.batch, self.n_heads, self.max_pages * self.block_size)
+        self.mass = self.pos_t = None
+        if self.track_mass:
+            # one more than the layers: eviction writes out of place and swaps
+            self.mass = [torch.zeros(shape, dtype=torch.float32, device=dev) for _ in range(self.n_layers + 1)]
+            self.pos_t = [torch.full(shape, -1, dtype=torch.int32, device=dev) for _ in range(self.n_layers + 1)]
+        self._finish_struct()
+
+    def _finish_struct(self) -> None:
+        self._struct = _lib.Q8CacheS(self.codes.data_ptr(), self.scale.data_ptr(), self.table_dev.data_ptr(),
+                                     self.codes.shape[0], self.block_size, self.max_pages)
+        self._dims = _lib.DimsS(self.n_layers, self.n_heads, self.d_head, self.batch)
+        self._work: dict = {}
+
+    def struct(self) -> "_lib.Q8CacheS":
+        self.sync_table()
+        return self._struct
+
+    @property
+    def host_resident(self) -> bool:
+        return False
+
+    def offload_to_host(self) -> None:
+        raise NotImplementedError("the 8-bit cache stays in device memory")
+
+    @property
+    def nbytes(self) -> int:
+        """Bytes of the pool (codes and scales)."""
+        return self.codes.numel() + self.scale.numel() * 4
+
+    def _workspace(self, T: int, group: int, split_keys: int, note_mass: bool):
+        """The attention scratch of a call shape: zero when made, left ready by
+        each call, one per stream (calls on one stream run in order).  Inside a
+        stream capture a fresh one, cleared by the graph itself, belongs to the
+        graph."""
+        stream = _lib.stream_ptr()
+        key = (T, group, split_keys, note_mass, stream)
+        w = self._work.get(key)
+        if w is None:
+            n = int(_lib.load().dkv_q8_attn_work_bytes(self._dims, group, T, self.capacity_tokens, split_keys,
+                                                       1 if note_mass else 0))
+            w = torch.zeros(max(n, 16), dtype=torch.uint8, device=self.device)
+            if not torch.cuda.is_current_stream_capturing():
+                self._work[key] = w
+        return w
+
+    def _on_device(self):
+        """The cache's device as the current one (launches go there)."""
+        if torch.cuda.current_device() != self.device.index:
+            raise ValueError(f"the cache is on {self.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+    # ------------------------------------------------------ device calls
+    def write(self, layer: int, k, v, entry0, n_rows=None, pos0=None, mass=None, pos=None) -> None:
+        """Quantizes rows into entries entry0[b] .. of `layer` on the device.
+        k, v: [batch, rows, n_kv, d] bf16 or fp32, any strides with the last
+        dimension contiguous (the same for both); entry0, n_rows, pos0: int32
+        [batch].  mass / pos ([batch, n_kv, capacity]): reset for the new
+        entries.  The pages must be in the table (`ensure`)."""
+        self._on_device()
+        if k.dim() != 4 or k.shape[0] != self.batch or k.shape[2] != self.n_heads or k.shape[3] != self.d_head:
+            raise ValueError(f"k must be [{self.batch}, rows, {self.n_heads}, {self.d_head}], got {tuple(k.shape)}")
+        if v.shape != k.shape or v.dtype != k.dtype or v.stride() != k.stride():
+            raise ValueError("k and v must have one shape, dtype and strides")
+        if k.device != self.device or v.device != self.device:
+            raise ValueError(f"k and v must be on {self.device}")
+        if k.dtype not in (torch.bfloat16, torch.float32) or k.stride(3) != 1:
+            raise ValueError("k and v must be bf16 or fp32 with a contiguous last dimension")
+        _check_i32("entry0", entry0, (self.batch,), self.device)
+        for name, t in (("n_rows", n_rows), ("pos0", pos0)):
+            if t is not None:
+                _check_i32(name, t, (self.batch,), self.device)
+        self._check_mass(mass)
+        if pos is not None:
+            _check_i32("pos", pos, self._mass_shape(), self.device)
+        rows = k.shape[1]
+        if rows == 0:
+            return
+        sb, st, sh, _ = k.stride()
+        _lib.call("dkv_q8_append", self.struct(), self._dims, layer, k.data_ptr(), v.data_ptr(), dtype_code(k.dtype), rows,
+                  sb, st, sh, entry0.data_ptr(), _lib.ptr(n_rows), _lib.ptr(pos0), _lib.ptr(mass), _lib.ptr(pos),
+                  _lib.stream_ptr())
+
+    def _mass_shape(self):
+        return (self.batch, self.n_heads, self.capacity_tokens)
+
+    def _check_mass(self, mass) -> None:
+        if mass is not None and (mass.dtype != torch.float32 or tuple(mass.shape) != self._mass_shape()
+                                 or not mass.is_contiguous() or mass.device != self.device):
+            raise ValueError(f"mass must be a contiguous float32 tensor of shape {self._mass_shape()} on {self.device}")
+
+    def attention(self, layer: int, q, entry0, n_rows=None, mass=None, out=None, out_dtype=None, split_keys: int = 0,
+                  work=None):
+        """Causal attention of q [batch, T, n_heads, d] fp32 over `layer`: token
+        t of sequence b sees entries 0 .. entry0[b] + t (those of the call must
+        have been written).  Returns [batch, T, n_heads, d] in out_dtype (bf16
+        by default); tokens t >= n_rows[b] are skipped and their rows of `out`
+        left as they were (zeros when `out` is made here).  mass (T * n_heads /
+        n_kv <= 64): every seen entry's softmax weights are added to it.  A row
+        of up to 64 equals the one-token call at that entry bit for bit.  `work`:
+        scratch of `dkv_q8_attn_work_bytes` (zero when first used) for a caller
+        that runs or replays calls side by side; by default the cache keeps one
+        per stream and call shape."""
+        self._on_device()
+        if q.dim() != 4 or q.shape[0] != self.batch or q.shape[3] != self.d_head or q.shape[2] % self.n_heads \
+                or q.shape[2] == 0:
+            raise ValueError(f"q must be [{self.batch}, T, a multiple of {self.n_heads} heads, {self.d_head}], "
+                             f"got {tuple(q.shape)}")
+        if q.dtype != torch.float32 or not q.is_contiguous() or q.device != self.device:
+            raise ValueError(f"q must be a contiguous float32 tensor on {self.device}")
+        _check_i32("entry0", entry0, (self.batch,), self.device)
+        if n_rows is not None:
+            _check_i32("n_rows", n_rows, (self.batch,), self.device)
+        self._check_mass(mass)
+        T, group = q.shape[1], q.shape[2] // self.n_heads
+        if out is None:
+            make = torch.empty if n_rows is None else torch.zeros
+            out = make(q.shape, dtype=out_dtype or torch.bfloat16, device=self.device)
+        elif out.shape != q.shape or not out.is_contiguous() or out.device != self.device \
+                or (out_dtype is not None and out.dtype != out_dtype):
+            raise ValueError("out must be contiguous and shaped like q")
+        if out.dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError("attention writes bf16 or fp32")
+        if T == 0:
+            return out
+        if work is None:
+            work = self._workspace(T, group, split_keys, mass is not None)
+        _lib.call("dkv_q8_attn", self.struct(), self._dims, layer, group, T, q.data_ptr(), entry0.data_ptr(),
+                  _lib.ptr(n_rows), out.data_ptr(), dtype_code(out.dtype), split_keys, _lib.ptr(mass), work.data_ptr(),
+                  work.numel(), _lib.stream_ptr())
+        return out
+
+    def evict_rows(self, layer: int, n, budget, out_table, mass, pos=None, sink: int = 0, recent: int = 0,
+                   mass_out=None, pos_out=None):
+        """Per (sequence, KV head), of the first n[b] entries of `layer` keeps
+        min(n, max(budget[b], sink + recent)): the first `sink`, the last
+        `recent` and those of the most mass (the lowest (mass, index) are
+        dropped).  They are written to the pages out_table [batch, out_pages],
+        which must be in no row of the page table.  Returns (kept [batch, n_kv,
+        out_pages * block_size] int32 entry indices, -1 behind; mass_out;
+        pos_out or None)."""
+        self._on_device()
+        _check_i32("n", n, (self.batch,), self.device)
+        _check_i32("budget", budget, (self.batch,), self.device)
+        if out_table.dim() != 2:
+            raise ValueError("out_table must be [batch, out_pages]")
+        _check_i32("out_table", out_table, (self.batch, out_table.shape[1]), self.device)
+        if mass is None:
+            raise ValueError("eviction goes by the attention mass")
+        self._check_mass(mass)
+        self._check_mass(mass_out)
+        for name, t in (("pos", pos), ("pos_out", pos_out)):
+            if t is not None:
+                _check_i32(name, t, self._mass_shape(), self.device)
+        if mass_out is None:
+            mass_out = torch.empty_like(mass)
+        if pos is None:
+            pos_out = None
+        elif pos_out is None:
+            pos_out = torch.empty_like(pos)
+        out_pages = out_table.shape[1]
+        kept = torch.empty((self.batch, self.n_heads, out_pages * self.block_size), dtype=torch.int32, device=self.device)
+        _lib.call("dkv_q8_evict", self.struct(), self._dims, layer, n.data_ptr(), budget.data_ptr(), sink, recent,
+                  mass.data_ptr(), _lib.ptr(pos), out_table.data_ptr(), out_pages, mass_out.data_ptr(), _lib.ptr(pos_out),
+                  kept.data_ptr(), _lib.stream_ptr())
+        return kept, mass_out, pos_out
+
+    def read_rows(self, layer: int, n: int, b: int = 0):
+        """Entries [0, n) of one sequence, dequantized: fp32 [n, n_kv, 2, d] on
+        the device."""
+        self._on_device()
+        out = torch.empty((n, self.n_heads, 2, self.d_head), dtype=torch.float32, device=self.device)
+        _lib.call("dkv_q8_read", self.struct(), self._dims, b, layer, n, out.data_ptr(), _lib.stream_ptr())
+        return out
+
+    # ---------------------------------------------------- cache protocol
+    def append(self, layer: int, k, v, pos) -> None:
+        """Rows (numpy [rows, n_kv, d]) of sequence 0 at its end; positions must
+        follow each other (after an eviction they run ahead of the entries)."""
+        k, v = np.asarray(k, np.float32), np.asarray(v, np.float32)
+        pos = np.asarray(pos).reshape(-1)
+        n, start = k.shape[0], self.counts[0][layer]
+        if n == 0:
+            return
+        if not np.array_equal(pos, np.arange(pos[0], pos[0] + n)) or pos[0] < start:
+            raise ValueError("appended positions must be consecutive and not below the entry they get")
+        self._ensure_layer(0, layer, start + n)
+        kv = torch.from_numpy(np.ascontiguousarray(np.stack([k, v])[:, None])).to(self.device)
+        rows = torch.zeros((self.batch,), dtype=torch.int32)
+        rows[0] = n
+        e0 = torch.zeros((self.batch,), dtype=torch.int32)
+        e0[0] = start
+        p0 = torch.full((self.batch,), int(pos[0]), dtype=torch.int32, device=self.device)
+        kv = kv.expand(2, self.batch, -1, -1, -1)
+        self.write(layer, kv[0], kv[1], e0.to(self.device), n_rows=rows.to(self.device), pos0=p0,
+                   mass=self.mass[layer] if self.mass else None, pos=self.pos_t[layer] if self.pos_t else None)
+        self.counts[0][layer] = start + n
+        if layer == 0:
+            self.next_pos[0] = int(pos[0]) + n
+
+    def _ensure_layer(self, b: int, layer: int, n_tokens: int) -> None:
+        need = -(-n_tokens // self.block_size)
+        if need > self.max_pages:
+            raise BlockPoolExhausted(f"sequence needs {need} blocks > max_blocks_per_seq {self.max_pages}")
+        tbl = self.block_tables[b][layer]
+        if len(tbl) < need:
+            new = self.pool.allocate_many(need - len(tbl))
+            self.table_host[b, layer, len(tbl):need] = torch.tensor(new, dtype=torch.int32)
+            tbl.extend(new)
+            self._dirty = True
+
+    def positions(self, layer: int, b: int = 0):
+        """Positions [n_kv, entries] of a sequence's entries (numpy int64)."""
+        n = self.counts[b][layer]
+        if self.pos_t is None:
+            return np.broadcast_to(np.arange(n, dtype=np.int64), (self.n_heads, n))
+        return self.pos_t[layer][b, :, :n].cpu().numpy().astype(np.int64)
+
+    def read(self, layer: int, b: int = 0):
+        """Dequantized (k, v, positions) of a sequence's entries.  Positions are
+        [entries] while every head holds the same ones, [n_kv, entries] after an
+        eviction that parted them."""
+        n = self.counts[b][layer]
+        if n == 0:
+            z = np.zeros((0, self.n_heads, self.d_head), np.float32)
+            return z, z.copy(), np.zeros((0,), np.int64)
+        o = self.read_rows(layer, n, b).cpu().numpy()
+        pos = self.positions(layer, b)
+        return o[:, :, 0], o[:, :, 1], pos[0] if (pos == pos[:1]).all() else pos
+
+    def truncate_seq(self, b: int, n_pos: int) -> None:
+        """Rollback to n_pos entries (paged.py:144-162); the scale of a partly
+        emptied block stays until the block is written from its start again."""
+        before = self.counts[b][0]
+        super().truncate_seq(b, n_pos)
+        self.next_pos[b] -= before - self.counts[b][0]
+
+    def set_length(self, b: int, n: int) -> None:
+        self.next_pos[b] += n - self.counts[b][0]
+        super().set_length(b, n)
+
+    def evict(self, budget: int, sink: int = 4, recent: int = 16, layers=None):
+        """Prunes every sequence to at most max(budget, sink + recent) entries a
+        layer by accumulated attention mass, per KV head.  New blocks are taken
+        from the pool before the old ones return to it (BlockPoolExhausted leaves
+        the cache as it was).  Returns {layer: kept entry indices [batch, n_kv,
+        .] on the device} of the layers that were pruned."""
+        if not self.track_mass:
+            raise ValueError("evict needs track_mass=True")
+        if budget < 1 or sink < 0 or recent < 0:
+            raise ValueError("evict: budget >= 1, sink >= 0, recent >= 0")
+        keep_to = max(budget, sink + recent)
+        out = {}
+        for L in range(self.n_layers) if layers is None else layers:
+            n = [self.counts[b][L] for b in range(self.batch)]
+            if max(n) <= keep_to:
+                continue
+            m = [min(x, keep_to) for x in n]
+            pages = [-(-x // self.block_size) for x in m]
+            if sum(pages) > self.pool.n_free:
+                raise BlockPoolExhausted(f"eviction needs {sum(pages)} free blocks, {self.pool.n_free} left")
+            new = [self.pool.allocate_many(p) for p in pages]
+            out_pages = max(max(pages), 1)
+            table = torch.full((self.batch, out_pages), -1, dtype=torch.int32)
+            for b, ids in enumerate(new):
+                table[b, :len(ids)] = torch.tensor(ids, dtype=torch.int32)
+            dev = self.device
+            out[L], _, _ = self.evict_rows(
+                L, torch.tensor(n, dtype=torch.int32).to(dev), torch.tensor(m, dtype=torch.int32).to(dev), table.to(dev),
+                self.mass[L], self.pos_t[L], sink, recent, self.mass[-1], self.pos_t[-1])
+            self.mass[L], self.mass[-1] = self.mass[-1], self.mass[L]
+            self.pos_t[L], self.pos_t[-1] = self.pos_t[-1], self.pos_t[L]
+            for b, ids in enumerate(new):
+                for blk in reversed(self.block_tables[b][L]):
+                    self.pool.free(blk)
+                self.block_tables[b][L] = list(ids)
+                self.table_host[b, L, :len(ids)] = table[b, :len(ids)]
+                self.counts[b][L] = m[b]
+            self._dirty = True
+        return out

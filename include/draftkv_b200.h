@@ -80,7 +80,9 @@ DKV_API const char* dkv_last_error(void);
 DKV_API int dkv_version(void);
 /* Reads and clears the device error word kernels set instead of trapping:
  * 0x10 append rows over the per-call limit, 0x20 drafter slot capacity,
- * 0x100 token id outside the vocabulary, 0x200 position outside the table. */
+ * 0x100 token id outside the vocabulary, 0x200 position outside the table,
+ * 0x400 page id or entry outside an 8-bit cache, 0x800 infinity or NaN
+ * written to an 8-bit cache. */
 DKV_API int dkv_device_error(uint32_t* out_code, void* stream);
 
 /* Launch timing by kernel class with CUDA events on the launching stream
@@ -225,6 +227,87 @@ DKV_API int dkv_attn_comp(const dkv_comp_cache* comp, dkv_dims dims, int layer, 
 /* Scratch bytes the two attention calls need for a given shape. */
 DKV_API size_t dkv_attn_work_bytes(dkv_dims dims, int group, int T, int max_ctx, int split_keys,
                            int comp_cap);
+
+/* ------------------------------------------------------------ 8-bit paged cache
+ * A paged cache in 8 bits beside the full cache (no counterpart in the
+ * reference): K and V as e4m3 codes with one power-of-two scale per page
+ * (block of page_size tokens), KV head and side; value = code * scale.
+ *     codes       [n_pages][n_kv][2][page_size * d]    K then V
+ *     scale       [n_pages][n_kv][2]                    f32
+ *     page_table  [batch][n_layers][max_pages]          int32
+ * page_size 16, 32, 64 or 128; d 64 or 128; capacity = max_pages * page_size
+ * entries a sequence.  Entries are counted from 0 and need not be positions:
+ * after an eviction entry i is the i-th kept token.
+ *
+ * Byte order of a page side: tiles of 16 tokens, 16 * d bytes each, in the
+ * tensor core's operand order: block j of 512 bytes covers dims 32j..32j+31;
+ * lane 4g+t owns 16 bytes of it; their 32-bit word w holds, lowest byte first,
+ *   K: token g + 8 (w & 1), dims 32j + 16 (w >> 1) + {2t, 2t+1, 2t+8, 2t+9};
+ *   V: dim 32j + 16 (w >> 1) + 8 (w & 1) + g, tokens {2t, 2t+1, 2t+8, 2t+9}.
+ *
+ * A page id outside [0, n_pages) in the table is never followed: nothing is
+ * written there, its entries are not seen, and 0x400 is recorded in the device
+ * error word, as for entries outside the capacity. */
+typedef struct dkv_q8_cache {
+    uint8_t* codes;
+    float* scale;
+    const int32_t* page_table;
+    int n_pages, page_size, max_pages;
+} dkv_q8_cache;
+
+/* Quantizes n_rows[b] (rows when n_rows is NULL) tokens of sequence b into
+ * entries entry0[b] .. of `layer`.  k, v: element (b, r, head, x) at
+ * b * seq_stride + r * token_stride + head * head_stride + x, in src_dtype.
+ * Per page, head and side: e = the smallest exponent with max|x| 2^-e <= 448
+ * over the new rows, in [-120, 119]; a page that holds earlier rows keeps the
+ * larger of its exponent and e, and re-rounds their codes when it grows.  A
+ * page written from its first row restarts its scale, so a rolled-back
+ * sequence is simply written over.  Rows behind the last new one keep their
+ * bytes.  Codes are rounded once, to nearest even.  Non-finite values are
+ * stored as the largest value (infinities) or zero (NaN) and recorded as 0x800.
+ * mass, pos ([batch][n_kv][capacity], either may be NULL): the new entries get
+ * mass 0 and position pos0[b] + r (entry0[b] + r when pos0 is NULL). */
+DKV_API int dkv_q8_append(const dkv_q8_cache* cache, dkv_dims dims, int layer, const void* d_k, const void* d_v,
+                          int src_dtype, int rows, int64_t seq_stride, int64_t token_stride, int64_t head_stride,
+                          const int32_t* d_entry0, const int32_t* d_n_rows, const int32_t* d_pos0, float* d_mass,
+                          int32_t* d_pos, void* stream);
+
+/* Entries [0, n) of (b, layer) as f32 [n][n_kv][2][d] (zero where the page id
+ * is bad). */
+DKV_API int dkv_q8_read(const dkv_q8_cache* cache, dkv_dims dims, int b, int layer, int n, float* d_dst, void* stream);
+
+/* Causal attention over the 8-bit cache: query token t of sequence b (each of
+ * its n_kv * group heads) sees entries 0 .. entry0[b] + t; tokens
+ * t >= n_rows[b] (when n_rows is given) are skipped and their output rows left
+ * as they were; a row that sees no entry (entry0[b] + t < 0) gives zeros.
+ * q [batch*T][n_kv*group][d] f32; out [batch*T][n_kv*group*d] (out_dtype);
+ * q, out, work 16-byte aligned.
+ * mass [batch][n_kv][capacity] (NULL: not wanted; T * group <= 64): adds to
+ * every seen entry its softmax weights, summed over the call's rows.
+ * Up to 64 query rows (T * group) a row's result does not depend on T or on
+ * the other rows, bit for bit.  split_keys: keys per split, a multiple of 128
+ * up to 8192, or 0 for a rule on (batch, n_kv, capacity).
+ * The work buffer must be zero when first used, is left ready for the next
+ * call, and must not serve two calls that may run at the same time (two
+ * streams, two captured graphs replayed side by side). */
+DKV_API size_t dkv_q8_attn_work_bytes(dkv_dims dims, int group, int T, int capacity, int split_keys, int note_mass);
+DKV_API int dkv_q8_attn(const dkv_q8_cache* cache, dkv_dims dims, int layer, int group, int T, const float* d_q,
+                        const int32_t* d_entry0, const int32_t* d_n_rows, void* d_out, int out_dtype, int split_keys,
+                        float* d_mass, void* d_work, size_t work_bytes, void* stream);
+
+/* Eviction by accumulated attention mass, per (sequence, KV head): of the
+ * n[b] entries of `layer`, min(n, max(budget[b], sink + recent)) stay -- the
+ * first `sink`, the last `recent`, and of the others those left after the
+ * lowest (mass, index) are dropped.  The kept entries, in order, are written to
+ * the pages of out_table [batch][out_pages] (pages that no table row of this
+ * call's cache uses) as an append of their values to empty pages would;
+ * out_pages * page_size must hold them (else fewer stay and 0x400 is recorded).
+ * kept [batch][n_kv][out_pages * page_size]: their entry indices, -1 behind.
+ * mass_out, pos_out [batch][n_kv][capacity]: mass and pos of the kept entries,
+ * 0 and -1 behind (out of place; pos and pos_out may both be NULL). */
+DKV_API int dkv_q8_evict(const dkv_q8_cache* cache, dkv_dims dims, int layer, const int32_t* d_n, const int32_t* d_budget,
+                         int sink, int recent, const float* d_mass, const int32_t* d_pos, const int32_t* d_out_table,
+                         int out_pages, float* d_mass_out, int32_t* d_pos_out, int32_t* d_kept, void* stream);
 
 /* ------------------------------------------------------------ GEMM
  * Y = X W^T for the projections, MLP and head (draftkv/llama.py:187-225,
