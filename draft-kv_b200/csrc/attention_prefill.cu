@@ -36,7 +36,7 @@
 // (error word 0x80); after a failed wait the CTA waits (bounded) for its
 // copies and MMAs in flight before it frees shared and tensor memory.
 #include "attn_common.cuh"
-#include "tcgen05.cuh"
+#include "prefill_common.cuh"
 
 namespace dkv {
 
@@ -69,47 +69,6 @@ DKV_DEV uint32_t pf_pack(float lo, float hi) {
     __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&v);
 }
-DKV_DEV float pf_ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
-    return y;
-}
-DKV_DEV float pf_max3(float a, float b, float c) {
-    float r;
-    asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
-// two fp32 lanes in one 64-bit register, and the sm_100 packed add / subtract
-DKV_DEV uint64_t pf_pack2(float lo, float hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-DKV_DEV void pf_unpack2(uint64_t v, float& lo, float& hi) {
-    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-DKV_DEV uint64_t pf_add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-DKV_DEV uint64_t pf_sub2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("sub.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-DKV_DEV void mbar_arrive(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(bar)) : "memory");
-}
-// D (TMEM) += A (TMEM: row i in lane i, two bf16 a 32-bit column) . B (shared)
-DKV_DEV void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
 template <int D>
 __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_tc_kernel(const __grid_constant__ KvMaps maps, AttnArgs a) {
     using Geo = PfGeo<D>;

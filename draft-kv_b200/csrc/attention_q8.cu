@@ -39,11 +39,6 @@ constexpr int kQdMaxSplit = 8192;      // keys a split may have (page ids and sc
 constexpr float kQdLazy = 8.f;         // growth of the max that forces a rescale (log2 units)
 constexpr int kQdBias = 6;             // probabilities enter as p * 2^6: f16 keeps 2^-30 of the max
 
-DKV_DEV float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
-    return y;
-}
 DKV_DEV uint32_t pack_h2(float lo, float hi) {
     __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&v);
@@ -86,7 +81,7 @@ __global__ void __launch_bounds__(QdGeo<NT, RG>::THREADS, QdGeo<NT, RG>::CTAS) q
     __shared__ int32_t page_s[kQdMaxSplit / 16];
     __shared__ float2 scale_s[kQdMaxSplit / 16];
     __shared__ float ms[RB], ls[RB];
-    __shared__ int is_last, failed;
+    __shared__ int failed;
     const Q8View& v = a.v;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -293,7 +288,7 @@ __global__ void __launch_bounds__(QdGeo<NT, RG>::THREADS, QdGeo<NT, RG>::CTAS) q
 #pragma unroll
                             for (int off = 4; off < 32; off <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, off));
                             const bool up = t > m[nt][c] + kQdLazy;
-                            al[c] = up ? ex2(m[nt][c] - t) : 1.f;
+                            al[c] = up ? q8_ex2(m[nt][c] - t) : 1.f;
                             if (up) m[nt][c] = t;
                             l[nt][c] *= al[c];
                         }
@@ -324,7 +319,7 @@ __global__ void __launch_bounds__(QdGeo<NT, RG>::THREADS, QdGeo<NT, RG>::CTAS) q
                     float p[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        p[e] = sh[nt][e] == -INFINITY ? 0.f : ex2(sh[nt][e] - m[nt][e & 1]);
+                        p[e] = sh[nt][e] == -INFINITY ? 0.f : q8_ex2(sh[nt][e] - m[nt][e & 1]);
                         if (e >= 2) l[nt][e & 1] += p[e - 2] + p[e];
                         p[e] = p[e];
                     }
@@ -416,7 +411,7 @@ __global__ void __launch_bounds__(QdGeo<NT, RG>::THREADS, QdGeo<NT, RG>::CTAS) q
 #pragma unroll
         for (int g = 0; g < kQdKG; ++g) {
             const float mg = mrg[((size_t)g * RB + r) * PS];
-            w[g] = mg == -INFINITY ? 0.f : ex2(mg - M);
+            w[g] = mg == -INFINITY ? 0.f : q8_ex2(mg - M);
             if (w[g] != 0.f) L += mrg[((size_t)g * RB + r) * PS + 1] * w[g];
             mrg[((size_t)g * RB + r) * PS] = w[g];
         }
@@ -429,15 +424,6 @@ __global__ void __launch_bounds__(QdGeo<NT, RG>::THREADS, QdGeo<NT, RG>::CTAS) q
         }
     }
     __syncthreads();
-    auto store = [&](int r, int e, float x0, float x1) {
-        const int gr = rbase + r, t = gr / G;
-        if (t >= n_tok) return;                            // rows behind a sequence's last stay as they were
-        const size_t at = (((size_t)b * a.T + t) * v.n_kv * G + h * G + gr % G) * D + e;
-        if (a.out_dtype == DKV_F32)
-            *reinterpret_cast<float2*>(reinterpret_cast<float*>(a.out) + at) = make_float2(x0, x1);
-        else
-            *reinterpret_cast<__nv_bfloat162*>(reinterpret_cast<uint16_t*>(a.out) + at) = __floats2bfloat162_rn(x0, x1);
-    };
     for (int i = threadIdx.x; i < R * (D / 2); i += Geo::THREADS) {
         const int r = i / (D / 2), e = i % (D / 2) * 2;
         float x0 = 0.f, x1 = 0.f;
@@ -453,67 +439,12 @@ __global__ void __launch_bounds__(QdGeo<NT, RG>::THREADS, QdGeo<NT, RG>::CTAS) q
         }
         if (alone) {
             const float L = ls[r];
-            store(r, e, L == 0.f ? 0.f : x0 / L, L == 0.f ? 0.f : x1 / L);
+            q8_store2<D>(a, b, h, rbase + r, n_tok, e, L == 0.f ? 0.f : x0 / L, L == 0.f ? 0.f : x1 / L);
         } else {
             *reinterpret_cast<float2*>(mypart + (size_t)r * PS + 2 + e) = make_float2(x0, x1);
         }
     }
-    if (!alone) {
-        // the last CTA of the row block to arrive merges the splits in order
-        __threadfence();
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            unsigned* tk = a.tickets + bhr;
-            is_last = atomicAdd(tk, 1u) == (unsigned)(a.n_splits - 1);
-            if (is_last) *tk = 0u;
-        }
-        __syncthreads();
-        if (!is_last) return;
-        __threadfence();
-        const float* parts = a.part + bhr * a.n_splits * (size_t)RB * PS;
-        const int ns = a.n_splits;
-        // per-(row, split) weights in the ring when they fit, else recomputed
-        float* wq = mrg;
-        const bool fit = (size_t)ns * RB * sizeof(float) <= Geo::SMEM;
-        for (int r = threadIdx.x; r < R; r += Geo::THREADS) {
-            float M = -INFINITY, L = 0.f;
-#pragma unroll 8
-            for (int q = 0; q < ns; ++q) M = fmaxf(M, __ldcg(parts + ((size_t)q * RB + r) * PS));
-#pragma unroll 8
-            for (int q = 0; q < ns; ++q) {
-                const float2 ml = __ldcg(reinterpret_cast<const float2*>(parts + ((size_t)q * RB + r) * PS));
-                const float w = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
-                if (w != 0.f) L += ml.y * w;
-                if (fit) wq[(size_t)q * RB + r] = w;
-            }
-            ms[r] = M;
-            ls[r] = L;
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < R * (D / 2); i += Geo::THREADS) {
-            const int r = i / (D / 2), e = i % (D / 2) * 2;
-            const float M = ms[r];
-            float x0 = 0.f, x1 = 0.f;
-#pragma unroll 8
-            for (int q = 0; q < ns; ++q) {
-                const float* at = parts + ((size_t)q * RB + r) * PS;
-                float w;
-                if (fit) {
-                    w = wq[(size_t)q * RB + r];
-                } else {
-                    const float mq = __ldcg(at);
-                    w = mq == -INFINITY ? 0.f : ex2(mq - M);
-                }
-                const float2 y = __ldcg(reinterpret_cast<const float2*>(at + 2 + e));
-                if (w != 0.f) {
-                    x0 += y.x * w;
-                    x1 += y.y * w;
-                }
-            }
-            const float L = ls[r];
-            store(r, e, L == 0.f ? 0.f : x0 / L, L == 0.f ? 0.f : x1 / L);
-        }
-    }
+    if (!alone && !q8_merge_splits<D, RB>(a, bhr, b, h, rbase, R, n_tok, mrg, Geo::SMEM, ms, ls)) return;
     if (a.stats)
         for (int r = threadIdx.x; r < R; r += Geo::THREADS)
             a.stats[((size_t)b * v.n_kv + h) * R_all + rbase + r] =
@@ -542,8 +473,8 @@ __global__ void __launch_bounds__(kMassThreads) q8_mass_kernel(Q8AttnArgs a, flo
     for (int r = 0; r < R; r += 2) {
         const float2 x = __ldcg(reinterpret_cast<const float2*>(sc + r));
         const float2 s0 = st_s[r], s1 = r + 1 < R ? st_s[r + 1] : make_float2(0.f, 0.f);
-        if (s0.y != 0.f && key <= e0 + r / a.group) sum += ex2(x.x - s0.x) * s0.y;
-        if (s1.y != 0.f && key <= e0 + (r + 1) / a.group) sum += ex2(x.y - s1.x) * s1.y;
+        if (s0.y != 0.f && key <= e0 + r / a.group) sum += q8_ex2(x.x - s0.x) * s0.y;
+        if (s1.y != 0.f && key <= e0 + (r + 1) / a.group) sum += q8_ex2(x.y - s1.x) * s1.y;
     }
     mass[bh * a.v.capacity() + key] += sum;
 }
@@ -600,7 +531,8 @@ using namespace dkv;
 extern "C" size_t dkv_q8_attn_work_bytes(dkv_dims dims, int group, int T, int capacity, int split_keys, int note_mass) {
     if (dims.batch < 1 || dims.n_kv < 1 || group < 1 || T < 1 || capacity < 1) return 0;
     const long long R = (long long)T * group;
-    if (R > kQ8MaxRows) return decode_work(dims, (int)std::min(R, 1ll << 30), capacity, pick_split(dims.batch, dims.n_kv, capacity, split_keys), false, nullptr, nullptr);
+    if (R > (1 << 24)) return 0;
+    if (R > kQ8MaxRows) return attn_q8_prefill_work(dims, group, T, capacity);
     return decode_work(dims, (int)R, capacity, pick_split(dims.batch, dims.n_kv, capacity, split_keys), note_mass != 0,
                        nullptr, nullptr);
 }
@@ -632,6 +564,12 @@ extern "C" int dkv_q8_attn(const dkv_q8_cache* cache, dkv_dims dims, int layer, 
     a.err = device_error_word();
     DKV_REQUIRE(a.err, "dkv_q8_attn: device error word unavailable");
     cudaStream_t st = (cudaStream_t)stream;
+    if (R > kQ8MaxRows) {
+        // more rows (a prompt chunk): the tcgen05 kernel, which picks its own splits
+        DKV_REQUIRE(work && work_bytes >= attn_q8_prefill_work(dims, group, T, cap),
+                    "dkv_q8_attn: work buffer of %zu bytes is too small", work_bytes);
+        return attn_q8_prefill(a, dims, work, work_bytes, st);
+    }
     a.split = pick_split(dims.batch, dims.n_kv, cap, split_keys);
     DKV_REQUIRE(work && work_bytes >= decode_work(dims, R, cap, a.split, mass != nullptr, nullptr, nullptr),
                 "dkv_q8_attn: work buffer of %zu bytes is too small", work_bytes);

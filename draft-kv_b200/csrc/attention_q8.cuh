@@ -38,7 +38,89 @@ struct Q8AttnArgs {
     }
 };
 
+DKV_DEV float q8_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Two outputs of query row gr (elements e, e + 1); rows of tokens a sequence
+// does not have stay as they were.
+template <int D>
+DKV_DEV void q8_store2(const Q8AttnArgs& a, int b, int h, int gr, int n_tok, int e, float x0, float x1) {
+    const int t = gr / a.group;
+    if (t >= n_tok) return;
+    const size_t at = (((size_t)b * a.T + t) * a.v.n_kv * a.group + h * a.group + gr % a.group) * D + e;
+    if (a.out_dtype == DKV_F32)
+        *reinterpret_cast<float2*>(reinterpret_cast<float*>(a.out) + at) = make_float2(x0, x1);
+    else
+        *reinterpret_cast<__nv_bfloat162*>(reinterpret_cast<uint16_t*>(a.out) + at) = __floats2bfloat162_rn(x0, x1);
+}
+
+// After a CTA has stored its split's partial rows (max in log2 units, sum,
+// unnormalised O) of row block `bhr`, the last CTA to arrive merges all splits
+// in split order (empty ones skipped), writes the outputs and returns true
+// with the merged max / sum in ms / ls.  wq: shared memory the caller no longer
+// needs, for the per-(split, row) weights when they fit.
+template <int D, int RB>
+DKV_DEV bool q8_merge_splits(const Q8AttnArgs& a, size_t bhr, int b, int h, int rbase, int R, int n_tok, float* wq,
+                             size_t wq_bytes, float* ms, float* ls) {
+    constexpr int PS = D + 2;
+    __shared__ int is_last;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        unsigned* tk = a.tickets + bhr;
+        is_last = atomicAdd(tk, 1u) == (unsigned)(a.n_splits - 1);
+        if (is_last) *tk = 0u;
+    }
+    __syncthreads();
+    if (!is_last) return false;
+    __threadfence();
+    const int ns = a.n_splits;
+    const float* parts = a.part + bhr * ns * (size_t)RB * PS;
+    const bool fit = (size_t)ns * RB * sizeof(float) <= wq_bytes;
+    for (int r = threadIdx.x; r < R; r += blockDim.x) {
+        float M = -INFINITY, L = 0.f;
+#pragma unroll 8
+        for (int q = 0; q < ns; ++q) M = fmaxf(M, __ldcg(parts + ((size_t)q * RB + r) * PS));
+#pragma unroll 8
+        for (int q = 0; q < ns; ++q) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(parts + ((size_t)q * RB + r) * PS));
+            const float w = ml.x == -INFINITY ? 0.f : q8_ex2(ml.x - M);
+            if (w != 0.f) L += ml.y * w;
+            if (fit) wq[(size_t)q * RB + r] = w;
+        }
+        ms[r] = M;
+        ls[r] = L;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < R * (D / 2); i += blockDim.x) {
+        const int r = i / (D / 2), e = i % (D / 2) * 2;
+        const float M = ms[r];
+        float x0 = 0.f, x1 = 0.f;
+#pragma unroll 8
+        for (int q = 0; q < ns; ++q) {
+            const float* at = parts + ((size_t)q * RB + r) * PS;
+            float w;
+            if (fit) {
+                w = wq[(size_t)q * RB + r];
+            } else {
+                const float mq = __ldcg(at);
+                w = mq == -INFINITY ? 0.f : q8_ex2(mq - M);
+            }
+            if (w == 0.f) continue;      // an empty split has no O
+            const float2 y = __ldcg(reinterpret_cast<const float2*>(at + 2 + e));
+            x0 += y.x * w;
+            x1 += y.y * w;
+        }
+        const float L = ls[r];
+        q8_store2<D>(a, b, h, rbase + r, n_tok, e, L == 0.f ? 0.f : x0 / L, L == 0.f ? 0.f : x1 / L);
+    }
+    return true;
+}
+
 int attn_q8_prefill(Q8AttnArgs& a, dkv_dims dims, void* work, size_t work_bytes, cudaStream_t st);
-size_t attn_q8_prefill_work(dkv_dims dims, int group, int T, int capacity, int split_keys);
+size_t attn_q8_prefill_work(dkv_dims dims, int group, int T, int capacity);
 
 }  // namespace dkv

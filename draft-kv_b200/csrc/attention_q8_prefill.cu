@@ -1,0 +1,542 @@
+// Prompt attention over the 8-bit paged cache on the fifth-generation tensor
+// cores: more than 64 query rows (token x GQA head) a KV head.
+//
+// Flash attention as in the bf16 prefill kernel (two 128-row query tiles a CTA
+// alternate on the tensor core; Q and K in shared memory, S, P and O in tensor
+// memory), with the cache's codes turned into f16 operands on the way:
+//   warps 8-11 -- converters: a 128-key tile's codes come from global memory
+//     straight into registers, one tile ahead (16-byte fragments, 512 B a warp
+//     and load), are widened e4m3 -> f16 (exact), multiplied by a power of two
+//     and stored in the swizzled K-major layout the MMA reads.  V's bytes are
+//     already dim-major, so V^T needs no transpose.  2 x 32 KB K and V rings;
+//   warp 12 -- tensor memory, and lane 0 issues the MMAs: per key tile j and
+//     query tile t, O_t += P_t(j-1) V(j-1), then S_t(j) = Q_t K_j^T;
+//   warps 0-3 / 4-7 -- softmax of query tiles A / B, one row a thread.
+// Rounding: the block scales are powers of two, so an operand is exactly
+// code * 2^(e - e_max + 6) with e_max the largest block exponent of the CTA's
+// key range (values 2^-30 below the range's largest go to zero); queries are
+// one f16 number each (2^-12 of the row's largest), probabilities too, biased
+// by 2^6 so that f16 keeps 2^-30 of the max; max, sum and O are fp32.
+// Bound by the tensor cores and the softmax warps: 4 * 128 * 128 * d MACs a
+// key tile against 128 * 2 d bytes.
+// Every mbarrier wait is bounded (error word 0x80).
+#include <algorithm>
+
+#include "attention_q8.cuh"
+#include "prefill_common.cuh"
+
+namespace dkv {
+
+namespace {
+
+constexpr int kQpTile = 128, kQpRows = 256, kQpKeys = 128;
+constexpr int kQpSoft = 256, kQpConv = 128;
+constexpr int kQpThreads = kQpSoft + kQpConv + 32;
+constexpr int kQpNst = 2;               // K and V ring depth
+constexpr int kQpTmemCols = 512;        // per query tile t: S at 256 t (P over it), O at 256 t + 128
+constexpr int kQpSplit = 16384;         // most keys a split has (page ids staged in shared memory)
+constexpr int kQpMinSplit = 2048;
+constexpr float kQpLazy = 8.f;
+constexpr int kQpBias = 6;
+
+template <int D>
+struct QpGeo {
+    static constexpr int CH = D / 64;
+    static constexpr int QT = CH * 16384;        // one query tile
+    static constexpr int KVB = kQpKeys * D * 2;  // one K (or V) tile
+    static constexpr int K0 = 2 * QT, V0 = K0 + kQpNst * KVB;
+    static constexpr size_t SMEM = (size_t)V0 + kQpNst * KVB + 1024;
+};
+
+// kind::f16 instruction descriptor: f16 A and B, f32 D, K-major both, M 128.
+__host__ __device__ constexpr uint32_t qp_idesc(int n) {
+    return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+DKV_DEV uint32_t h2(float lo, float hi) {
+    __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+}
+DKV_DEV uint32_t hmul2(uint32_t a, uint32_t b) {
+    __half2 r = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<uint32_t*>(&r);
+}
+// 2^e twice as f16 (0 below 2^-24), e <= 15
+DKV_DEV uint32_t h2_pow2(int e) {
+    const float f = e < -24 ? 0.f : q8_pow2(e);
+    return h2(f, f);
+}
+
+template <int D>
+__global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_constant__ Q8AttnArgs a) {
+    using Geo = QpGeo<D>;
+    constexpr int PS = D + 2;
+    extern __shared__ uint8_t qp_raw[];
+    uint8_t* sm = qp_raw + ((1024u - (smem_u32(qp_raw) & 1023u)) & 1023u);
+    __shared__ __align__(8) uint64_t k_full[kQpNst], k_empty[kQpNst], v_full[kQpNst], v_empty[kQpNst];
+    __shared__ __align__(8) uint64_t s_full[2], p_full[2], o_done, drain;
+    __shared__ uint32_t tmem_slot;
+    __shared__ float ms[kQpRows], ls[kQpRows];
+    __shared__ int32_t page_s[kQpSplit / 16];
+    __shared__ int8_t ek_s[kQpSplit / 16], ev_s[kQpSplit / 16];      // block exponents
+    __shared__ uint32_t bad_s[kQpSplit / kQpKeys / 4];               // 8 bits a key tile: 16-key groups not to be seen
+    __shared__ int emax_s[2];
+
+    const Q8View& v = a.v;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // row block fastest: the row blocks of a (sequence, head, split) run
+    // together and read the same codes through L2
+    const int rb = (int)(blockIdx.x % a.n_rb);
+    const int s = (int)(blockIdx.x / a.n_rb % a.n_splits);
+    const int h = (int)(blockIdx.x / a.n_rb / a.n_splits % v.n_kv);
+    const int b = (int)(blockIdx.x / a.n_rb / a.n_splits / v.n_kv);
+    const int G = a.group;
+    const int r0 = rb * kQpRows, R = min(kQpRows, a.T * G - r0);
+    const size_t bhr = ((size_t)b * v.n_kv + h) * a.n_rb + rb;
+    const bool alone = a.n_splits == 1;
+    constexpr size_t kWq = (size_t)Geo::V0 + kQpNst * Geo::KVB;
+
+    pdl_trigger();
+    pdl_wait();
+    const int e0 = a.entry0[b];
+    const int n_tok = a.n_rows ? min(a.n_rows[b], a.T) : a.T;
+    const int t_last = min((r0 + R - 1) / G, n_tok - 1);
+    const int n_keys = t_last >= r0 / G ? max(0, min(a.n_keys(b), e0 + t_last + 1)) : 0;
+    const int k0 = s * a.split;                               // a multiple of 128
+    const int kend = min(n_keys, k0 + a.split);
+    const int ntiles = kend > k0 ? (kend - k0 + kQpKeys - 1) / kQpKeys : 0;
+    if (s == 0 && h == 0 && rb == 0 && threadIdx.x == 0 && a.beyond(b)) atomicOr(a.err, kErrQ8Page);
+    if (ntiles == 0) {
+        if (alone) {
+            for (int i = threadIdx.x; i < R * (D / 2); i += kQpThreads)
+                q8_store2<D>(a, b, h, r0 + i / (D / 2), n_tok, i % (D / 2) * 2, 0.f, 0.f);
+            return;
+        }
+        for (int r = threadIdx.x; r < R; r += kQpThreads)
+            *reinterpret_cast<float2*>(a.part + ((bhr * a.n_splits + s) * kQpRows + r) * PS) = make_float2(-INFINITY, 0.f);
+        q8_merge_splits<D, kQpRows>(a, bhr, b, h, r0, R, n_tok, reinterpret_cast<float*>(sm), kWq, ms, ls);
+        return;
+    }
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kQpNst; ++i) {
+            mbar_init(&k_full[i], kQpConv);
+            mbar_init(&k_empty[i], 1);
+            mbar_init(&v_full[i], kQpConv);
+            mbar_init(&v_empty[i], 1);
+        }
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&s_full[t], 1);
+            mbar_init(&p_full[t], 128);
+        }
+        mbar_init(&o_done, 1);
+        mbar_init(&drain, 1);
+        fence_barrier_init();
+        fence_async_shared();
+        emax_s[0] = emax_s[1] = kQ8ExpMin;
+    }
+    for (int i = threadIdx.x; i < (ntiles + 3) / 4; i += kQpThreads) bad_s[i] = 0u;
+    if (warp == 12) tmem_alloc(&tmem_slot, kQpTmemCols);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    // page ids and exponents of the key range; keys of a bad page are not seen
+    const int n_pg = (kend - k0 + v.page - 1) >> v.page_shift;
+    for (int i = threadIdx.x; i < n_pg; i += kQpThreads) {
+        const int pid = __ldg(v.row(b) + (k0 >> v.page_shift) + i);
+        const bool ok = v.ok(pid);
+        page_s[i] = ok ? pid : -1;
+        int ek = kQ8ExpMin, ev = kQ8ExpMin;
+        if (ok) {
+            const float2 sc = *reinterpret_cast<const float2*>(v.scale + v.scale_at(pid, h, 0));
+            ek = min(max(q8_scale_exp(sc.x), kQ8ExpMin), kQ8ExpMax);
+            ev = min(max(q8_scale_exp(sc.y), kQ8ExpMin), kQ8ExpMax);
+        } else {
+            atomicOr(a.err, kErrQ8Page);
+            for (int g = 0; g < v.page / 16; ++g) {
+                const int grp = i * (v.page / 16) + g;
+                if (grp < ntiles * 8) atomicOr(&bad_s[grp >> 5], 1u << (grp & 31));
+            }
+        }
+        ek_s[i] = (int8_t)ek;
+        ev_s[i] = (int8_t)ev;
+        atomicMax(&emax_s[0], ek);
+        atomicMax(&emax_s[1], ev);
+    }
+    __syncthreads();
+    const int ekm = emax_s[0], evm = emax_s[1];
+
+    bool ok = true;
+    if (warp >= 8 && warp < 12) {
+        // ---------------- converters.  Warp w takes 8 of the 32 (or 16) 512-byte
+        // K blocks of a tile, and of V: block x = group x / (D / 32), dims 32 (x % (D / 32)) ..
+        constexpr int NJ = D / 32, NB = 8 * NJ / 4;               // blocks a warp
+        const int w = warp - 8, g = lane >> 2, t = lane & 3;
+        uint4 kr[NB], vr[NB];
+        auto page_of = [&](int j, int grp) { return ((j * kQpKeys + grp * 16) >> v.page_shift); };
+        auto load = [&](int j, int i, uint4 (&r)[NB]) {
+#pragma unroll
+            for (int u = 0; u < NB; ++u) {
+                const int x = w * NB + u, grp = x / NJ, blk = x % NJ;
+                const int key = j * kQpKeys + grp * 16;           // from k0
+                r[u] = make_uint4(0u, 0u, 0u, 0u);
+                if (j < ntiles && k0 + key < kend) {
+                    const int pid = page_s[page_of(j, grp)];
+                    if (pid >= 0)
+                        r[u] = __ldg(reinterpret_cast<const uint4*>(v.side(pid, h, i) +
+                                                                    (size_t)((k0 + key) & (v.page - 1)) * D + blk * 512 +
+                                                                    lane * 16));
+                }
+            }
+        };
+        // K: word q of a fragment is token g + 8 (q & 1), dims 32 blk + 16 (q >> 1) + {2t, 2t+1 | 2t+8, 2t+9}
+        auto put_k = [&](int j, uint8_t* dst) {
+#pragma unroll
+            for (int u = 0; u < NB; ++u) {
+                const int x = w * NB + u, grp = x / NJ, blk = x % NJ;
+                const int key = j * kQpKeys + grp * 16;
+                const uint32_t f = k0 + key < kend ? h2_pow2(ek_s[page_of(j, grp)] - ekm + kQpBias) : 0u;
+                const uint32_t ws[4] = {kr[u].x, kr[u].y, kr[u].z, kr[u].w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t lo, hi;
+                    q8_decode4(ws[q], lo, hi);
+                    const int row = grp * 16 + g + 8 * (q & 1);
+                    const int unit = (blk * 4 + (q >> 1) * 2) & 7;
+                    uint8_t* at = dst + (blk >> 1) * 16384 + row * 128 + 4 * t;
+                    *reinterpret_cast<uint32_t*>(at + ((unit ^ (row & 7)) << 4)) = hmul2(lo, f);
+                    *reinterpret_cast<uint32_t*>(at + (((unit + 1) ^ (row & 7)) << 4)) = hmul2(hi, f);
+                }
+            }
+        };
+        // V: word q is dim 32 blk + 16 (q >> 1) + 8 (q & 1) + g, tokens {2t, 2t+1 | 2t+8, 2t+9}
+        auto put_v = [&](int j, uint8_t* dst) {
+#pragma unroll
+            for (int u = 0; u < NB; ++u) {
+                const int x = w * NB + u, grp = x / NJ, blk = x % NJ;
+                const int key = j * kQpKeys + grp * 16, left = kend - k0 - key;      // live tokens of the group
+                const uint32_t f = left > 0 ? h2_pow2(ev_s[page_of(j, grp)] - evm + kQpBias) : 0u;
+                // bytes of tokens that are not there as zeros (their weight is 0, but 0 x NaN would not be)
+                uint32_t vm = 0xffffffffu;
+                if (left < 16)
+                    vm = (2 * t < left ? 0xffu : 0u) | (2 * t + 1 < left ? 0xff00u : 0u) |
+                         (2 * t + 8 < left ? 0xff0000u : 0u) | (2 * t + 9 < left ? 0xff000000u : 0u);
+                const uint32_t ws[4] = {vr[u].x, vr[u].y, vr[u].z, vr[u].w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t lo, hi;
+                    q8_decode4(ws[q] & vm, lo, hi);
+                    const int row = blk * 32 + (q >> 1) * 16 + (q & 1) * 8 + g;
+                    const int unit = (grp * 2) & 7;
+                    uint8_t* at = dst + (grp >> 2) * (D * 128) + row * 128 + 4 * t;
+                    *reinterpret_cast<uint32_t*>(at + ((unit ^ (row & 7)) << 4)) = hmul2(lo, f);
+                    *reinterpret_cast<uint32_t*>(at + (((unit + 1) ^ (row & 7)) << 4)) = hmul2(hi, f);
+                }
+            }
+        };
+        load(0, 0, kr);
+        load(0, 1, vr);
+        for (int j = 0; j < ntiles; ++j) {
+            const int slot = j % kQpNst;
+            const uint32_t ph = (uint32_t)((j / kQpNst - 1) & 1);
+            // the slot's K was read by S_A(j-2), S_B(j-2); its V by the P V products of tile j - 2
+            if (j >= kQpNst && !__all_sync(0xffffffffu, mbar_wait(&k_empty[slot], ph, a.err))) {
+                ok = false;
+                break;
+            }
+            put_k(j, sm + Geo::K0 + slot * Geo::KVB);
+            fence_async_shared();
+            mbar_arrive(&k_full[slot]);
+            load(j + 1, 0, kr);
+            if (j >= kQpNst && !__all_sync(0xffffffffu, mbar_wait(&v_empty[slot], ph, a.err))) {
+                ok = false;
+                break;
+            }
+            put_v(j, sm + Geo::V0 + slot * Geo::KVB);
+            fence_async_shared();
+            mbar_arrive(&v_full[slot]);
+            load(j + 1, 1, vr);
+        }
+    } else if (warp == 12) {
+        // ---------------- MMA issuer (the warp waits together, lane 0 issues)
+        const uint32_t q_s = smem_u32(sm), k_s0 = smem_u32(sm + Geo::K0), v_s0 = smem_u32(sm + Geo::V0);
+        constexpr uint32_t idS = qp_idesc(kQpKeys), idO = qp_idesc(D);
+        auto wait_all = [&](uint64_t* bar, uint32_t parity) {
+            return __all_sync(0xffffffffu, mbar_wait(bar, parity, a.err));
+        };
+        auto issue_pv = [&](int t, int i) {
+            const uint32_t v_s = v_s0 + (i % kQpNst) * Geo::KVB;
+            const uint32_t base = tmem + (uint32_t)(t * 256);
+#pragma unroll
+            for (int ks = 0; ks < kQpKeys / 16; ++ks)
+                tc_mma_ts(base + 128, base + ks * 8, sw128_desc(v_s + (ks >> 2) * (D * 128) + (ks & 3) * 32), idO,
+                          (i | ks) != 0 ? 1u : 0u);
+        };
+        auto issue_s = [&](int t, int j) {
+            const uint32_t k_s = k_s0 + (j % kQpNst) * Geo::KVB;
+            const uint32_t qt = q_s + t * Geo::QT;
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk)
+                tc_mma_i(tmem + (uint32_t)(t * 256), sw128_desc(qt + (kk >> 2) * 16384 + (kk & 3) * 32),
+                         sw128_desc(k_s + (kk >> 2) * 16384 + (kk & 3) * 32), idS, kk != 0 ? 1u : 0u);
+            tc_commit(&s_full[t]);
+        };
+        named_sync(1, kQpSoft + 32);      // Q is in shared memory
+        for (int j = 0; j < ntiles && ok; ++j) {
+            if (!wait_all(&k_full[j % kQpNst], (uint32_t)((j / kQpNst) & 1)) ||
+                (j >= 1 && !wait_all(&v_full[(j - 1) % kQpNst], (uint32_t)(((j - 1) / kQpNst) & 1)))) {
+                ok = false;
+                break;
+            }
+            for (int t = 0; t < 2; ++t) {
+                if (j >= 1 && !wait_all(&p_full[t], (uint32_t)((j - 1) & 1))) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                if (lane == 0) {
+                    if (j >= 1) issue_pv(t, j - 1);
+                    issue_s(t, j);
+                }
+                __syncwarp();
+            }
+            if (!ok) break;
+            if (lane == 0) {
+                tc_commit(&k_empty[j % kQpNst]);
+                if (j >= 1) tc_commit(&v_empty[(j - 1) % kQpNst]);
+            }
+            __syncwarp();
+        }
+        if (ok) {
+            const int i = ntiles - 1;
+            ok = wait_all(&v_full[i % kQpNst], (uint32_t)((i / kQpNst) & 1));
+            for (int t = 0; t < 2 && ok; ++t) {
+                if (!wait_all(&p_full[t], (uint32_t)(i & 1))) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                if (lane == 0) issue_pv(t, i);
+                __syncwarp();
+            }
+            if (ok && lane == 0) tc_commit(&o_done);
+            __syncwarp();
+        }
+    } else {
+        // ---------------- softmax: row rt of query tile t = TMEM lane rt; CTA row cr
+        const int t = warp >> 2, rt = threadIdx.x & 127, cr = t * kQpTile + rt, gr = r0 + cr;
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t sb = lanes + (uint32_t)(t * 256), ob = sb + 128;
+        const bool mine = cr < R && gr / G < n_tok;
+        float c;                                                  // scores = S * c (log2 units)
+        {
+            // the row of Q as f16 of q * log2 e / sqrt(d) * 2^-x, x the row's exponent
+            const float* qrow =
+                mine ? a.q + (((size_t)b * a.T + gr / G) * v.n_kv * G + h * G + gr % G) * D : nullptr;
+            float am = 0.f;
+            if (qrow)
+#pragma unroll 8
+                for (int u = 0; u < D / 4; ++u) {
+                    const float4 x = __ldg(reinterpret_cast<const float4*>(qrow + 4 * u));
+                    am = fmaxf(fmaxf(am, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
+                }
+            const int ex = min(max((int)(__float_as_uint(am * a.scale) >> 23) - 127, -100), 126);
+            const float f = a.scale * q8_pow2(-ex);
+            c = q8_pow2(min(max(ex + ekm - kQpBias, -126), 127));
+            uint8_t* qt = sm + t * Geo::QT;
+#pragma unroll 4
+            for (int u = 0; u < D / 8; ++u) {
+                float4 x0 = make_float4(0.f, 0.f, 0.f, 0.f), x1 = x0;
+                if (qrow) {
+                    x0 = __ldg(reinterpret_cast<const float4*>(qrow + 8 * u));
+                    x1 = __ldg(reinterpret_cast<const float4*>(qrow + 8 * u + 4));
+                }
+                *reinterpret_cast<uint4*>(qt + (u >> 3) * 16384 + rt * 128 + (((u & 7) ^ (rt & 7)) << 4)) =
+                    make_uint4(h2(x0.x * f, x0.y * f), h2(x0.z * f, x0.w * f), h2(x1.x * f, x1.y * f),
+                               h2(x1.z * f, x1.w * f));
+            }
+            fence_async_shared();
+            named_sync(1, kQpSoft + 32);
+        }
+        // this row's last key; rows that are not there see every key
+        const int lim = mine ? min(e0 + gr / G, kend - 1) : kend - 1;
+        float m = -INFINITY, l = 0.f;
+        for (int j = 0; j < ntiles; ++j) {
+            if (!__all_sync(0xffffffffu, mbar_wait(&s_full[t], (uint32_t)(j & 1), a.err))) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const int lc = lim - (k0 + j * kQpKeys);              // last live column
+            const uint32_t bad = (bad_s[j >> 2] >> ((j & 3) * 8)) & 0xffu;
+            const bool masked = lc < kQpKeys - 1 || bad != 0u;
+            auto mask = [&](int col, uint32_t& x) {
+                if (col > lc || ((bad >> (col >> 4)) & 1u)) x = __float_as_uint(-INFINITY);
+            };
+            float mx[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) mx[k] = -INFINITY;
+#pragma unroll
+            for (int cc = 0; cc < 4; ++cc) {
+                uint32_t sr[32];
+                tmem_ld32(sb + cc * 32, sr);
+                tmem_wait_ld();
+                if (masked) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) mask(cc * 32 + e, sr[e]);
+                }
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                    const int k = 2 * cc + (e >> 4);
+                    mx[k] = pf_max3(mx[k], __uint_as_float(sr[e]), __uint_as_float(sr[e + 1]));
+                }
+            }
+            const float mn = c * pf_max3(pf_max3(mx[0], mx[1], mx[2]), pf_max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7]));
+            float alpha = 1.f;
+            if (mn > m + kQpLazy) {
+                alpha = pf_ex2(m - mn);                           // 0 from -infinity
+                m = mn;
+            }
+            const float off = m == -INFINITY ? 0.f : (float)kQpBias - m;
+            const uint64_t cc2 = pf_pack2(c, c), oo = pf_pack2(off, off);
+            uint64_t sum2[2] = {0ull, 0ull};
+            uint32_t sr[2][32];
+#pragma unroll 1
+            for (int k = 0; k < 2; ++k) {
+                tmem_ld32(sb + 64 * k, sr[0]);
+                tmem_ld32(sb + 64 * k + 32, sr[1]);
+                tmem_wait_ld();
+                uint32_t pk[32];
+#pragma unroll
+                for (int h3 = 0; h3 < 2; ++h3) {
+                    if (masked) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) mask((2 * k + h3) * 32 + e, sr[h3][e]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        float d0, d1;
+                        pf_unpack2(pf_fma2(pf_pack2(__uint_as_float(sr[h3][e]), __uint_as_float(sr[h3][e + 1])), cc2, oo),
+                                   d0, d1);
+                        const float p0 = pf_ex2(d0), p1 = pf_ex2(d1);
+                        sum2[h3] = pf_add2(sum2[h3], pf_pack2(p0, p1));
+                        pk[h3 * 16 + e / 2] = h2(p0, p1);
+                    }
+                }
+                tmem_st32(sb + 32 * k, pk);
+            }
+            float a0, a1, a2, a3;
+            pf_unpack2(sum2[0], a0, a1);
+            pf_unpack2(sum2[1], a2, a3);
+            l = l * alpha + ((a0 + a1) + (a2 + a3));
+            if (j >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll 1
+                for (int c0 = 0; c0 < D; c0 += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(ob + c0, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                    tmem_st32(ob + c0, o);
+                }
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&p_full[t]);
+        }
+        if (ok) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&o_done, 0u, a.err));
+            tc_fence_after();
+        }
+        // ---- the row's output (one split) or its partial (max, sum, O)
+        float* mypart = alone ? nullptr : a.part + ((bhr * a.n_splits + s) * kQpRows + cr) * PS;
+        if (l != l && m == -INFINITY) m = 0.f;     // NaN scores have no max: give the row one, so that its NaN comes out
+        const bool live = ok && m != -INFINITY;
+        // O holds code * 2^(kQpBias - evm) units, l the probabilities' 2^kQpBias
+        const float un = q8_pow2(evm) * q8_pow2(-kQpBias);
+        const float f = alone ? (live ? un / l : 0.f) : un * q8_pow2(-kQpBias);
+        if (__all_sync(0xffffffffu, ok)) {
+#pragma unroll 1
+            for (int c0 = 0; c0 < D; c0 += 32) {
+                uint32_t o[32];
+                tmem_ld32(ob + c0, o);
+                tmem_wait_ld();
+                if (!mine) continue;
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                    const float x0 = live ? __uint_as_float(o[e]) * f : 0.f, x1 = live ? __uint_as_float(o[e + 1]) * f : 0.f;
+                    if (alone)
+                        q8_store2<D>(a, b, h, gr, n_tok, c0 + e, x0, x1);
+                    else if (live)
+                        *reinterpret_cast<float2*>(mypart + 2 + c0 + e) = make_float2(x0, x1);
+                }
+            }
+        }
+        if (!alone && cr < R)
+            *reinterpret_cast<float2*>(mypart) = make_float2(live ? m : -INFINITY, live ? l * q8_pow2(-kQpBias) : 0.f);
+    }
+
+    const bool all_ok = __syncthreads_and(ok) != 0;
+    if (!all_ok && warp == 12 && lane == 0) {
+        // a wait ran out: the MMAs still in flight end before the memory is let go
+        tc_commit(&drain);
+        mbar_wait(&drain, 0u, nullptr);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        tc_fence_after();
+        tmem_dealloc(tmem, kQpTmemCols);
+    }
+    if (!alone) q8_merge_splits<D, kQpRows>(a, bhr, b, h, r0, R, n_tok, reinterpret_cast<float*>(sm), all_ok ? kWq : 0, ms, ls);
+}
+
+// Keys per split: the whole capacity up to 16384 keys; where the row blocks
+// alone leave SMs idle, as many splits of at least 2048 keys as fill them.
+int prefill_split(dkv_dims dims, int n_rb, int capacity) {
+    const long long ctas = (long long)dims.batch * dims.n_kv * n_rb;
+    const int most = std::max(1, (capacity + kQpMinSplit - 1) / kQpMinSplit);
+    const int want = std::max((capacity + kQpSplit - 1) / kQpSplit, (int)std::min<long long>(most, std::max(1ll, 148 / ctas)));
+    const int keys = (capacity + want - 1) / want;
+    return std::min((keys + kQpKeys - 1) / kQpKeys * kQpKeys, kQpSplit);
+}
+
+size_t prefill_layout(dkv_dims dims, int group, int T, int capacity, Q8AttnArgs* a, Arena* ar) {
+    const int R = T * group, n_rb = (R + kQpRows - 1) / kQpRows;
+    const int split = prefill_split(dims, n_rb, capacity), ns = std::max(1, (capacity + split - 1) / split);
+    const size_t part = ns == 1 ? 0 : (size_t)dims.batch * dims.n_kv * n_rb * ns * kQpRows * (dims.d + 2);
+    if (a) {
+        a->split = split;
+        a->n_splits = ns;
+        a->n_rb = n_rb;
+        a->tickets = ar->take<unsigned>(kQ8Tickets);
+        a->part = ar->take<float>(part);
+    }
+    return kQ8Tickets * sizeof(unsigned) + align_up(part * sizeof(float), 256) + 1024;
+}
+
+}  // namespace
+
+size_t attn_q8_prefill_work(dkv_dims dims, int group, int T, int capacity) {
+    return prefill_layout(dims, group, T, capacity, nullptr, nullptr);
+}
+
+int attn_q8_prefill(Q8AttnArgs& a, dkv_dims dims, void* work, size_t work_bytes, cudaStream_t st) {
+    Arena ar(work, work_bytes);
+    prefill_layout(dims, a.group, a.T, a.v.capacity(), &a, &ar);
+    DKV_REQUIRE(a.tickets && a.part, "dkv_q8_attn: work buffer");
+    const size_t n_tk = (size_t)dims.batch * dims.n_kv * a.n_rb;
+    DKV_REQUIRE(n_tk <= kQ8Tickets && n_tk * a.n_splits <= 0x7fffffffu, "dkv_q8_attn: batch x heads x row blocks too large");
+    ProfScope ps(DKV_PROF_ATTN_FULL, 0.0, st);
+    const dim3 grid((unsigned)(n_tk * a.n_splits));
+    if (dims.d == 128) {
+        DKV_CUDA(allow_smem_max_once<q8_prefill_kernel<128>>());
+        DKV_CUDA(launch_pdl(q8_prefill_kernel<128>, grid, dim3(kQpThreads), QpGeo<128>::SMEM, st, a));
+    } else {
+        DKV_CUDA(allow_smem_max_once<q8_prefill_kernel<64>>());
+        DKV_CUDA(launch_pdl(q8_prefill_kernel<64>, grid, dim3(kQpThreads), QpGeo<64>::SMEM, st, a));
+    }
+    return DKV_OK;
+}
+
+}  // namespace dkv

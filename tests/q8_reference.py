@@ -133,3 +133,12 @@ def attention_tolerance(d, n, bound, vmax, out_eps):
     numbers (2^-22).  Then one rounding to the output type."""
     delta = (d + 8) * 2.0 ** -23 * bound + 2.0 ** -20
     return out_eps / 2, 2 * vmax * (delta + (n / 16 + 128) * 2.0 ** -23)
+
+
+def prompt_tolerance(d, n, bound, vmax, out_eps):
+    """The same for more than 64 rows: queries are one f16 number (2^-11 of a
+    value, at least 2^-25 of the row's largest: bound * 2^-11 covers both),
+    probabilities too (2^-11 of the numerator's terms, and 2^-31 of the max
+    for each key)."""
+    rel, ab = attention_tolerance(d, n, bound, vmax, out_eps)
+    return rel, ab + 2 * vmax * (2.0 ** -11 * bound) + vmax * (2.0 ** -11 + n * 2.0 ** -31)

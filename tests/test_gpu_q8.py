@@ -212,7 +212,9 @@ def check_attention(mk, r, q, entry0, layer=0, n_rows=None, out_dtype=torch.bflo
     n = max(max(entry0) + q.shape[1], 1)
     vmax = max([1e-30] + [np.abs(r.entries(b, layer, h, entry0[b] + q.shape[1])[1]).max() for b in range(mk.batch)
                           for h in range(mk.kv) if entry0[b] + q.shape[1] > 0])
-    rel, ab = ref.attention_tolerance(mk.d, n, bound, vmax, torch.finfo(out_dtype).eps)
+    rows = q.shape[1] * q.shape[2] // mk.kv
+    rel, ab = (ref.attention_tolerance if rows <= 64 else ref.prompt_tolerance)(mk.d, n, bound, vmax,
+                                                                              torch.finfo(out_dtype).eps)
     got = out.double().cpu().numpy()
     live = ~np.isnan(want)
     assert np.isfinite(got[live]).all()
@@ -363,6 +365,101 @@ def test_bad_pages_and_entries_beyond_the_capacity():
     assert device_error() == 0x400
     mk.cache.attention(0, torch.from_numpy(q).cuda(), i32([2 ** 31 - 1]))
     assert device_error() == 0x400
+
+
+# ------------------------------------------------------------ prompt chunks
+PROMPTS = [   # batch, kv, group, d, page, pages, T, entries before the call
+    (1, 1, 1, 64, 16, 5, 65, [0]), (2, 2, 4, 128, 16, 20, 17, [300, 0]), (1, 2, 1, 64, 32, 10, 301, [3]),
+    (2, 1, 3, 128, 64, 6, 100, [250, 7]), (1, 1, 8, 128, 128, 4, 70, [400]), (3, 1, 2, 64, 16, 40, 129, [500, 128, 1]),
+    (1, 1, 5, 64, 16, 9, 13, [127]),
+]
+
+
+@pytest.mark.parametrize("shape", PROMPTS, ids=lambda s: f"b{s[0]}kv{s[1]}g{s[2]}d{s[3]}p{s[4]}T{s[6]}")
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
+def test_prompt_attention_matches_the_definition(shape, out_dtype):
+    batch, kv, group, d, page, pages, T, e0 = shape
+    mk = Made(batch, 2, kv, d, page, pages, seed=T)
+    rng = np.random.default_rng(d + T)
+    r = mk.fill([x + T for x in e0], rng, layer=1, spread=0.7)
+    q = (rng.standard_normal((batch, T, kv * group, d)) * 1.5).astype(np.float32)
+    check_attention(mk, r, q, e0, layer=1, out_dtype=out_dtype)
+
+
+@pytest.mark.parametrize("d,page", [(128, 16), (64, 128)])
+def test_prompt_attention_over_key_splits(d, page):
+    """A capacity of several splits, of which the sequence fills the first two and a bit."""
+    mk = Made(1, 1, 1, d, page, 40960 // page, seed=2)
+    rng = np.random.default_rng(d)
+    T, e0 = 70, 5000
+    r = mk.fill([e0 + T], rng, spread=0.5)
+    q = rng.standard_normal((1, T, 2, d)).astype(np.float32)
+    check_attention(mk, r, q, [e0])
+    r0 = mk.cache.attention(0, torch.from_numpy(q).cuda(), i32([-T]))
+    assert (r0 == 0).all()
+
+
+def test_prompt_rows_that_see_nothing_or_are_not_there():
+    mk = Made(2, 1, 1, 64, 16, 30, seed=9)
+    rng = np.random.default_rng(5)
+    r = mk.fill([150, 200], rng)
+    q = rng.standard_normal((2, 90, 2, 64)).astype(np.float32)
+    check_attention(mk, r, q, [-30, 100], n_rows=[90, 41])
+    out = torch.full((2, 90, 2, 64), 5.0, dtype=torch.bfloat16, device="cuda")
+    mk.cache.attention(0, torch.from_numpy(q).cuda(), i32([-30, 100]), n_rows=i32([0, 41]), out=out)
+    assert (out[0] == 5).all() and (out[1, 41:] == 5).all() and not (out[1, :41] == 5).all()
+    # a NaN query poisons its own row alone
+    clean = mk.cache.attention(0, torch.from_numpy(q).cuda(), i32([10, 100]))
+    q[1, 3, 1, 0] = np.nan
+    got = mk.cache.attention(0, torch.from_numpy(q).cuda(), i32([10, 100]))
+    assert torch.isnan(got[1, 3, 1]).all()
+    keep = torch.ones((2, 90, 2), dtype=torch.bool)
+    keep[1, 3, 1] = False
+    assert torch.equal(got[keep], clean[keep])
+
+
+def test_prompt_attention_with_bad_pages():
+    mk = Made(1, 1, 1, 64, 32, 8, seed=6)
+    rng = np.random.default_rng(0)
+    r = mk.fill([240], rng)
+    q = rng.standard_normal((1, 80, 1, 64)).astype(np.float32)
+    kk, vv = r.entries(0, 0, 0, 240)
+    mk.table[0, 0, 4] = mk.codes.shape[0] + 7
+    out = mk.cache.attention(0, torch.from_numpy(q).cuda(), i32([160]), out_dtype=torch.float32).cpu().numpy()
+    assert device_error() == 0x400
+    for t in (0, 5, 79):
+        see = np.r_[0:128, 160:161 + t]
+        s = q[0, t, 0].astype(np.float64) @ kk[see].T / 8
+        p = np.exp(s - s.max())
+        assert np.abs(out[0, t, 0] - p / p.sum() @ vv[see]).max() < 1e-2 * np.abs(vv).max()
+    mk.table[0, 0, 4] = int(mk.table_np[0, 0, 4])
+    mk.cache.attention(0, torch.from_numpy(q).cuda(), i32([200]))
+    assert device_error() == 0x400                           # entries past the capacity
+
+
+def test_prompt_values_of_very_different_size():
+    mk = Made(1, 1, 1, 128, 16, 8, seed=1)
+    rng = np.random.default_rng(3)
+    k = rng.standard_normal((1, 128, 1, 128)).astype(np.float32)
+    v = rng.standard_normal((1, 128, 1, 128)).astype(np.float32)
+    v *= np.repeat(2.0 ** np.array([0, -12, 3, -9, 0, -14, 6, -3]), 16).astype(np.float32)[None, :, None, None]
+    v[:, 64:80] = 0
+    k[:, 32:48] *= 20
+    r = mk.reference()
+    mk.cache.write(0, torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda(), i32([0]))
+    r.append(0, k, v, [0], [128])
+    kk, vv = r.entries(0, 0, 0, 128)
+    q = (kk / (kk ** 2).sum(-1, keepdims=True) * 40 * np.sqrt(128)).astype(np.float32).reshape(1, 128, 1, 128)
+    out = mk.cache.attention(0, torch.from_numpy(q).cuda(), i32([0]), out_dtype=torch.float32).cpu().numpy()
+    want, _, bound = r.attention(0, q, [0])
+    for t in range(127):
+        s = kk[:t + 1] @ q[0, t, 0].astype(np.float64) / np.sqrt(128)
+        p = np.exp(s - s.max())
+        p /= p.sum()
+        # weights off by 2 delta + 2^-11; f16 values keep 2^-30 of the largest block's
+        delta = ref.prompt_tolerance(128, 128, bound, 1.0, 0.0)[1]
+        ab = delta * (p @ np.abs(vv[:t + 1])) + 2.0 ** -30 * np.abs(vv).max()
+        assert (np.abs(out[0, t, 0] - want[0, t, 0]) <= ab).all(), t
 
 
 # ---------------------------------------------------------------- eviction
