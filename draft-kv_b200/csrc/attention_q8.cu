@@ -11,16 +11,18 @@
 //
 // Rounding: K and V enter exactly (block scales are powers of two: K's is
 // multiplied into the fp32 scores, V's into the probabilities).  Queries are
-// the sum of two f16 numbers (22 bits), probabilities too, so what is rounded
-// is what fp32 arithmetic rounds; max, sum and outputs are fp32.
+// the sum of two f16 numbers (22 bits), so scores, and the mass, are what fp32
+// arithmetic gives; probabilities are two f16 numbers for fp32 outputs, one
+// for bf16 outputs; max, sum and O are fp32.
 //
-// One CTA per (key split, KV head, sequence x row block).  A producer warp
-// streams 16 KB stages with bulk copies (one contiguous record of K and V per
-// page and head) through a ring; 4 warps per row group take every fourth
-// 16-token tile of a stage and keep (max, sum, O) of their own, merged in a
-// fixed order.  Split boundaries are absolute key positions and a row's
-// arithmetic does not depend on the other rows of the call, so a verify row
-// equals the decode step at that entry bit for bit.
+// One CTA per (key split, KV head, sequence x row block), two an SM.  Its 8
+// warps are on their own until the end: warp w takes units w, w + 8, ... of the
+// split (a unit is 4 KB: the K and V of 16 tokens at d = 128, of 32 at d = 64),
+// lane 0 fetches them with bulk copies into a ring of its warp's, and each warp
+// keeps (max, sum, O), merged in a fixed order.  Split and unit boundaries are
+// absolute key positions and a row's arithmetic does not depend on the other
+// rows of the call, so a verify row equals the decode step at that entry bit
+// for bit.
 //
 // The running max is raised lazily: only when a score exceeds it by more than
 // 8 (log2 units), which keeps the common tile free of shuffles and rescaling;
@@ -33,9 +35,12 @@ namespace dkv {
 
 namespace {
 
-constexpr int kQdStage = 16384;        // bytes of a ring stage
-constexpr int kQdKG = 4;               // key groups (warps a row group)
-constexpr int kQdMaxSplit = 8192;      // keys a split may have (page ids and scales staged in shared memory)
+constexpr int kQdKG = 8;               // key groups: the CTA's warps
+constexpr int kQdUnit = 4096;          // bytes of a unit
+constexpr int kQdDepth = 3;            // units of a warp's ring
+constexpr int kQdThreads = 32 * kQdKG;
+constexpr size_t kQdSmem = (size_t)kQdKG * kQdDepth * kQdUnit;
+constexpr int kQdMinBytes = 1 << 18;   // codes a split streams where the library picks it, at least
 constexpr float kQdLazy = 8.f;         // growth of the max that forces a rescale (log2 units)
 constexpr int kQdBias = 6;             // probabilities enter as p * 2^6: f16 keeps 2^-30 of the max
 
@@ -55,329 +60,418 @@ DKV_DEV uint32_t movm_trans(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
     return y;
 }
-DKV_DEV void mbar_arrive1(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(bar)) : "memory");
-}
-
-// NT: tiles of 8 query rows a warp carries; RG: row groups of 4 warps.
-template <int NT, int RG>
-struct QdGeo {
-    static constexpr int ROWS = 8 * NT * RG;           // query rows a CTA
-    static constexpr int WARPS = kQdKG * RG;
-    static constexpr int THREADS = 32 * (WARPS + 1);   // + the producer warp
-    static constexpr int STAGES = RG > 1 ? 10 : 5;     // one CTA an SM, or two
-    static constexpr int CTAS = RG > 1 ? 1 : 2;
-    static constexpr size_t SMEM = (size_t)STAGES * kQdStage;
+// Page ids and scales of a warp's next tiles, one tile a lane; the K scale of a
+// tile that must not be seen (bad page id, past the end) is negative.
+struct QdMeta {
+    int pid;
+    float ks, vs;
 };
 
-template <int D, int NT, int RG>
-__global__ void __launch_bounds__(QdGeo<NT, RG>::THREADS, QdGeo<NT, RG>::CTAS) q8_decode_kernel(const __grid_constant__ Q8AttnArgs a) {
-    using Geo = QdGeo<NT, RG>;
-    constexpr int KEYS = kQdStage / (2 * D);           // keys a stage
-    constexpr int TPW = KEYS / 16 / kQdKG;             // tiles a warp takes of a stage
-    constexpr int KS = D / 16, PS = D + 2, RB = Geo::ROWS;
-    extern __shared__ __align__(128) uint8_t ring[];
-    __shared__ __align__(8) uint64_t full_bar[Geo::STAGES], empty_bar[Geo::STAGES];
-    __shared__ int32_t page_s[kQdMaxSplit / 16];
-    __shared__ float2 scale_s[kQdMaxSplit / 16];
+// NT: tiles of 8 query rows; PLO: probabilities as two f16 numbers (fp32
+// outputs; one keeps 2^-12 of a weight, a sixteenth of a bf16 output's
+// rounding).  PAIR (up to 4 rows): columns 4..7 of the score product hold the
+// queries' lower parts, so one product gives both sums; the same numbers are
+// multiplied and added as without, so a row's bits do not depend on it.
+template <int D, int NT, bool PLO, bool PAIR>
+__global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const __grid_constant__ Q8AttnArgs a) {
+    constexpr int UT = kQdUnit / (2 * D);              // tokens a unit
+    constexpr int TPU = UT / 16;                       // 16-token tiles a unit
+    constexpr int UPB = 32 / TPU;                      // units whose tiles a warp's lanes describe at once
+    constexpr int KS = D / 16, PS = D + 2, RB = 8 * NT;
+    static_assert(!PAIR || NT == 1, "paired columns: one row tile");
+    constexpr int QP = PAIR ? 1 : 2;                   // query operands a row tile
+    static_assert(RB * PS * sizeof(float) <= kQdDepth * kQdUnit, "a warp's partial rows fit its ring");
+    extern __shared__ __align__(128) uint8_t ring_all[];
+    __shared__ __align__(8) uint64_t full_bar[kQdKG][kQdDepth];
+    __shared__ uint2 qs[NT > 1 ? QP * NT * KS * 32 : 1];       // query operands (NT 1: in registers)
     __shared__ float ms[RB], ls[RB];
+    __shared__ float gw[RB * kQdKG];
     __shared__ int failed;
     const Q8View& v = a.v;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < Geo::STAGES; ++i) {
-            mbar_init(&full_bar[i], 1);
-            mbar_init(&empty_bar[i], Geo::WARPS);
-        }
-        failed = 0;
+    uint8_t* ring = ring_all + (size_t)warp * kQdDepth * kQdUnit;
+    uint64_t* full = full_bar[warp];
+    if (lane == 0) {
+        for (int i = 0; i < kQdDepth; ++i) mbar_init(&full[i], 1);
+        if (warp == 0) failed = 0;
         fence_async_shared();
     }
+    __syncwarp();
     pdl_trigger();
     pdl_wait();            // queries and the new entries come from earlier kernels
 
+    // one round of loads: the first page ids (any entry of the table row may be
+    // read), the query rows, entry0 and n_rows
     const int s = blockIdx.x, h = blockIdx.y;
     const int b = blockIdx.z / a.n_rb, rb = blockIdx.z % a.n_rb;
     const int G = a.group, R_all = a.T * G;
     const int rbase = rb * RB, R = min(RB, R_all - rbase);
+    const int k0 = s * a.split;
+    const int32_t* tab = v.row(b);
+    auto key_of = [&](int u) { return k0 + (u * kQdKG + warp) * UT; };
+    // page id of tile `lane` of the batch that starts at this warp's unit u0 (-1 beyond the table)
+    auto load_pid = [&](int u0) {
+        const int pg = (key_of(u0 + lane / TPU) + (lane % TPU) * 16) >> v.page_shift;
+        return pg < v.max_pages ? __ldg(tab + pg) : -1;
+    };
+    const int first_pid = load_pid(0);
+    const int qr = lane >> 2, qc = lane & 3;
+    float2 xq[NT > 1 ? 1 : KS][2];
+    auto load_q = [&](int nt, int kk, int u) {
+        const int r = nt * 8 + (PAIR ? qr & 3 : qr), gr = rbase + r;      // this lane's operand row
+        return r < R ? __ldg(reinterpret_cast<const float2*>(
+                           a.q + (((size_t)b * a.T + gr / G) * v.n_kv * G + h * G + gr % G) * D + kk * 16 + u * 8 + 2 * qc))
+                     : make_float2(0.f, 0.f);
+    };
+    if (NT == 1) {
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk) xq[NT > 1 ? 0 : kk][0] = load_q(0, kk, 0), xq[NT > 1 ? 0 : kk][1] = load_q(0, kk, 1);
+    }
     const int n_tok = a.n_rows ? min(a.n_rows[b], a.T) : a.T;
     const int e0 = a.entry0[b];
-    const int k0 = s * a.split;
     // the block's last token decides what is read
     const int t_last = min((rbase + R - 1) / G, n_tok - 1);
     const int n_keys = t_last >= rbase / G ? max(0, min(a.n_keys(b), e0 + t_last + 1)) : 0;
     const int kend = min(n_keys, k0 + a.split);
-    const int psx = min(v.page, KEYS);                 // tokens of a page inside a stage
-    const int n_pg = kend > k0 ? (kend - k0 + v.page - 1) >> v.page_shift : 0;
     if (s == 0 && h == 0 && rb == 0 && threadIdx.x == 0 && a.beyond(b)) atomicOr(a.err, kErrQ8Page);
-    // page ids and scales of the split: a page with a bad id gets -1 and its keys are not seen
-    for (int i = threadIdx.x; i < n_pg; i += Geo::THREADS) {
-        const int pid = __ldg(v.row(b) + (k0 >> v.page_shift) + i);
-        const bool ok = v.ok(pid);
-        page_s[i] = ok ? pid : -1;
-        scale_s[i] = ok ? *reinterpret_cast<const float2*>(v.scale + v.scale_at(pid, h, 0)) : make_float2(1.f, 1.f);
-        if (!ok) atomicOr(a.err, kErrQ8Page);
-    }
-    __syncthreads();
-    const int n_st = kend > k0 ? (kend - k0 + KEYS - 1) / KEYS : 0;
+    const int n_units = kend > k0 ? (kend - k0 + UT - 1) / UT : 0;
+    const int mine = n_units > warp ? (n_units - warp + kQdKG - 1) / kQdKG : 0;      // this warp's units
 
-    float m[NT][2], l[NT][2];
+    // -1 for tiles past the end and for bad ids (recorded; their keys are not seen)
+    auto check_pid = [&](int u0, int pid) {
+        const int u = u0 + lane / TPU;
+        if (u >= mine || key_of(u) + (lane % TPU) * 16 >= kend) return -1;
+        if (v.ok(pid)) return pid;
+        atomicOr(a.err, kErrQ8Page);
+        return -1;
+    };
+    auto load_scale = [&](int pid, float& ks, float& vs) {
+        float2 sc = make_float2(-1.f, 1.f);
+        if (pid >= 0) sc = __ldg(reinterpret_cast<const float2*>(v.scale + v.scale_at(pid, h, 0)));
+        ks = sc.x;
+        vs = sc.y;
+    };
+    // unit u into ring slot `slot` (u % depth); pids: the page ids of its batch.
+    // A tile is [K 16 d][V 16 d]; a 16-token page is one copy, of longer ones two
+    const int rec = 2 * v.page * D;
+    const uint8_t* base_h = v.codes + (size_t)h * rec;
+    const size_t page_stride = (size_t)v.n_kv * rec;
+    auto issue = [&](int u, int slot, int pids) {
+        int pid[TPU], live = 0;
+#pragma unroll
+        for (int tt = 0; tt < TPU; ++tt) {
+            pid[tt] = __shfl_sync(0xffffffffu, pids, (u % UPB) * TPU + tt);
+            live += pid[tt] >= 0;
+        }
+        if (lane == 0) {
+            uint8_t* to = ring + slot * kQdUnit;
+            uint64_t* bar = &full[slot];
+            mbar_expect_tx(bar, (uint32_t)(live * 32 * D));
+#pragma unroll
+            for (int tt = 0; tt < TPU; ++tt) {
+                if (pid[tt] < 0) continue;
+                const uint8_t* kp = base_h + (size_t)pid[tt] * page_stride;
+                if (v.page == 16) {
+                    bulk_g2s(to + tt * 32 * D, kp, 32 * D, bar);
+                } else {
+                    kp += ((key_of(u) + tt * 16) & (v.page - 1)) * D;
+                    bulk_g2s(to + tt * 32 * D, kp, 16 * D, bar);
+                    bulk_g2s(to + tt * 32 * D + 16 * D, kp + v.page * D, 16 * D, bar);
+                }
+            }
+        }
+        __syncwarp();
+    };
+    QdMeta cur{-1, -1.f, 1.f}, nxt{-1, -1.f, 1.f};
+    cur.pid = check_pid(0, first_pid);
+    const int prologue = min(mine, kQdDepth);
+    for (int u = 0; u < prologue; ++u) issue(u, u, cur.pid);     // (kQdDepth <= UPB)
+    load_scale(cur.pid, cur.ks, cur.vs);
+
+    // ---------------- queries: column qr of row tile nt, as hi (+ lo) f16
+    // numbers of q * log2 e / sqrt(d) * 2^-x, x the row's exponent
+    uint2 qreg[NT > 1 ? 1 : QP * KS];
+    float cs[NT][2];                                   // 2^x of this thread's score columns
+    int lim[NT][2];                                    // last visible entry of them
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        float2 x[KS][2];
+        float am = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                x[kk][u] = NT == 1 ? xq[NT > 1 ? 0 : kk][u] : load_q(nt, kk, u);
+                x[kk][u].x *= a.scale;
+                x[kk][u].y *= a.scale;
+                am = fmaxf(am, fmaxf(fabsf(x[kk][u].x), fabsf(x[kk][u].y)));
+            }
+        am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 1));
+        am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 2));
+        // am = 1.m * 2^ex; an infinite row keeps its infinities
+        const int ex = min(max((int)(__float_as_uint(am) >> 23) - 127, -100), 126);
+        const float down = q8_pow2(-ex);
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk) {
+            uint2 hi, lo;
+            uint32_t* hp = &hi.x;
+            uint32_t* lp = &lo.x;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const float p = x[kk][u].x * down, q = x[kk][u].y * down;
+                hp[u] = pack_h2(p, q);
+                const float2 hf = unpack_h2(hp[u]);
+                lp[u] = pack_h2(p - hf.x, q - hf.y);
+            }
+            if (NT > 1) {
+                if (warp == kk % kQdKG) {              // (every warp holds the same rows)
+                    qs[(kk * NT + nt) * 32 + lane] = hi;
+                    qs[((KS + kk) * NT + nt) * 32 + lane] = lo;
+                }
+            } else if (PAIR) {
+                qreg[kk] = qr < 4 ? hi : lo;
+            } else {
+                qreg[kk] = hi;
+                qreg[(QP - 1) * KS + kk] = lo;
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            cs[nt][c] = __shfl_sync(0xffffffffu, q8_pow2(ex), (2 * qc + c) * 4);
+            const int rc = nt * 8 + 2 * qc + c, t = (rbase + rc) / G;
+            lim[nt][c] = rc < R && (!PAIR || qc < 2) && t < n_tok ? min(e0 + t, n_keys - 1) : -1;
+        }
+    }
+    if (NT > 1) __syncthreads();
+    auto query = [&](int piece, int kk, int nt) -> uint2 {
+        if (NT > 1) return qs[((piece * KS + kk) * NT + nt) * 32 + lane];
+        return qreg[piece * KS + kk];
+    };
+
+    // m: the running max (0 until a key was seen, for which thr is -infinity);
+    // thr: the score that forces m up
+    float m[NT][2], thr[NT][2], l[NT][2];
     float o[NT][KS][4];
     int eo = kQ8ExpMin;                                // O is in units of 2^(eo - kQdBias)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        m[nt][0] = m[nt][1] = -INFINITY;
-        l[nt][0] = l[nt][1] = 0.f;
+        m[nt][0] = m[nt][1] = l[nt][0] = l[nt][1] = 0.f;
+        thr[nt][0] = thr[nt][1] = -INFINITY;
 #pragma unroll
         for (int md = 0; md < KS; ++md) o[nt][md][0] = o[nt][md][1] = o[nt][md][2] = o[nt][md][3] = 0.f;
     }
-    const int kg = warp % kQdKG, rg = warp / kQdKG;
-    const int qr = lane >> 2, qc = lane & 3;
+    float* sc_base = a.scores ? a.scores + (((size_t)b * v.n_kv + h) * v.capacity()) * a.s_ld : nullptr;
+    // entries up to here are seen by every row of the block that is there
+    const int all_see = min(e0 + rbase / G, kend - 1);
 
-    if (warp == Geo::WARPS) {
-        // ---------------- producer: lane j copies page j of a stage
-        for (int it = 0; it < n_st; ++it) {
-            const int slot = it % Geo::STAGES;
-            if (it >= Geo::STAGES &&
-                !__all_sync(0xffffffffu, mbar_wait(&empty_bar[slot], (uint32_t)((it / Geo::STAGES - 1) & 1), a.err))) {
-                if (lane == 0) failed = 1;
-                break;
-            }
-            const int t0 = k0 + it * KEYS;
-            uint8_t* dst = ring + (size_t)slot * kQdStage;
-            const int live = (min(kend - t0, KEYS) + psx - 1) / psx;     // page parts with a visible key
-            const int pid = lane < live ? page_s[(t0 + lane * psx - k0) >> v.page_shift] : -1;
-            const int parts = __popc(__ballot_sync(0xffffffffu, pid >= 0));
-            if (lane == 0) mbar_expect_tx(&full_bar[slot], (uint32_t)(parts * psx * 2 * D));
-            __syncwarp();
-            if (pid >= 0) {
-                const int in_page = (t0 + lane * psx) & (v.page - 1);
-                const uint8_t* kp = v.side(pid, h, 0) + (size_t)in_page * D;
-                uint8_t* to = dst + (size_t)lane * psx * 2 * D;
-                if (psx == v.page) {
-                    bulk_g2s(to, kp, (uint32_t)(psx * 2 * D), &full_bar[slot]);
-                } else {
-                    bulk_g2s(to, kp, (uint32_t)(psx * D), &full_bar[slot]);
-                    bulk_g2s(to + psx * D, v.side(pid, h, 1) + (size_t)in_page * D, (uint32_t)(psx * D),
-                             &full_bar[slot]);
-                }
+    int slot = 0;
+    uint32_t phase = 0;
+    for (int u = 0; u < mine; ++u) {
+        const int ub = u % UPB;
+        if (ub == 0) {
+            if (u > 0) cur = nxt;
+            nxt.pid = check_pid(u + UPB, load_pid(u + UPB));
+        } else if (ub == UPB / 2) {
+            load_scale(nxt.pid, nxt.ks, nxt.vs);
+        }
+        const uint8_t* st = ring + slot * kQdUnit + lane * 16;
+        if (!__all_sync(0xffffffffu, mbar_wait(&full[slot], phase, a.err))) {
+            // a copy never came (error word 0x80): wait, bounded, for those still in flight
+            if (lane == 0) {
+                failed = 1;
+                for (int w = u + 1; w < min(mine, u + kQdDepth); ++w)
+                    mbar_wait(&full[w % kQdDepth], (uint32_t)((w / kQdDepth) & 1), nullptr);
             }
             __syncwarp();
+            break;
         }
-    } else {
-        // ---------------- queries: column qr of row tile nt, as hi + lo f16
-        // numbers of q * log2 e / sqrt(d) * 2^-x, x the row's exponent
-        uint32_t qh[NT][KS][2], ql[NT][KS][2];
-        float cs[NT][2];                               // 2^x of this thread's score columns
-        int lim[NT][2];                                // last visible entry of them
+        const int key0 = key_of(u);
+        float ks[TPU], vs[TPU];
+        bool whole = key0 + UT - 1 <= all_see;         // every key of the unit is there for every row
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int r = (rg * NT + nt) * 8 + qr;     // this lane's operand row
-            const int gr = rbase + r;
-            const float* qv = r < R ? a.q + (((size_t)b * a.T + gr / G) * v.n_kv * G + h * G + gr % G) * D : nullptr;
-            float2 x[KS][2];
-            float am = 0.f;
-#pragma unroll
-            for (int kk = 0; kk < KS; ++kk)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    x[kk][u] = qv ? __ldg(reinterpret_cast<const float2*>(qv + kk * 16 + u * 8 + 2 * qc))
-                                  : make_float2(0.f, 0.f);
-                    x[kk][u].x *= a.scale;
-                    x[kk][u].y *= a.scale;
-                    am = fmaxf(am, fmaxf(fabsf(x[kk][u].x), fabsf(x[kk][u].y)));
-                }
-            am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 1));
-            am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 2));
-            // am = 1.m * 2^ex; an infinite row keeps its infinities
-            const int ex = min(max((int)(__float_as_uint(am) >> 23) - 127, -100), 126);
-            const float down = q8_pow2(-ex);
-#pragma unroll
-            for (int kk = 0; kk < KS; ++kk)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const float p = x[kk][u].x * down, q = x[kk][u].y * down;
-                    qh[nt][kk][u] = pack_h2(p, q);
-                    const float2 hi = unpack_h2(qh[nt][kk][u]);
-                    ql[nt][kk][u] = pack_h2(p - hi.x, q - hi.y);
-                }
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                cs[nt][c] = __shfl_sync(0xffffffffu, q8_pow2(ex), (2 * qc + c) * 4);
-                const int rc = (rg * NT + nt) * 8 + 2 * qc + c, t = (rbase + rc) / G;
-                lim[nt][c] = rc < R && t < n_tok ? min(e0 + t, n_keys - 1) : -1;
-            }
+        for (int tt = 0; tt < TPU; ++tt) {
+            ks[tt] = __shfl_sync(0xffffffffu, cur.ks, ub * TPU + tt);
+            vs[tt] = __shfl_sync(0xffffffffu, cur.vs, ub * TPU + tt);
+            whole = whole && ks[tt] >= 0.f;
         }
-        const int row0 = rbase + rg * NT * 8 + 2 * qc;     // row of score column (nt 0, c 0)
-        float* sc_base = a.scores ? a.scores + (((size_t)b * v.n_kv + h) * v.capacity()) * a.s_ld : nullptr;
-
-        for (int it = 0; it < n_st; ++it) {
-            const int slot = it % Geo::STAGES, t0 = k0 + it * KEYS;
-            const uint8_t* st = ring + (size_t)slot * kQdStage;
-            if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[slot], (uint32_t)((it / Geo::STAGES) & 1), a.err))) {
-                if (lane == 0) failed = 1;
-                break;
-            }
+        // ---- S^T: keys qr (+8), columns 2qc, 2qc + 1 of each row tile
+        float sh[TPU][NT][4];
+        bool grow = false;
 #pragma unroll
-            for (int tw = 0; tw < TPW; ++tw) {
-                const int tile = tw * kQdKG + kg, key0 = t0 + tile * 16;
-                if (key0 >= kend) break;
-                const int part = tile * 16 / psx, inside = tile * 16 % psx;
-                const uint8_t* kb = st + (size_t)part * psx * 2 * D + (size_t)inside * D + lane * 16;
-                const uint8_t* vb = kb + psx * D;
-                const int pi = (key0 - k0) >> v.page_shift;
-                const bool bad = page_s[pi] < 0;
-                const float2 sc2 = scale_s[pi];
-                // ---- S^T: keys qr (+8), columns 2qc, 2qc + 1 of each row tile
-                float sh[NT][4], sl[NT][4];
+        for (int tt = 0; tt < TPU; ++tt) {
+            float sl[NT][4];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) sh[nt][e] = sl[nt][e] = 0.f;
+                for (int e = 0; e < 4; ++e) sh[tt][nt][e] = sl[nt][e] = 0.f;
 #pragma unroll
-                for (int j = 0; j < D / 32; ++j) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(kb + j * 512);
-                    uint32_t a0[4], a1[4];
-                    q8_decode4(w.x, a0[0], a0[2]);
-                    q8_decode4(w.y, a0[1], a0[3]);
-                    q8_decode4(w.z, a1[0], a1[2]);
-                    q8_decode4(w.w, a1[1], a1[3]);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        mma_f16_16816(sh[nt], a0, qh[nt][2 * j][0], qh[nt][2 * j][1]);
-                        mma_f16_16816(sl[nt], a0, ql[nt][2 * j][0], ql[nt][2 * j][1]);
-                        mma_f16_16816(sh[nt], a1, qh[nt][2 * j + 1][0], qh[nt][2 * j + 1][1]);
-                        mma_f16_16816(sl[nt], a1, ql[nt][2 * j + 1][0], ql[nt][2 * j + 1][1]);
-                    }
-                }
-                const int ka = key0 + qr, kb2 = ka + 8;
-                bool grow = false;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const float f = cs[nt][c] * sc2.x;
-                        const int last = bad ? -1 : lim[nt][c];
-                        const float x = ka <= last ? (sh[nt][c] + sl[nt][c]) * f : -INFINITY;
-                        const float y = kb2 <= last ? (sh[nt][c + 2] + sl[nt][c + 2]) * f : -INFINITY;
-                        sh[nt][c] = x;
-                        sh[nt][c + 2] = y;
-                        grow = grow || fmaxf(x, y) > m[nt][c] + kQdLazy;
-                    }
-                if (sc_base) {
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        const int r = row0 + nt * 8;
-                        if (r < a.s_ld && r - rbase < RB) {
-                            if (ka < kend)
-                                *reinterpret_cast<float2*>(sc_base + (size_t)ka * a.s_ld + r) =
-                                    make_float2(sh[nt][0], sh[nt][1]);
-                            if (kb2 < kend)
-                                *reinterpret_cast<float2*>(sc_base + (size_t)kb2 * a.s_ld + r) =
-                                    make_float2(sh[nt][2], sh[nt][3]);
-                        }
-                    }
-                }
-                if (__any_sync(0xffffffffu, grow)) {
-                    // raise the max of the columns that need it (alpha 1 for the others)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        float al[2];
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            float t = fmaxf(sh[nt][c], sh[nt][c + 2]);
-#pragma unroll
-                            for (int off = 4; off < 32; off <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, off));
-                            const bool up = t > m[nt][c] + kQdLazy;
-                            al[c] = up ? q8_ex2(m[nt][c] - t) : 1.f;
-                            if (up) m[nt][c] = t;
-                            l[nt][c] *= al[c];
-                        }
-#pragma unroll
-                        for (int md = 0; md < KS; ++md) {
-                            o[nt][md][0] *= al[0];
-                            o[nt][md][1] *= al[1];
-                            o[nt][md][2] *= al[0];
-                            o[nt][md][3] *= al[1];
-                        }
-                    }
-                }
-                const int ev = q8_scale_exp(sc2.y);
-                if (ev > eo) {                         // (uniform) larger V values: O to their units
-                    const float dn = q8_pow2(max(eo - ev, -126));
-                    eo = ev;
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int md = 0; md < KS; ++md)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) o[nt][md][e] *= dn;
-                }
-                const float vf = q8_pow2(max(ev - eo + kQdBias, -126));
-                uint32_t ph[NT][2], pl[NT][2];
+            for (int j = 0; j < D / 32; ++j) {
+                const uint4 w = *reinterpret_cast<const uint4*>(st + tt * 32 * D + j * 512);
+                uint32_t a0[4], a1[4];
+                q8_decode4(w.x, a0[0], a0[2]);
+                q8_decode4(w.y, a0[1], a0[3]);
+                q8_decode4(w.z, a1[0], a1[2]);
+                q8_decode4(w.w, a1[1], a1[3]);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    float p[4];
+                    const uint2 q0 = query(0, 2 * j, nt), q1 = query(0, 2 * j + 1, nt);
+                    mma_f16_16816(sh[tt][nt], a0, q0.x, q0.y);
+                    if (!PAIR) {
+                        const uint2 p0 = query(1, 2 * j, nt);
+                        mma_f16_16816(sl[nt], a0, p0.x, p0.y);
+                    }
+                    mma_f16_16816(sh[tt][nt], a1, q1.x, q1.y);
+                    if (!PAIR) {
+                        const uint2 p1 = query(1, 2 * j + 1, nt);
+                        mma_f16_16816(sl[nt], a1, p1.x, p1.y);
+                    }
+                }
+            }
+            if (PAIR) {                                // lane qc holds columns 2qc, + 1; qc + 2 their lower parts
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sl[0][e] = __shfl_xor_sync(0xffffffffu, sh[tt][0][e], 2);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sh[tt][nt][e] = (sh[tt][nt][e] + sl[nt][e]) * (cs[nt][e & 1] * ks[tt]);
+        }
+        if (!whole) {
+#pragma unroll
+            for (int tt = 0; tt < TPU; ++tt)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        p[e] = sh[nt][e] == -INFINITY ? 0.f : q8_ex2(sh[nt][e] - m[nt][e & 1]);
-                        if (e >= 2) l[nt][e & 1] += p[e - 2] + p[e];
-                        p[e] = p[e];
+                        const int key = key0 + tt * 16 + qr + (e >> 1) * 8;
+                        if (key > lim[nt][e & 1] || ks[tt] < 0.f) sh[tt][nt][e] = -INFINITY;
                     }
+        }
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const float x = p[2 * u] * vf, y = p[2 * u + 1] * vf;
-                        const uint32_t hi = pack_h2(x, y);
-                        const float2 hf = unpack_h2(hi);
-                        ph[nt][u] = movm_trans(hi);
-                        pl[nt][u] = movm_trans(pack_h2(x - hf.x, y - hf.y));
+        for (int tt = 0; tt < TPU; ++tt)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+                grow = grow || fmaxf(sh[tt][nt][0], sh[tt][nt][2]) > thr[nt][0] || fmaxf(sh[tt][nt][1], sh[tt][nt][3]) > thr[nt][1];
+        if (sc_base) {
+#pragma unroll
+            for (int tt = 0; tt < TPU; ++tt)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const int r = rbase + nt * 8 + 2 * qc, ka = key0 + tt * 16 + qr;
+                    if (r < a.s_ld && (!PAIR || qc < 2)) {
+                        if (ka < kend)
+                            *reinterpret_cast<float2*>(sc_base + (size_t)ka * a.s_ld + r) =
+                                make_float2(sh[tt][nt][0], sh[tt][nt][1]);
+                        if (ka + 8 < kend)
+                            *reinterpret_cast<float2*>(sc_base + (size_t)(ka + 8) * a.s_ld + r) =
+                                make_float2(sh[tt][nt][2], sh[tt][nt][3]);
                     }
                 }
+        }
+        if (__any_sync(0xffffffffu, grow)) {
+            // raise the max of the columns that need it (alpha 1 for the others)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float al[2];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float t = -INFINITY;
+#pragma unroll
+                    for (int tt = 0; tt < TPU; ++tt) t = fmaxf(t, fmaxf(sh[tt][nt][c], sh[tt][nt][c + 2]));
+#pragma unroll
+                    for (int off = 4; off < 32; off <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, off));
+                    const bool up = t > thr[nt][c];
+                    al[c] = !up ? 1.f : thr[nt][c] == -INFINITY ? 0.f : q8_ex2(m[nt][c] - t);
+                    if (up) m[nt][c] = t, thr[nt][c] = t + kQdLazy;
+                    l[nt][c] *= al[c];
+                }
+#pragma unroll
+                for (int md = 0; md < KS; ++md) {
+                    o[nt][md][0] *= al[0];
+                    o[nt][md][1] *= al[1];
+                    o[nt][md][2] *= al[0];
+                    o[nt][md][3] *= al[1];
+                }
+            }
+        }
+        int ev = q8_scale_exp(vs[0]);
+#pragma unroll
+        for (int tt = 1; tt < TPU; ++tt) ev = max(ev, q8_scale_exp(vs[tt]));
+        if (ev > eo) {                                 // (uniform) larger V values: O to their units
+            const float dn = q8_pow2(max(eo - ev, -126));
+            eo = ev;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int md = 0; md < KS; ++md)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[nt][md][e] *= dn;
+        }
+#pragma unroll
+        for (int tt = 0; tt < TPU; ++tt) {
+            const float vf = q8_pow2(max(q8_scale_exp(vs[tt]) - eo + kQdBias, -126));
+            uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float p[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[e] = q8_ex2(sh[tt][nt][e] - m[nt][e & 1]);
+                l[nt][0] += p[0] + p[2];
+                l[nt][1] += p[1] + p[3];
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    const float x = p[2 * w] * vf, y = p[2 * w + 1] * vf;
+                    const uint32_t hi = pack_h2(x, y);
+                    ph[nt][w] = movm_trans(hi);
+                    if (PLO) {
+                        const float2 hf = unpack_h2(hi);
+                        pl[nt][w] = movm_trans(pack_h2(x - hf.x, y - hf.y));
+                    }
+                }
+            }
+            const uint8_t* vb = st + tt * 32 * D + 16 * D;
+            uint4 w[D / 32];
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) w[j] = *reinterpret_cast<const uint4*>(vb + j * 512);
+            if (!whole) {
                 // bytes of keys that are not there (past the end, bad page) as zeros:
                 // their probability is 0, but 0 x NaN would not be
-                uint32_t vm = 0xffffffffu;
-                if (key0 + 16 > kend || bad) {
-                    vm = 0u;
-                    const int ke = bad ? 0 : kend - key0;
-                    if (2 * qc < ke) vm |= 0xffu;
-                    if (2 * qc + 1 < ke) vm |= 0xff00u;
-                    if (2 * qc + 8 < ke) vm |= 0xff0000u;
-                    if (2 * qc + 9 < ke) vm |= 0xff000000u;
-                }
+                const int ke = ks[tt] < 0.f ? 0 : kend - key0 - tt * 16;
+                const uint32_t vm = (2 * qc < ke ? 0xffu : 0u) | (2 * qc + 1 < ke ? 0xff00u : 0u) |
+                                    (2 * qc + 8 < ke ? 0xff0000u : 0u) | (2 * qc + 9 < ke ? 0xff000000u : 0u);
 #pragma unroll
-                for (int j = 0; j < D / 32; ++j) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(vb + j * 512);
-                    uint32_t a0[4], a1[4];
-                    q8_decode4(w.x & vm, a0[0], a0[2]);
-                    q8_decode4(w.y & vm, a0[1], a0[3]);
-                    q8_decode4(w.z & vm, a1[0], a1[2]);
-                    q8_decode4(w.w & vm, a1[1], a1[3]);
+                for (int j = 0; j < D / 32; ++j) w[j].x &= vm, w[j].y &= vm, w[j].z &= vm, w[j].w &= vm;
+            }
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        mma_f16_16816(o[nt][2 * j], a0, ph[nt][0], ph[nt][1]);
-                        mma_f16_16816(o[nt][2 * j + 1], a1, ph[nt][0], ph[nt][1]);
+            for (int j = 0; j < D / 32; ++j) {
+                uint32_t a0[4], a1[4];
+                q8_decode4(w[j].x, a0[0], a0[2]);
+                q8_decode4(w[j].y, a0[1], a0[3]);
+                q8_decode4(w[j].z, a1[0], a1[2]);
+                q8_decode4(w[j].w, a1[1], a1[3]);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    mma_f16_16816(o[nt][2 * j], a0, ph[nt][0], ph[nt][1]);
+                    mma_f16_16816(o[nt][2 * j + 1], a1, ph[nt][0], ph[nt][1]);
+                    if (PLO) {
                         mma_f16_16816(o[nt][2 * j], a0, pl[nt][0], pl[nt][1]);
                         mma_f16_16816(o[nt][2 * j + 1], a1, pl[nt][0], pl[nt][1]);
                     }
                 }
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive1(&empty_bar[slot]);
         }
+        // the slot's bytes are in registers: refill it
+        __syncwarp();
+        const int un = u + kQdDepth;
+        if (un < mine) issue(un, slot, ub + kQdDepth < UPB ? cur.pid : nxt.pid);
+        if (++slot == kQdDepth) slot = 0, phase ^= 1u;
     }
-    __syncthreads();
-    if (failed) {
-        // a wait ran out (error word 0x80): wait, bounded, for the copies still
-        // in flight before the ring is reused; the split counts as empty
-        if (threadIdx.x == 0)
-            for (int it = max(0, n_st - Geo::STAGES); it < n_st; ++it)
-                mbar_wait(&full_bar[it % Geo::STAGES], (uint32_t)((it / Geo::STAGES) & 1), nullptr);
-        __syncthreads();
-    }
+    __syncwarp();
 
-    // ---- the key groups' (max, sum, O) of every row to the drained ring
-    float* mrg = reinterpret_cast<float*>(ring);           // [KG][RB][D + 2]
-    if (warp < Geo::WARPS) {
-        const float un = q8_pow2(eo) * q8_pow2(-kQdBias);  // (eo - bias may pass the smallest exponent)
+    // ---- this warp's (max, sum, O) of every row to its drained ring
+    {
+        float* mine_f = reinterpret_cast<float*>(ring);        // [RB][D + 2]
+        const float un = q8_pow2(eo), bias = q8_pow2(-kQdBias);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -385,17 +479,17 @@ __global__ void __launch_bounds__(QdGeo<NT, RG>::THREADS, QdGeo<NT, RG>::CTAS) q
                 float ll = l[nt][c];
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) ll += __shfl_xor_sync(0xffffffffu, ll, off);
-                // a row with NaN scores has no max: give it one, so that its NaN sum is merged
-                const float mm = ll != ll && m[nt][c] == -INFINITY ? 0.f : m[nt][c];
-                float* to = mrg + ((size_t)kg * RB + (rg * NT + nt) * 8 + 2 * qc + c) * PS;
+                // no key seen: -infinity (a row with NaN scores has a NaN sum, to be merged)
+                const float mm = thr[nt][c] == -INFINITY && ll == ll ? -INFINITY : m[nt][c];
+                float* to = mine_f + (nt * 8 + 2 * qc + c) * PS;
                 if (qr == 0) {
                     to[0] = mm;
                     to[1] = ll;
                 }
 #pragma unroll
                 for (int md = 0; md < KS; ++md) {
-                    to[2 + 16 * md + qr] = o[nt][md][c] * un;
-                    to[2 + 16 * md + qr + 8] = o[nt][md][c + 2] * un;
+                    to[2 + 16 * md + qr] = o[nt][md][c] * un * bias;
+                    to[2 + 16 * md + qr + 8] = o[nt][md][c + 2] * un * bias;
                 }
             }
     }
@@ -403,36 +497,33 @@ __global__ void __launch_bounds__(QdGeo<NT, RG>::THREADS, QdGeo<NT, RG>::CTAS) q
     const size_t bhr = ((size_t)b * v.n_kv + h) * a.n_rb + rb;
     const bool alone = a.n_splits == 1;
     float* mypart = alone ? nullptr : a.part + (bhr * a.n_splits + s) * (size_t)RB * PS;
-    // group weights first (in place over the maxima), then the sums
-    for (int r = threadIdx.x; r < R; r += Geo::THREADS) {
-        float M = -INFINITY, L = 0.f, w[kQdKG];
+    auto group_row = [&](int g, int r) { return reinterpret_cast<const float*>(ring_all + (size_t)g * kQdDepth * kQdUnit) + r * PS; };
+    if (threadIdx.x < R) {
+        const int r = threadIdx.x;
+        float M = -INFINITY, L = 0.f;
 #pragma unroll
-        for (int g = 0; g < kQdKG; ++g) M = fmaxf(M, mrg[((size_t)g * RB + r) * PS]);
+        for (int g = 0; g < kQdKG; ++g) M = fmaxf(M, group_row(g, r)[0]);
 #pragma unroll
         for (int g = 0; g < kQdKG; ++g) {
-            const float mg = mrg[((size_t)g * RB + r) * PS];
-            w[g] = mg == -INFINITY ? 0.f : q8_ex2(mg - M);
-            if (w[g] != 0.f) L += mrg[((size_t)g * RB + r) * PS + 1] * w[g];
-            mrg[((size_t)g * RB + r) * PS] = w[g];
+            const float mg = group_row(g, r)[0];
+            const float w = mg == -INFINITY ? 0.f : q8_ex2(mg - M);
+            if (w != 0.f) L += group_row(g, r)[1] * w;
+            gw[r * kQdKG + g] = w;
         }
-        if (failed) M = -INFINITY, L = 0.f;
+        if (failed) M = -INFINITY, L = 0.f;            // a failed split counts as empty
         ms[r] = M;
         ls[r] = L;
-        if (!alone) {
-            mypart[(size_t)r * PS] = M;
-            mypart[(size_t)r * PS + 1] = L;
-        }
+        if (!alone) *reinterpret_cast<float2*>(mypart + (size_t)r * PS) = make_float2(M, L);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < R * (D / 2); i += Geo::THREADS) {
+    for (int i = threadIdx.x; i < R * (D / 2); i += kQdThreads) {
         const int r = i / (D / 2), e = i % (D / 2) * 2;
         float x0 = 0.f, x1 = 0.f;
 #pragma unroll
         for (int g = 0; g < kQdKG; ++g) {
-            const float* at = mrg + ((size_t)g * RB + r) * PS;
-            const float w = at[0];
+            const float w = gw[r * kQdKG + g];
             if (w != 0.f) {
-                const float2 y = *reinterpret_cast<const float2*>(at + 2 + e);
+                const float2 y = *reinterpret_cast<const float2*>(group_row(g, r) + 2 + e);
                 x0 += y.x * w;
                 x1 += y.y * w;
             }
@@ -444,65 +535,89 @@ __global__ void __launch_bounds__(QdGeo<NT, RG>::THREADS, QdGeo<NT, RG>::CTAS) q
             *reinterpret_cast<float2*>(mypart + (size_t)r * PS + 2 + e) = make_float2(x0, x1);
         }
     }
-    if (!alone && !q8_merge_splits<D, RB>(a, bhr, b, h, rbase, R, n_tok, mrg, Geo::SMEM, ms, ls)) return;
-    if (a.stats)
-        for (int r = threadIdx.x; r < R; r += Geo::THREADS)
+    if (!alone) {
+        q8_merge_splits<D, RB>(a, bhr, b, h, rbase, R, n_tok);
+    } else if (a.stats) {
+        for (int r = threadIdx.x; r < R; r += kQdThreads)
             a.stats[((size_t)b * v.n_kv + h) * R_all + rbase + r] =
-                make_float2(ms[r], ls[r] == 0.f ? 0.f : 1.f / ls[r]);
+                make_float2(ms[r], ls[r] == 0.f || (rbase + r) / G >= n_tok ? 0.f : 1.f / ls[r]);
+    }
 }
 
 // mass[b][h][j] += sum over the call's rows of p_j: the scores of the pass
 // above under the merged (max, sum), rows in order (no atomics).
-constexpr int kMassThreads = 256;
+// A thread takes kMassKeys keys, kMassThreads apart, whose loads are in flight
+// together.
+constexpr int kMassThreads = 256, kMassKeys = 4;
 __global__ void __launch_bounds__(kMassThreads) q8_mass_kernel(Q8AttnArgs a, float* mass) {
-    __shared__ float2 st_s[kQ8MaxRows];
+    __shared__ float2 st_s[kQ8MaxRows + 1];
     pdl_trigger();
     pdl_wait();
     const int h = blockIdx.y, b = blockIdx.z, R = a.T * a.group;
-    const int n = a.n_keys(b);
-    if ((int)(blockIdx.x * kMassThreads) >= n) return;
-    const size_t bh = (size_t)b * a.v.n_kv + h;
-    for (int r = threadIdx.x; r < R; r += kMassThreads) st_s[r] = a.stats[bh * R + r];
-    __syncthreads();
-    const int key = blockIdx.x * kMassThreads + threadIdx.x;
-    if (key >= n) return;
-    const float* sc = a.scores + (bh * a.v.capacity() + key) * a.s_ld;
-    // a row block's scores exist up to its last token's entry only
-    float sum = 0.f;
-    const int e0 = a.entry0[b];
-    for (int r = 0; r < R; r += 2) {
-        const float2 x = __ldcg(reinterpret_cast<const float2*>(sc + r));
-        const float2 s0 = st_s[r], s1 = r + 1 < R ? st_s[r + 1] : make_float2(0.f, 0.f);
-        if (s0.y != 0.f && key <= e0 + r / a.group) sum += q8_ex2(x.x - s0.x) * s0.y;
-        if (s1.y != 0.f && key <= e0 + (r + 1) / a.group) sum += q8_ex2(x.y - s1.x) * s1.y;
+    const int n = a.n_keys(b), e0 = a.entry0[b], key0 = blockIdx.x * kMassThreads * kMassKeys + threadIdx.x;
+    if ((int)(blockIdx.x * kMassThreads * kMassKeys) >= n) return;
+    const size_t bh = (size_t)b * a.v.n_kv + h, cap = a.v.capacity();
+    float old[kMassKeys], sum[kMassKeys];
+    float2 x0[kMassKeys];
+    const float* sc = a.scores + (bh * cap + key0) * a.s_ld;
+#pragma unroll
+    for (int k = 0; k < kMassKeys; ++k) {
+        const int key = key0 + k * kMassThreads;
+        sum[k] = 0.f;
+        old[k] = key < n ? mass[bh * cap + key] : 0.f;
+        x0[k] = key < n ? __ldcg(reinterpret_cast<const float2*>(sc + (size_t)k * kMassThreads * a.s_ld))
+                        : make_float2(0.f, 0.f);
     }
-    mass[bh * a.v.capacity() + key] += sum;
+    for (int r = threadIdx.x; r <= R; r += kMassThreads) st_s[r] = r < R ? a.stats[bh * R + r] : make_float2(0.f, 0.f);
+    __syncthreads();
+    for (int r = 0; r < R; r += 2) {
+        const float2 s0 = st_s[r], s1 = st_s[r + 1];
+        const int l0 = e0 + r / a.group, l1 = e0 + (r + 1) / a.group;     // a row's scores exist up to its own entry
+#pragma unroll
+        for (int k = 0; k < kMassKeys; ++k) {
+            const int key = key0 + k * kMassThreads;
+            if (key >= n) continue;
+            const float2 x = r == 0 ? x0[k]
+                                    : __ldcg(reinterpret_cast<const float2*>(sc + (size_t)k * kMassThreads * a.s_ld + r));
+            if (s0.y != 0.f && key <= l0) sum[k] += q8_ex2(x.x - s0.x) * s0.y;
+            if (s1.y != 0.f && key <= l1) sum[k] += q8_ex2(x.y - s1.x) * s1.y;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kMassKeys; ++k)
+        if (key0 + k * kMassThreads < n) mass[bh * cap + key0 + k * kMassThreads] = old[k] + sum[k];
 }
 
-template <int D, int NT, int RG>
+template <int D, int NT, bool PLO, bool PAIR>
 cudaError_t launch_decode(const Q8AttnArgs& a, dim3 grid, cudaStream_t st) {
-    using Geo = QdGeo<NT, RG>;
-    static_assert(Geo::SMEM >= (size_t)kQdKG * Geo::ROWS * (D + 2) * sizeof(float), "the merge fits the ring");
-    const cudaError_t e = allow_smem_max_once<q8_decode_kernel<D, NT, RG>>();
+    const cudaError_t e = allow_smem_max_once<q8_decode_kernel<D, NT, PLO, PAIR>>();
     if (e != cudaSuccess) return e;
-    return launch_pdl(q8_decode_kernel<D, NT, RG>, grid, dim3(Geo::THREADS), Geo::SMEM, st, a);
+    return launch_pdl(q8_decode_kernel<D, NT, PLO, PAIR>, grid, dim3(kQdThreads), kQdSmem, st, a);
+}
+template <int D, bool PLO>
+cudaError_t launch_decode_rows(const Q8AttnArgs& a, int R, dim3 grid, cudaStream_t st) {
+    return R <= 4 ? launch_decode<D, 1, PLO, true>(a, grid, st)
+                  : R <= 8 ? launch_decode<D, 1, PLO, false>(a, grid, st) : launch_decode<D, 2, PLO, false>(a, grid, st);
 }
 
-// Query rows a CTA: 8, 16 or 32.
-int row_block(int R) { return R <= 8 ? 8 : R <= 16 ? 16 : 32; }
+// Query rows a CTA: 8 or 16.
+int row_block(int R) { return R <= 8 ? 8 : 16; }
 
-// Keys per split (a multiple of 128) where the caller names none: one wave of
-// two CTAs an SM over (sequence, head, split), from 256 keys up to the staged
-// limit.  It depends on the batch, the heads and the capacity only, so a
-// sequence's verify and decode calls share it.
-int default_split(int batch, int n_kv, int capacity) {
+// Keys per split (a multiple of 256: whole units of all 8 warps) where the
+// caller names none: one wave of two CTAs an SM over (sequence, head, split),
+// and at least 256 KB of codes a split.  A CTA costs about 8 us apart from its
+// stream (measured on B200 over one sequence of 262144 entries: 37 splits a
+// head 98 us, 256 splits 147 us) and streams 256 KB in about as long.  It
+// depends on the batch, the heads and the capacity only, so a sequence's verify
+// and decode calls share it.
+int default_split(int batch, int n_kv, int d, int capacity) {
     const int ctas = std::max(1, 2 * 148 / std::max(1, batch * n_kv));
     const int keys = (int)(((long long)capacity + ctas - 1) / ctas);
-    return std::min(std::max((keys + 127) / 128 * 128, 256), kQdMaxSplit);
+    return std::max((keys + 255) / 256 * 256, kQdMinBytes / (2 * d));
 }
 
-int pick_split(int batch, int n_kv, int capacity, int split_keys) {
-    return split_keys > 0 ? split_keys : default_split(batch, n_kv, capacity);
+int pick_split(dkv_dims dims, int capacity, int split_keys) {
+    return split_keys > 0 ? split_keys : default_split(dims.batch, dims.n_kv, dims.d, capacity);
 }
 
 size_t decode_work(dkv_dims dims, int R, int capacity, int split, bool mass, Q8AttnArgs* a, Arena* ar) {
@@ -533,7 +648,7 @@ extern "C" size_t dkv_q8_attn_work_bytes(dkv_dims dims, int group, int T, int ca
     const long long R = (long long)T * group;
     if (R > (1 << 24)) return 0;
     if (R > kQ8MaxRows) return attn_q8_prefill_work(dims, group, T, capacity);
-    return decode_work(dims, (int)R, capacity, pick_split(dims.batch, dims.n_kv, capacity, split_keys), note_mass != 0,
+    return decode_work(dims, (int)R, capacity, pick_split(dims, capacity, split_keys), note_mass != 0,
                        nullptr, nullptr);
 }
 
@@ -548,8 +663,8 @@ extern "C" int dkv_q8_attn(const dkv_q8_cache* cache, dkv_dims dims, int layer, 
     DKV_REQUIRE(((uintptr_t)q & 15) == 0 && ((uintptr_t)out & 15) == 0 && ((uintptr_t)work & 15) == 0,
                 "dkv_q8_attn: q, out and work must be 16-byte aligned");
     const int R = T * group, cap = a.v.capacity();
-    DKV_REQUIRE(split_keys <= kQdMaxSplit && (split_keys <= 0 || split_keys % 128 == 0),
-                "dkv_q8_attn: split_keys %d (a multiple of 128 up to %d, or 0)", split_keys, kQdMaxSplit);
+    DKV_REQUIRE(split_keys <= 0 || split_keys % 128 == 0, "dkv_q8_attn: split_keys %d (a multiple of 128, or 0)",
+                split_keys);
     DKV_UNSUPPORTED(!mass || R <= kQ8MaxRows, "dkv_q8_attn: the mass of %d query rows a head (at most %d)", R,
                     kQ8MaxRows);
     a.group = group;
@@ -570,7 +685,7 @@ extern "C" int dkv_q8_attn(const dkv_q8_cache* cache, dkv_dims dims, int layer, 
                     "dkv_q8_attn: work buffer of %zu bytes is too small", work_bytes);
         return attn_q8_prefill(a, dims, work, work_bytes, st);
     }
-    a.split = pick_split(dims.batch, dims.n_kv, cap, split_keys);
+    a.split = pick_split(dims, cap, split_keys);
     DKV_REQUIRE(work && work_bytes >= decode_work(dims, R, cap, a.split, mass != nullptr, nullptr, nullptr),
                 "dkv_q8_attn: work buffer of %zu bytes is too small", work_bytes);
     Arena ar(work, work_bytes);
@@ -582,16 +697,15 @@ extern "C" int dkv_q8_attn(const dkv_q8_cache* cache, dkv_dims dims, int layer, 
     const dim3 grid((unsigned)a.n_splits, (unsigned)dims.n_kv, (unsigned)(dims.batch * a.n_rb));
     ProfScope ps(DKV_PROF_ATTN_FULL, 0.0, st);
     cudaError_t e;
-    const int rb = row_block(R);
+    const bool plo = out_dtype == DKV_F32;
     if (dims.d == 128)
-        e = rb == 8 ? launch_decode<128, 1, 1>(a, grid, st)
-                    : rb == 16 ? launch_decode<128, 2, 1>(a, grid, st) : launch_decode<128, 2, 2>(a, grid, st);
+        e = plo ? launch_decode_rows<128, true>(a, R, grid, st) : launch_decode_rows<128, false>(a, R, grid, st);
     else
-        e = rb == 8 ? launch_decode<64, 1, 1>(a, grid, st)
-                    : rb == 16 ? launch_decode<64, 2, 1>(a, grid, st) : launch_decode<64, 2, 2>(a, grid, st);
+        e = plo ? launch_decode_rows<64, true>(a, R, grid, st) : launch_decode_rows<64, false>(a, R, grid, st);
     DKV_CUDA(e);
     if (mass)
-        DKV_CUDA(launch_pdl(q8_mass_kernel, dim3((unsigned)((cap + kMassThreads - 1) / kMassThreads), (unsigned)dims.n_kv, (unsigned)dims.batch),
+        DKV_CUDA(launch_pdl(q8_mass_kernel, dim3((unsigned)((cap + kMassThreads * kMassKeys - 1) / (kMassThreads * kMassKeys)), (unsigned)dims.n_kv,
+                                 (unsigned)dims.batch),
                             dim3(kMassThreads), 0, st, a, mass));
     return DKV_OK;
 }

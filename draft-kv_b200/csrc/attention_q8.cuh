@@ -58,66 +58,65 @@ DKV_DEV void q8_store2(const Q8AttnArgs& a, int b, int h, int gr, int n_tok, int
 }
 
 // After a CTA has stored its split's partial rows (max in log2 units, sum,
-// unnormalised O) of row block `bhr`, the last CTA to arrive merges all splits
-// in split order (empty ones skipped), writes the outputs and returns true
-// with the merged max / sum in ms / ls.  wq: shared memory the caller no longer
-// needs, for the per-(split, row) weights when they fit.
+// unnormalised O; an empty split has max -infinity and no O) of row block
+// `bhr`, the last CTA to arrive merges all splits and writes the outputs (and
+// the rows' stats).  A thread merges an element pair on its own, online in
+// split order with kMergeQ splits' loads in flight: no barrier, one round of
+// loads up to kMergeQ splits.
 template <int D, int RB>
-DKV_DEV bool q8_merge_splits(const Q8AttnArgs& a, size_t bhr, int b, int h, int rbase, int R, int n_tok, float* wq,
-                             size_t wq_bytes, float* ms, float* ls) {
-    constexpr int PS = D + 2;
+DKV_DEV void q8_merge_splits(const Q8AttnArgs& a, size_t bhr, int b, int h, int rbase, int R, int n_tok) {
+    constexpr int PS = D + 2, kMergeQ = 16;
     __shared__ int is_last;
-    __threadfence();
-    __syncthreads();
+    __syncthreads();                     // the CTA's partials are stored
     if (threadIdx.x == 0) {
         unsigned* tk = a.tickets + bhr;
+        __threadfence();                 // (cumulative: the other threads' stores too, by the barrier)
         is_last = atomicAdd(tk, 1u) == (unsigned)(a.n_splits - 1);
         if (is_last) *tk = 0u;
+        __threadfence();
     }
     __syncthreads();
-    if (!is_last) return false;
-    __threadfence();
+    if (!is_last) return;
     const int ns = a.n_splits;
     const float* parts = a.part + bhr * ns * (size_t)RB * PS;
-    const bool fit = (size_t)ns * RB * sizeof(float) <= wq_bytes;
-    for (int r = threadIdx.x; r < R; r += blockDim.x) {
-        float M = -INFINITY, L = 0.f;
-#pragma unroll 8
-        for (int q = 0; q < ns; ++q) M = fmaxf(M, __ldcg(parts + ((size_t)q * RB + r) * PS));
-#pragma unroll 8
-        for (int q = 0; q < ns; ++q) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(parts + ((size_t)q * RB + r) * PS));
-            const float w = ml.x == -INFINITY ? 0.f : q8_ex2(ml.x - M);
-            if (w != 0.f) L += ml.y * w;
-            if (fit) wq[(size_t)q * RB + r] = w;
-        }
-        ms[r] = M;
-        ls[r] = L;
-    }
-    __syncthreads();
     for (int i = threadIdx.x; i < R * (D / 2); i += blockDim.x) {
         const int r = i / (D / 2), e = i % (D / 2) * 2;
-        const float M = ms[r];
-        float x0 = 0.f, x1 = 0.f;
-#pragma unroll 8
-        for (int q = 0; q < ns; ++q) {
-            const float* at = parts + ((size_t)q * RB + r) * PS;
-            float w;
-            if (fit) {
-                w = wq[(size_t)q * RB + r];
-            } else {
-                const float mq = __ldcg(at);
-                w = mq == -INFINITY ? 0.f : q8_ex2(mq - M);
+        float M = -INFINITY, L = 0.f, x0 = 0.f, x1 = 0.f;
+        for (int q0 = 0; q0 < ns; q0 += kMergeQ) {
+            float2 ml[kMergeQ], y[kMergeQ];
+#pragma unroll
+            for (int k = 0; k < kMergeQ; ++k) {
+                ml[k] = make_float2(-INFINITY, 0.f);
+                y[k] = make_float2(0.f, 0.f);
+                if (q0 + k < ns) {
+                    const float* at = parts + ((size_t)(q0 + k) * RB + r) * PS;
+                    ml[k] = __ldcg(reinterpret_cast<const float2*>(at));
+                    y[k] = __ldcg(reinterpret_cast<const float2*>(at + 2 + e));
+                }
             }
-            if (w == 0.f) continue;      // an empty split has no O
-            const float2 y = __ldcg(reinterpret_cast<const float2*>(at + 2 + e));
-            x0 += y.x * w;
-            x1 += y.y * w;
+            float m = M;
+#pragma unroll
+            for (int k = 0; k < kMergeQ; ++k) m = fmaxf(m, ml[k].x);
+            if (m == -INFINITY) continue;
+            const float al = M == -INFINITY ? 0.f : q8_ex2(M - m);
+            M = m;
+            L *= al;
+            x0 *= al;
+            x1 *= al;
+#pragma unroll
+            for (int k = 0; k < kMergeQ; ++k) {
+                if (ml[k].x == -INFINITY) continue;        // (its O was never written)
+                const float w = q8_ex2(ml[k].x - m);
+                L += ml[k].y * w;
+                x0 += y[k].x * w;
+                x1 += y[k].y * w;
+            }
         }
-        const float L = ls[r];
         q8_store2<D>(a, b, h, rbase + r, n_tok, e, L == 0.f ? 0.f : x0 / L, L == 0.f ? 0.f : x1 / L);
+        if (e == 0 && a.stats)
+            a.stats[((size_t)b * a.v.n_kv + h) * (a.T * a.group) + rbase + r] =
+                make_float2(M, L == 0.f || (rbase + r) / a.group >= n_tok ? 0.f : 1.f / L);
     }
-    return true;
 }
 
 int attn_q8_prefill(Q8AttnArgs& a, dkv_dims dims, void* work, size_t work_bytes, cudaStream_t st);

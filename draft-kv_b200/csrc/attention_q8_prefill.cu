@@ -76,7 +76,6 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
     __shared__ __align__(8) uint64_t k_full[kQpNst], k_empty[kQpNst], v_full[kQpNst], v_empty[kQpNst];
     __shared__ __align__(8) uint64_t s_full[2], p_full[2], o_done, drain;
     __shared__ uint32_t tmem_slot;
-    __shared__ float ms[kQpRows], ls[kQpRows];
     __shared__ int32_t page_s[kQpSplit / 16];
     __shared__ int8_t ek_s[kQpSplit / 16], ev_s[kQpSplit / 16];      // block exponents
     __shared__ uint32_t bad_s[kQpSplit / kQpKeys / 4];               // 8 bits a key tile: 16-key groups not to be seen
@@ -94,7 +93,6 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
     const int r0 = rb * kQpRows, R = min(kQpRows, a.T * G - r0);
     const size_t bhr = ((size_t)b * v.n_kv + h) * a.n_rb + rb;
     const bool alone = a.n_splits == 1;
-    constexpr size_t kWq = (size_t)Geo::V0 + kQpNst * Geo::KVB;
 
     pdl_trigger();
     pdl_wait();
@@ -114,7 +112,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
         }
         for (int r = threadIdx.x; r < R; r += kQpThreads)
             *reinterpret_cast<float2*>(a.part + ((bhr * a.n_splits + s) * kQpRows + r) * PS) = make_float2(-INFINITY, 0.f);
-        q8_merge_splits<D, kQpRows>(a, bhr, b, h, r0, R, n_tok, reinterpret_cast<float*>(sm), kWq, ms, ls);
+        q8_merge_splits<D, kQpRows>(a, bhr, b, h, r0, R, n_tok);
         return;
     }
     if (threadIdx.x == 0) {
@@ -488,7 +486,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
         tc_fence_after();
         tmem_dealloc(tmem, kQpTmemCols);
     }
-    if (!alone) q8_merge_splits<D, kQpRows>(a, bhr, b, h, r0, R, n_tok, reinterpret_cast<float*>(sm), all_ok ? kWq : 0, ms, ls);
+    if (!alone) q8_merge_splits<D, kQpRows>(a, bhr, b, h, r0, R, n_tok);
 }
 
 // Keys per split: the whole capacity up to 16384 keys; where the row blocks

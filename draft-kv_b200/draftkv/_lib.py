@@ -124,11 +124,12 @@ _SIGS = {
 }
 
 _lib: C.CDLL | None = None
+_device_seen = False
 
 
 def load(require_device: bool = True) -> C.CDLL:
     """The loaded library; raises DraftKVError when it cannot be used."""
-    global _lib
+    global _lib, _device_seen
     if _lib is None:
         if not LIB_PATH.exists():
             raise DraftKVError(
@@ -140,10 +141,11 @@ def load(require_device: bool = True) -> C.CDLL:
             fn.restype = res
             fn.argtypes = args
         _lib = lib
-    if require_device:
+    if require_device and not _device_seen:
         import torch
         if not torch.cuda.is_available():
             raise DraftKVError("draftkv_b200 needs a CUDA device (B200, sm_100a); none is visible")
+        _device_seen = True
     return _lib
 
 
@@ -188,5 +190,10 @@ def pack_weight(w):
 
 
 def stream_ptr() -> int:
+    """The current stream of the current device (the raw getter where torch has
+    it: a Stream object costs several microseconds a call)."""
     import torch
-    return torch.cuda.current_stream().cuda_stream
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    if raw is None or not torch.cuda.is_initialized():
+        return torch.cuda.current_stream().cuda_stream
+    return raw(torch.cuda.current_device())

@@ -40,7 +40,7 @@ def tile_bytes(d_head: int):
 
 
 def _check_i32(name: str, t, shape, device) -> None:
-    if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.device != device:
+    if t.dtype is not torch.int32 or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)} on {device}")
 
 
@@ -134,12 +134,11 @@ class Q8KVCache(PagedKVCache):
         """Bytes of the pool (codes and scales)."""
         return self.codes.numel() + self.scale.numel() * 4
 
-    def _workspace(self, T: int, group: int, split_keys: int, note_mass: bool):
+    def _workspace(self, T: int, group: int, split_keys: int, note_mass: bool, stream: int):
         """The attention scratch of a call shape: zero when made, left ready by
         each call, one per stream (calls on one stream run in order).  Inside a
         stream capture a fresh one, cleared by the graph itself, belongs to the
         graph."""
-        stream = _lib.stream_ptr()
         key = (T, group, split_keys, note_mass, stream)
         w = self._work.get(key)
         if w is None:
@@ -190,7 +189,7 @@ class Q8KVCache(PagedKVCache):
         return (self.batch, self.n_heads, self.capacity_tokens)
 
     def _check_mass(self, mass) -> None:
-        if mass is not None and (mass.dtype != torch.float32 or tuple(mass.shape) != self._mass_shape()
+        if mass is not None and (mass.dtype is not torch.float32 or mass.shape != self._mass_shape()
                                  or not mass.is_contiguous() or mass.device != self.device):
             raise ValueError(f"mass must be a contiguous float32 tensor of shape {self._mass_shape()} on {self.device}")
 
@@ -228,11 +227,12 @@ class Q8KVCache(PagedKVCache):
             raise ValueError("attention writes bf16 or fp32")
         if T == 0:
             return out
+        stream = _lib.stream_ptr()
         if work is None:
-            work = self._workspace(T, group, split_keys, mass is not None)
+            work = self._workspace(T, group, split_keys, mass is not None, stream)
         _lib.call("dkv_q8_attn", self.struct(), self._dims, layer, group, T, q.data_ptr(), entry0.data_ptr(),
                   _lib.ptr(n_rows), out.data_ptr(), dtype_code(out.dtype), split_keys, _lib.ptr(mass), work.data_ptr(),
-                  work.numel(), _lib.stream_ptr())
+                  work.numel(), stream)
         return out
 
     def evict_rows(self, layer: int, n, budget, out_table, mass, pos=None, sink: int = 0, recent: int = 0,

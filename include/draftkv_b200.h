@@ -285,8 +285,8 @@ DKV_API int dkv_q8_read(const dkv_q8_cache* cache, dkv_dims dims, int b, int lay
  * mass [batch][n_kv][capacity] (NULL: not wanted; T * group <= 64): adds to
  * every seen entry its softmax weights, summed over the call's rows.
  * Up to 64 query rows (T * group) a row's result does not depend on T or on
- * the other rows, bit for bit.  split_keys: keys per split, a multiple of 128
- * up to 8192, or 0 for a rule on (batch, n_kv, capacity).
+ * the other rows, bit for bit.  split_keys: keys per split, a multiple of 128,
+ * or 0 for a rule on (batch, n_kv, capacity).
  * The work buffer must be zero when first used, is left ready for the next
  * call, and must not serve two calls that may run at the same time (two
  * streams, two captured graphs replayed side by side). */

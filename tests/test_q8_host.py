@@ -75,7 +75,7 @@ def test_bad_arguments_are_refused(lib):
            append(lib, dt=7), append(lib, rows=-1), append(lib, rows=65),
            attn(lib, layer=2), attn(lib, q=None), attn(lib, e0=None), attn(lib, out=None), attn(lib, dt=7),
            attn(lib, group=0), attn(lib, T=0), attn(lib, q=P + 4), attn(lib, out=P + 2), attn(lib, split=100),
-           attn(lib, split=16384), attn(lib, work=None), attn(lib, nbytes=64),
+           attn(lib, work=None), attn(lib, nbytes=64),
            evict(lib, n=None), evict(lib, mass=None), evict(lib, mass_out=None), evict(lib, mass_out=P),
            evict(lib, table=None), evict(lib, kept=None), evict(lib, sink=-1), evict(lib, recent=-1), evict(lib, pages=0),
            evict(lib, pages=5), evict(lib, pos=P), evict(lib, pos=P, pos_out=P),
