@@ -6,19 +6,24 @@
 // memory), with the cache's codes turned into f16 operands on the way:
 //   warps 8-11 -- converters: a 128-key tile's codes come from global memory
 //     straight into registers, one tile ahead (16-byte fragments, 512 B a warp
-//     and load), are widened e4m3 -> f16 (exact), multiplied by a power of two
-//     and stored in the swizzled K-major layout the MMA reads.  V's bytes are
-//     already dim-major, so V^T needs no transpose.  2 x 32 KB K and V rings;
+//     and load), are widened e4m3 -> f16 (exact) and stored with 16-byte stores
+//     in the swizzled K-major layout the MMA reads.  2 x 32 KB K and V rings;
 //   warp 12 -- tensor memory, and lane 0 issues the MMAs: per key tile j and
 //     query tile t, O_t += P_t(j-1) V(j-1), then S_t(j) = Q_t K_j^T;
 //   warps 0-3 / 4-7 -- softmax of query tiles A / B, one row a thread.
-// Rounding: the block scales are powers of two, so an operand is exactly
-// code * 2^(e - e_max + 6) with e_max the largest block exponent of the CTA's
-// key range (values 2^-30 below the range's largest go to zero); queries are
-// one f16 number each (2^-12 of the row's largest), probabilities too, biased
-// by 2^6 so that f16 keeps 2^-30 of the max; max, sum and O are fp32.
-// Bound by the tensor cores and the softmax warps: 4 * 128 * 128 * d MACs a
-// key tile against 128 * 2 d bytes.
+// The order of a contraction is free, so both operands of each product take the
+// order in which a lane's bytes lie: dims are permuted alike in Q and K
+// (qp_dim), keys alike in S, P and V (qp_key: a tile's column c belongs to the
+// 16-token group (c >> 6) * 4 + ((c >> 2) & 3)).
+// Block scales never touch the operands: K's multiplies the fp32 score, V's
+// (over the largest of the CTA's key range) is added to the exponent of the
+// probability that enters the product, and divided out of the row sum again; V
+// blocks more than 2^20 smaller are scaled as f16 numbers beyond that.
+// Rounding: queries are one f16 number each (2^-12 of the row's largest),
+// probabilities too, biased by 2^6 so that f16 keeps 2^-30 of the max; max, sum
+// and O are fp32.
+// Bound by the softmax warps and the tensor cores: 4 * 128 * 128 * d MACs a key
+// tile against 128 * 2 d bytes.
 // Every mbarrier wait is bounded (error word 0x80).
 #include <algorithm>
 
@@ -38,6 +43,18 @@ constexpr int kQpSplit = 16384;         // most keys a split has (page ids stage
 constexpr int kQpMinSplit = 2048;
 constexpr float kQpLazy = 8.f;
 constexpr int kQpBias = 6;
+constexpr int kQpDown = -20;            // V block exponents below the largest that probabilities carry
+
+// Dim of element i (0..7) of a row's 16-byte unit u (of the d / 8): what lane
+// t = (u & 7) >> 1 of a fragment of block 2 (u >> 3) + (u & 1) holds.
+__host__ __device__ constexpr int qp_dim(int u, int i) {
+    return (2 * (u >> 3) + (u & 1)) * 32 + (i >> 2) * 16 + ((i >> 1) & 1) * 8 + 2 * ((u & 7) >> 1) + (i & 1);
+}
+// Key (0..127) of a tile's column c: 16-byte unit 2 t + pair of a 64-key half,
+// 4 tokens of each of the pair's groups.
+__host__ __device__ constexpr int qp_key(int c) {
+    return (c >> 6) * 64 + ((c >> 3) & 1) * 32 + ((c >> 2) & 1) * 16 + ((c >> 1) & 1) * 8 + 2 * ((c >> 4) & 3) + (c & 1);
+}
 
 template <int D>
 struct QpGeo {
@@ -77,9 +94,12 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
     __shared__ __align__(8) uint64_t s_full[2], p_full[2], o_done, drain;
     __shared__ uint32_t tmem_slot;
     __shared__ int32_t page_s[kQpSplit / 16];
-    __shared__ int8_t ek_s[kQpSplit / 16], ev_s[kQpSplit / 16];      // block exponents
+    // per 16-key group: K scale, V exponent below the largest (at least kQpDown), 2^-that, and what of
+    // the V scale is left for the operand (1 but for far smaller blocks)
+    __shared__ __align__(16) float kf_s[kQpSplit / 16], dv_s[kQpSplit / 16], iv_s[kQpSplit / 16];
+    __shared__ int8_t ev_s[kQpSplit / 16];
     __shared__ uint32_t bad_s[kQpSplit / kQpKeys / 4];               // 8 bits a key tile: 16-key groups not to be seen
-    __shared__ int emax_s[2];
+    __shared__ int emax_s;
 
     const Q8View& v = a.v;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -130,7 +150,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
         mbar_init(&drain, 1);
         fence_barrier_init();
         fence_async_shared();
-        emax_s[0] = emax_s[1] = kQ8ExpMin;
+        emax_s = kQ8ExpMin;
     }
     for (int i = threadIdx.x; i < (ntiles + 3) / 4; i += kQpThreads) bad_s[i] = 0u;
     if (warp == 12) tmem_alloc(&tmem_slot, kQpTmemCols);
@@ -138,99 +158,107 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
-    // page ids and exponents of the key range; keys of a bad page are not seen
-    const int n_pg = (kend - k0 + v.page - 1) >> v.page_shift;
-    for (int i = threadIdx.x; i < n_pg; i += kQpThreads) {
-        const int pid = __ldg(v.row(b) + (k0 >> v.page_shift) + i);
+    // per 16-key group of the key range: page id and scales; keys of a bad page are not seen
+    const int n_grp = (kend - k0 + 15) / 16;
+    for (int i = threadIdx.x; i < ntiles * 8; i += kQpThreads) {
+        const int pid = i < n_grp ? __ldg(v.row(b) + ((k0 + i * 16) >> v.page_shift)) : -1;
         const bool ok = v.ok(pid);
-        page_s[i] = ok ? pid : -1;
-        int ek = kQ8ExpMin, ev = kQ8ExpMin;
+        float2 sc = make_float2(1.f, 1.f);
+        int ev = kQ8ExpMin;
         if (ok) {
-            const float2 sc = *reinterpret_cast<const float2*>(v.scale + v.scale_at(pid, h, 0));
-            ek = min(max(q8_scale_exp(sc.x), kQ8ExpMin), kQ8ExpMax);
+            sc = __ldg(reinterpret_cast<const float2*>(v.scale + v.scale_at(pid, h, 0)));
             ev = min(max(q8_scale_exp(sc.y), kQ8ExpMin), kQ8ExpMax);
-        } else {
+            atomicMax(&emax_s, ev);
+        } else if (i < n_grp) {
             atomicOr(a.err, kErrQ8Page);
-            for (int g = 0; g < v.page / 16; ++g) {
-                const int grp = i * (v.page / 16) + g;
-                if (grp < ntiles * 8) atomicOr(&bad_s[grp >> 5], 1u << (grp & 31));
-            }
+            atomicOr(&bad_s[i >> 5], 1u << (i & 31));
         }
-        ek_s[i] = (int8_t)ek;
+        page_s[i] = ok ? pid : -1;
+        kf_s[i] = sc.x;
         ev_s[i] = (int8_t)ev;
-        atomicMax(&emax_s[0], ek);
-        atomicMax(&emax_s[1], ev);
     }
     __syncthreads();
-    const int ekm = emax_s[0], evm = emax_s[1];
+    const int evm = emax_s;
+    for (int i = threadIdx.x; i < ntiles * 8; i += kQpThreads) {
+        const int dv = max((int)ev_s[i] - evm, kQpDown);
+        dv_s[i] = (float)dv;
+        iv_s[i] = q8_pow2(-dv);
+    }
+    __syncthreads();
 
     bool ok = true;
     if (warp >= 8 && warp < 12) {
-        // ---------------- converters.  Warp w takes 8 of the 32 (or 16) 512-byte
-        // K blocks of a tile, and of V: block x = group x / (D / 32), dims 32 (x % (D / 32)) ..
-        constexpr int NJ = D / 32, NB = 8 * NJ / 4;               // blocks a warp
+        // ---------------- converters: warp w takes groups 2 w and 2 w + 1 of a tile
+        constexpr int NJ = D / 32;                                // 512-byte blocks a group and side
         const int w = warp - 8, g = lane >> 2, t = lane & 3;
-        uint4 kr[NB], vr[NB];
-        auto page_of = [&](int j, int grp) { return ((j * kQpKeys + grp * 16) >> v.page_shift); };
-        auto load = [&](int j, int i, uint4 (&r)[NB]) {
+        uint4 kr[2][NJ], vr[2][NJ];
+        auto load = [&](int j, int i, uint4 (&r)[2][NJ]) {
 #pragma unroll
-            for (int u = 0; u < NB; ++u) {
-                const int x = w * NB + u, grp = x / NJ, blk = x % NJ;
-                const int key = j * kQpKeys + grp * 16;           // from k0
-                r[u] = make_uint4(0u, 0u, 0u, 0u);
-                if (j < ntiles && k0 + key < kend) {
-                    const int pid = page_s[page_of(j, grp)];
-                    if (pid >= 0)
-                        r[u] = __ldg(reinterpret_cast<const uint4*>(v.side(pid, h, i) +
-                                                                    (size_t)((k0 + key) & (v.page - 1)) * D + blk * 512 +
-                                                                    lane * 16));
+            for (int gb = 0; gb < 2; ++gb) {
+                const int grp = j * 8 + 2 * w + gb;               // from k0
+                const int pid = j < ntiles ? page_s[grp] : -1;
+                const uint8_t* at = v.side(max(pid, 0), h, i) + (size_t)((k0 + grp * 16) & (v.page - 1)) * D + lane * 16;
+#pragma unroll
+                for (int x = 0; x < NJ; ++x)
+                    r[gb][x] = pid >= 0 ? __ldg(reinterpret_cast<const uint4*>(at + x * 512)) : make_uint4(0u, 0u, 0u, 0u);
+            }
+        };
+        // row of key g (+8: row + 2) of group 2 w + gb, see qp_key; unit 2 t + (x & 1) of the 64-dim half x >> 1
+        auto put_k = [&](uint8_t* dst) {
+#pragma unroll
+            for (int gb = 0; gb < 2; ++gb) {
+                const int row = (w >> 1) * 64 + (2 * (g >> 1) + (w & 1)) * 8 + gb * 4 + (g & 1);
+#pragma unroll
+                for (int x = 0; x < NJ; ++x) {
+                    const uint4 f = kr[gb][x];
+                    uint4 a0, a1;
+                    q8_decode4(f.x, a0.x, a0.y);
+                    q8_decode4(f.z, a0.z, a0.w);
+                    q8_decode4(f.y, a1.x, a1.y);
+                    q8_decode4(f.w, a1.z, a1.w);
+                    uint8_t* at = dst + (x >> 1) * 16384 + row * 128;
+                    const int unit = 2 * t + (x & 1);
+                    *reinterpret_cast<uint4*>(at + ((unit ^ (row & 7)) << 4)) = a0;
+                    *reinterpret_cast<uint4*>(at + 256 + ((unit ^ ((row + 2) & 7)) << 4)) = a1;
                 }
             }
         };
-        // K: word q of a fragment is token g + 8 (q & 1), dims 32 blk + 16 (q >> 1) + {2t, 2t+1 | 2t+8, 2t+9}
-        auto put_k = [&](int j, uint8_t* dst) {
-#pragma unroll
-            for (int u = 0; u < NB; ++u) {
-                const int x = w * NB + u, grp = x / NJ, blk = x % NJ;
-                const int key = j * kQpKeys + grp * 16;
-                const uint32_t f = k0 + key < kend ? h2_pow2(ek_s[page_of(j, grp)] - ekm + kQpBias) : 0u;
-                const uint32_t ws[4] = {kr[u].x, kr[u].y, kr[u].z, kr[u].w};
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    uint32_t lo, hi;
-                    q8_decode4(ws[q], lo, hi);
-                    const int row = grp * 16 + g + 8 * (q & 1);
-                    const int unit = (blk * 4 + (q >> 1) * 2) & 7;
-                    uint8_t* at = dst + (blk >> 1) * 16384 + row * 128 + 4 * t;
-                    *reinterpret_cast<uint32_t*>(at + ((unit ^ (row & 7)) << 4)) = hmul2(lo, f);
-                    *reinterpret_cast<uint32_t*>(at + (((unit + 1) ^ (row & 7)) << 4)) = hmul2(hi, f);
-                }
-            }
-        };
-        // V: word q is dim 32 blk + 16 (q >> 1) + 8 (q & 1) + g, tokens {2t, 2t+1 | 2t+8, 2t+9}
+        // V: rows are dims 32 x + 8 q' + g; unit 2 t + (w & 1) of key half w >> 1 holds 4 tokens of each group
         auto put_v = [&](int j, uint8_t* dst) {
+            uint32_t vm[2], f[2];
+            bool plain = true;
 #pragma unroll
-            for (int u = 0; u < NB; ++u) {
-                const int x = w * NB + u, grp = x / NJ, blk = x % NJ;
-                const int key = j * kQpKeys + grp * 16, left = kend - k0 - key;      // live tokens of the group
-                const uint32_t f = left > 0 ? h2_pow2(ev_s[page_of(j, grp)] - evm + kQpBias) : 0u;
+            for (int gb = 0; gb < 2; ++gb) {
+                const int grp = j * 8 + 2 * w + gb, left = kend - k0 - grp * 16;
                 // bytes of tokens that are not there as zeros (their weight is 0, but 0 x NaN would not be)
-                uint32_t vm = 0xffffffffu;
-                if (left < 16)
-                    vm = (2 * t < left ? 0xffu : 0u) | (2 * t + 1 < left ? 0xff00u : 0u) |
-                         (2 * t + 8 < left ? 0xff0000u : 0u) | (2 * t + 9 < left ? 0xff000000u : 0u);
-                const uint32_t ws[4] = {vr[u].x, vr[u].y, vr[u].z, vr[u].w};
+                vm[gb] = left >= 16 ? 0xffffffffu
+                                    : (2 * t < left ? 0xffu : 0u) | (2 * t + 1 < left ? 0xff00u : 0u) |
+                                          (2 * t + 8 < left ? 0xff0000u : 0u) | (2 * t + 9 < left ? 0xff000000u : 0u);
+                const int rest = min((int)ev_s[grp] - evm - kQpDown, 0);
+                f[gb] = h2_pow2(rest);
+                plain = plain && left >= 16 && rest == 0;
+            }
+            if (!plain) {
+#pragma unroll
+                for (int gb = 0; gb < 2; ++gb)
+#pragma unroll
+                    for (int x = 0; x < NJ; ++x) {
+                        uint4& r = vr[gb][x];
+                        r.x &= vm[gb], r.y &= vm[gb], r.z &= vm[gb], r.w &= vm[gb];
+                    }
+            }
+            auto word = [&](const uint4& r, int q) { return q == 0 ? r.x : q == 1 ? r.y : q == 2 ? r.z : r.w; };
+#pragma unroll
+            for (int x = 0; x < NJ; ++x)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    uint32_t lo, hi;
-                    q8_decode4(ws[q] & vm, lo, hi);
-                    const int row = blk * 32 + (q >> 1) * 16 + (q & 1) * 8 + g;
-                    const int unit = (grp * 2) & 7;
-                    uint8_t* at = dst + (grp >> 2) * (D * 128) + row * 128 + 4 * t;
-                    *reinterpret_cast<uint32_t*>(at + ((unit ^ (row & 7)) << 4)) = hmul2(lo, f);
-                    *reinterpret_cast<uint32_t*>(at + (((unit + 1) ^ (row & 7)) << 4)) = hmul2(hi, f);
+                    uint4 o;
+                    q8_decode4(word(vr[0][x], q), o.x, o.y);
+                    q8_decode4(word(vr[1][x], q), o.z, o.w);
+                    if (!plain) o.x = hmul2(o.x, f[0]), o.y = hmul2(o.y, f[0]), o.z = hmul2(o.z, f[1]), o.w = hmul2(o.w, f[1]);
+                    const int row = x * 32 + (q >> 1) * 16 + (q & 1) * 8 + g, unit = 2 * t + (w & 1);
+                    *reinterpret_cast<uint4*>(dst + (w >> 1) * (D * 128) + row * 128 + ((unit ^ (row & 7)) << 4)) = o;
                 }
-            }
         };
         load(0, 0, kr);
         load(0, 1, vr);
@@ -242,7 +270,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
                 ok = false;
                 break;
             }
-            put_k(j, sm + Geo::K0 + slot * Geo::KVB);
+            put_k(sm + Geo::K0 + slot * Geo::KVB);
             fence_async_shared();
             mbar_arrive(&k_full[slot]);
             load(j + 1, 0, kr);
@@ -326,7 +354,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t sb = lanes + (uint32_t)(t * 256), ob = sb + 128;
         const bool mine = cr < R && gr / G < n_tok;
-        float c;                                                  // scores = S * c (log2 units)
+        float c;                                                  // scores = S * c * (K scale), log2 units
         {
             // the row of Q as f16 of q * log2 e / sqrt(d) * 2^-x, x the row's exponent
             const float* qrow =
@@ -340,18 +368,19 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
                 }
             const int ex = min(max((int)(__float_as_uint(am * a.scale) >> 23) - 127, -100), 126);
             const float f = a.scale * q8_pow2(-ex);
-            c = q8_pow2(min(max(ex + ekm - kQpBias, -126), 127));
+            c = q8_pow2(ex);
             uint8_t* qt = sm + t * Geo::QT;
 #pragma unroll 4
             for (int u = 0; u < D / 8; ++u) {
-                float4 x0 = make_float4(0.f, 0.f, 0.f, 0.f), x1 = x0;
-                if (qrow) {
-                    x0 = __ldg(reinterpret_cast<const float4*>(qrow + 8 * u));
-                    x1 = __ldg(reinterpret_cast<const float4*>(qrow + 8 * u + 4));
-                }
+                uint32_t o[4] = {0u, 0u, 0u, 0u};
+                if (qrow)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 x = __ldg(reinterpret_cast<const float2*>(qrow + qp_dim(u, 2 * i)));
+                        o[i] = h2(x.x * f, x.y * f);
+                    }
                 *reinterpret_cast<uint4*>(qt + (u >> 3) * 16384 + rt * 128 + (((u & 7) ^ (rt & 7)) << 4)) =
-                    make_uint4(h2(x0.x * f, x0.y * f), h2(x0.z * f, x0.w * f), h2(x1.x * f, x1.y * f),
-                               h2(x1.z * f, x1.w * f));
+                    make_uint4(o[0], o[1], o[2], o[3]);
             }
             fence_async_shared();
             named_sync(1, kQpSoft + 32);
@@ -368,65 +397,85 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
             const int lc = lim - (k0 + j * kQpKeys);              // last live column
             const uint32_t bad = (bad_s[j >> 2] >> ((j & 3) * 8)) & 0xffu;
             const bool masked = lc < kQpKeys - 1 || bad != 0u;
-            auto mask = [&](int col, uint32_t& x) {
-                if (col > lc || ((bad >> (col >> 4)) & 1u)) x = __float_as_uint(-INFINITY);
+            auto mask = [&](int half, int col, uint32_t& x) {     // column 64 half + col
+                if (half * 64 + qp_key(col) > lc || ((bad >> (half * 4 + ((col >> 2) & 3))) & 1u)) x = __float_as_uint(-INFINITY);
             };
-            float mx[8];
+            // pass 1: the largest score, group by group (one factor a group)
+            float mn = -INFINITY;
+            const float4* kf = reinterpret_cast<const float4*>(kf_s + j * 8);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) mx[k] = -INFINITY;
+            for (int half = 0; half < 2; ++half) {
+                float mx[8];
 #pragma unroll
-            for (int cc = 0; cc < 4; ++cc) {
-                uint32_t sr[32];
-                tmem_ld32(sb + cc * 32, sr);
-                tmem_wait_ld();
-                if (masked) {
+                for (int k = 0; k < 8; ++k) mx[k] = -INFINITY;
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) mask(cc * 32 + e, sr[e]);
+                for (int cc = 0; cc < 2; ++cc) {
+                    uint32_t sr[32];
+                    tmem_ld32(sb + half * 64 + cc * 32, sr);
+                    tmem_wait_ld();
+                    if (masked) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) mask(half, cc * 32 + e, sr[e]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        const int k = 2 * ((e >> 2) & 3) + ((e >> 1) & 1);
+                        mx[k] = pf_max3(mx[k], __uint_as_float(sr[e]), __uint_as_float(sr[e + 1]));
+                    }
                 }
-#pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    const int k = 2 * cc + (e >> 4);
-                    mx[k] = pf_max3(mx[k], __uint_as_float(sr[e]), __uint_as_float(sr[e + 1]));
-                }
+                const float4 f = kf[half];
+                mn = pf_max3(mn, fmaxf(mx[0], mx[1]) * f.x, fmaxf(mx[2], mx[3]) * f.y);
+                mn = pf_max3(mn, fmaxf(mx[4], mx[5]) * f.z, fmaxf(mx[6], mx[7]) * f.w);
             }
-            const float mn = c * pf_max3(pf_max3(mx[0], mx[1], mx[2]), pf_max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7]));
+            mn *= c;
             float alpha = 1.f;
             if (mn > m + kQpLazy) {
                 alpha = pf_ex2(m - mn);                           // 0 from -infinity
                 m = mn;
             }
+            // pass 2: probabilities 2^(s - m + bias + dv), as f16 pairs into columns read before
             const float off = m == -INFINITY ? 0.f : (float)kQpBias - m;
-            const uint64_t cc2 = pf_pack2(c, c), oo = pf_pack2(off, off);
-            uint64_t sum2[2] = {0ull, 0ull};
+            l *= alpha;
             uint32_t sr[2][32];
 #pragma unroll 1
             for (int k = 0; k < 2; ++k) {
                 tmem_ld32(sb + 64 * k, sr[0]);
                 tmem_ld32(sb + 64 * k + 32, sr[1]);
+                const float4 f = kf[k], dv = *reinterpret_cast<const float4*>(dv_s + j * 8 + 4 * k);
+                const float4 iv = *reinterpret_cast<const float4*>(iv_s + j * 8 + 4 * k);
+                uint64_t cg[4], og[4], sum2[4] = {0ull, 0ull, 0ull, 0ull};
+                cg[0] = pf_pack2(c * f.x, c * f.x), cg[1] = pf_pack2(c * f.y, c * f.y);
+                cg[2] = pf_pack2(c * f.z, c * f.z), cg[3] = pf_pack2(c * f.w, c * f.w);
+                og[0] = pf_pack2(off + dv.x, off + dv.x), og[1] = pf_pack2(off + dv.y, off + dv.y);
+                og[2] = pf_pack2(off + dv.z, off + dv.z), og[3] = pf_pack2(off + dv.w, off + dv.w);
                 tmem_wait_ld();
                 uint32_t pk[32];
 #pragma unroll
                 for (int h3 = 0; h3 < 2; ++h3) {
                     if (masked) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) mask((2 * k + h3) * 32 + e, sr[h3][e]);
+                        for (int e = 0; e < 32; ++e) mask(k, h3 * 32 + e, sr[h3][e]);
                     }
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
+                        const int gi = (e >> 2) & 3;
                         float d0, d1;
-                        pf_unpack2(pf_fma2(pf_pack2(__uint_as_float(sr[h3][e]), __uint_as_float(sr[h3][e + 1])), cc2, oo),
+                        pf_unpack2(pf_fma2(pf_pack2(__uint_as_float(sr[h3][e]), __uint_as_float(sr[h3][e + 1])), cg[gi], og[gi]),
                                    d0, d1);
                         const float p0 = pf_ex2(d0), p1 = pf_ex2(d1);
-                        sum2[h3] = pf_add2(sum2[h3], pf_pack2(p0, p1));
+                        sum2[gi] = pf_add2(sum2[gi], pf_pack2(p0, p1));
                         pk[h3 * 16 + e / 2] = h2(p0, p1);
                     }
                 }
                 tmem_st32(sb + 32 * k, pk);
+                const float ivs[4] = {iv.x, iv.y, iv.z, iv.w};
+#pragma unroll
+                for (int gi = 0; gi < 4; ++gi) {
+                    float a0, a1;
+                    pf_unpack2(sum2[gi], a0, a1);
+                    l += (a0 + a1) * ivs[gi];
+                }
             }
-            float a0, a1, a2, a3;
-            pf_unpack2(sum2[0], a0, a1);
-            pf_unpack2(sum2[1], a2, a3);
-            l = l * alpha + ((a0 + a1) + (a2 + a3));
             if (j >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll 1
                 for (int c0 = 0; c0 < D; c0 += 32) {
@@ -450,8 +499,8 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
         float* mypart = alone ? nullptr : a.part + ((bhr * a.n_splits + s) * kQpRows + cr) * PS;
         if (l != l && m == -INFINITY) m = 0.f;     // NaN scores have no max: give the row one, so that its NaN comes out
         const bool live = ok && m != -INFINITY;
-        // O holds code * 2^(kQpBias - evm) units, l the probabilities' 2^kQpBias
-        const float un = q8_pow2(evm) * q8_pow2(-kQpBias);
+        // O is in units of 2^(evm - bias), l in units of 2^-bias
+        const float un = q8_pow2(evm);
         const float f = alone ? (live ? un / l : 0.f) : un * q8_pow2(-kQpBias);
         if (__all_sync(0xffffffffu, ok)) {
 #pragma unroll 1
