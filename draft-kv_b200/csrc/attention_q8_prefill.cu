@@ -18,7 +18,8 @@
 // Block scales never touch the operands: K's multiplies the fp32 score, V's
 // (over the largest of the CTA's key range) is added to the exponent of the
 // probability that enters the product, and divided out of the row sum again; V
-// blocks more than 2^20 smaller are scaled as f16 numbers beyond that.
+// blocks more than 2^20 smaller are brought to that scale (their values lie 2^-20
+// and more below the range's largest; what is rounded off, 2^-37 below).
 // Rounding: queries are one f16 number each (2^-12 of the row's largest),
 // probabilities too, biased by 2^6 so that f16 keeps 2^-30 of the max; max, sum
 // and O are fp32.
@@ -74,14 +75,12 @@ DKV_DEV uint32_t h2(float lo, float hi) {
     __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&v);
 }
-DKV_DEV uint32_t hmul2(uint32_t a, uint32_t b) {
-    __half2 r = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
-    return *reinterpret_cast<uint32_t*>(&r);
-}
-// 2^e twice as f16 (0 below 2^-24), e <= 15
-DKV_DEV uint32_t h2_pow2(int e) {
-    const float f = e < -24 ? 0.f : q8_pow2(e);
-    return h2(f, f);
+// Four codes times f (a power of two up to 1), rounded to codes again.
+DKV_DEV uint32_t rescaled(uint32_t w, float f) {
+    uint32_t lo, hi;
+    q8_decode4(w, lo, hi);
+    const float2 a = __half22float2(*reinterpret_cast<__half2*>(&lo)), b = __half22float2(*reinterpret_cast<__half2*>(&hi));
+    return q8_encode2(a.x * f, a.y * f) | (q8_encode2(b.x * f, b.y * f) << 16);
 }
 
 template <int D>
@@ -225,27 +224,24 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
         };
         // V: rows are dims 32 x + 8 q' + g; unit 2 t + (w & 1) of key half w >> 1 holds 4 tokens of each group
         auto put_v = [&](int j, uint8_t* dst) {
-            uint32_t vm[2], f[2];
-            bool plain = true;
+            // rare: bytes of tokens that are not there become zeros (their weight is
+            // 0, but 0 x NaN would not be), and blocks more than 2^20 below the
+            // largest are brought to that scale (rounded to e4m3 again)
 #pragma unroll
             for (int gb = 0; gb < 2; ++gb) {
                 const int grp = j * 8 + 2 * w + gb, left = kend - k0 - grp * 16;
-                // bytes of tokens that are not there as zeros (their weight is 0, but 0 x NaN would not be)
-                vm[gb] = left >= 16 ? 0xffffffffu
-                                    : (2 * t < left ? 0xffu : 0u) | (2 * t + 1 < left ? 0xff00u : 0u) |
-                                          (2 * t + 8 < left ? 0xff0000u : 0u) | (2 * t + 9 < left ? 0xff000000u : 0u);
-                const int rest = min((int)ev_s[grp] - evm - kQpDown, 0);
-                f[gb] = h2_pow2(rest);
-                plain = plain && left >= 16 && rest == 0;
-            }
-            if (!plain) {
-#pragma unroll
-                for (int gb = 0; gb < 2; ++gb)
+                const int rest = (int)ev_s[grp] - evm - kQpDown;
+                if (left < 16 || rest < 0) {
+                    const uint32_t vm = (2 * t < left ? 0xffu : 0u) | (2 * t + 1 < left ? 0xff00u : 0u) |
+                                        (2 * t + 8 < left ? 0xff0000u : 0u) | (2 * t + 9 < left ? 0xff000000u : 0u);
+                    const float f = q8_pow2(max(min(rest, 0), -126));
 #pragma unroll
                     for (int x = 0; x < NJ; ++x) {
                         uint4& r = vr[gb][x];
-                        r.x &= vm[gb], r.y &= vm[gb], r.z &= vm[gb], r.w &= vm[gb];
+                        r.x = rescaled(r.x & vm, f), r.y = rescaled(r.y & vm, f);
+                        r.z = rescaled(r.z & vm, f), r.w = rescaled(r.w & vm, f);
                     }
+                }
             }
             auto word = [&](const uint4& r, int q) { return q == 0 ? r.x : q == 1 ? r.y : q == 2 ? r.z : r.w; };
 #pragma unroll
@@ -255,7 +251,6 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
                     uint4 o;
                     q8_decode4(word(vr[0][x], q), o.x, o.y);
                     q8_decode4(word(vr[1][x], q), o.z, o.w);
-                    if (!plain) o.x = hmul2(o.x, f[0]), o.y = hmul2(o.y, f[0]), o.z = hmul2(o.z, f[1]), o.w = hmul2(o.w, f[1]);
                     const int row = x * 32 + (q >> 1) * 16 + (q & 1) * 8 + g, unit = 2 * t + (w & 1);
                     *reinterpret_cast<uint4*>(dst + (w >> 1) * (D * 128) + row * 128 + ((unit ^ (row & 7)) << 4)) = o;
                 }
@@ -396,10 +391,23 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
             tc_fence_after();
             const int lc = lim - (k0 + j * kQpKeys);              // last live column
             const uint32_t bad = (bad_s[j >> 2] >> ((j & 3) * 8)) & 0xffu;
-            const bool masked = lc < kQpKeys - 1 || bad != 0u;
-            auto mask = [&](int half, int col, uint32_t& x) {     // column 64 half + col
-                if (half * 64 + qp_key(col) > lc || ((bad >> (half * 4 + ((col >> 2) & 3))) & 1u)) x = __float_as_uint(-INFINITY);
-            };
+            if (__any_sync(0xffffffffu, lc < kQpKeys - 1 || bad != 0u)) {
+                // a row's last tiles, or a bad page: -infinity over what is not seen
+                // (kept out of the loops below: their code has to stay small)
+#pragma unroll 1
+                for (int cc = 0; cc < 4; ++cc) {
+                    uint32_t x[32];
+                    tmem_ld32(sb + 32 * cc, x);
+                    tmem_wait_ld();
+                    const int last = lc - (cc >> 1) * 64 - (cc & 1) * 4;      // qp_key(32 cc + e) = qp_key(e) + that
+                    const uint32_t groups = bad >> ((cc >> 1) * 4);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if (qp_key(e) > last || ((groups >> ((e >> 2) & 3)) & 1u)) x[e] = __float_as_uint(-INFINITY);
+                    tmem_st32(sb + 32 * cc, x);
+                }
+                tmem_wait_st();
+            }
             // pass 1: the largest score, group by group (one factor a group)
             float mn = -INFINITY;
             const float4* kf = reinterpret_cast<const float4*>(kf_s + j * 8);
@@ -413,10 +421,6 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
                     uint32_t sr[32];
                     tmem_ld32(sb + half * 64 + cc * 32, sr);
                     tmem_wait_ld();
-                    if (masked) {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) mask(half, cc * 32 + e, sr[e]);
-                    }
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
                         const int k = 2 * ((e >> 2) & 3) + ((e >> 1) & 1);
@@ -452,10 +456,6 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
                 uint32_t pk[32];
 #pragma unroll
                 for (int h3 = 0; h3 < 2; ++h3) {
-                    if (masked) {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) mask(k, h3 * 32 + e, sr[h3][e]);
-                    }
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
                         const int gi = (e >> 2) & 3;
