@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
     constexpr int UT = kQdUnit / (2 * D);              // tokens a unit
     constexpr int TPU = UT / 16;                       // 16-token tiles a unit
     constexpr int UPB = 32 / TPU;                      // units whose tiles a warp's lanes describe at once
-    constexpr int KS = D / 16, PS = D + 2, RB = 8 * NT;
+    constexpr int KS = D / 16, PS = D + 4, RB = 8 * NT;
     static_assert(!PAIR || NT == 1, "paired columns: one row tile");
     constexpr int QP = PAIR ? 1 : 2;                   // query operands a row tile
     static_assert(RB * PS * sizeof(float) <= kQdDepth * kQdUnit, "a warp's partial rows fit its ring");
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
 
     // ---- this warp's (max, sum, O) of every row to its drained ring
     {
-        float* mine_f = reinterpret_cast<float*>(ring);        // [RB][D + 2]
+        float* mine_f = reinterpret_cast<float*>(ring);        // [RB][max, sum, -, -, O]
         const float un = q8_pow2(eo), bias = q8_pow2(-kQdBias);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -488,8 +488,8 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
                 }
 #pragma unroll
                 for (int md = 0; md < KS; ++md) {
-                    to[2 + 16 * md + qr] = o[nt][md][c] * un * bias;
-                    to[2 + 16 * md + qr + 8] = o[nt][md][c + 2] * un * bias;
+                    to[4 + 16 * md + qr] = o[nt][md][c] * un * bias;
+                    to[4 + 16 * md + qr + 8] = o[nt][md][c + 2] * un * bias;
                 }
             }
     }
@@ -523,7 +523,7 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
         for (int g = 0; g < kQdKG; ++g) {
             const float w = gw[r * kQdKG + g];
             if (w != 0.f) {
-                const float2 y = *reinterpret_cast<const float2*>(group_row(g, r) + 2 + e);
+                const float2 y = *reinterpret_cast<const float2*>(group_row(g, r) + 4 + e);
                 x0 += y.x * w;
                 x1 += y.y * w;
             }
@@ -532,7 +532,7 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
             const float L = ls[r];
             q8_store2<D>(a, b, h, rbase + r, n_tok, e, L == 0.f ? 0.f : x0 / L, L == 0.f ? 0.f : x1 / L);
         } else {
-            *reinterpret_cast<float2*>(mypart + (size_t)r * PS + 2 + e) = make_float2(x0, x1);
+            *reinterpret_cast<float2*>(mypart + (size_t)r * PS + 4 + e) = make_float2(x0, x1);
         }
     }
     if (!alone) {
@@ -623,7 +623,7 @@ int pick_split(dkv_dims dims, int capacity, int split_keys) {
 size_t decode_work(dkv_dims dims, int R, int capacity, int split, bool mass, Q8AttnArgs* a, Arena* ar) {
     const int rb = row_block(R), n_rb = (R + rb - 1) / rb, ns = std::max(1, (capacity + split - 1) / split);
     const size_t bh = (size_t)dims.batch * dims.n_kv;
-    const size_t part = bh * n_rb * ns * rb * (dims.d + 2), s_ld = (size_t)(R + 1) / 2 * 2;
+    const size_t part = bh * n_rb * ns * rb * (dims.d + 4), s_ld = (size_t)(R + 1) / 2 * 2;
     if (a) {
         a->tickets = ar->take<unsigned>(kQ8Tickets);
         a->part = ar->take<float>(part);

@@ -18,7 +18,7 @@ struct Q8AttnArgs {
     int out_dtype;
     int split, n_splits, n_rb;   // keys per split, splits, row blocks per (sequence, head)
     float scale;                 // log2 e / sqrt(d)
-    float* part;                 // [batch][n_kv][n_rb][n_splits][rows a block][d + 2]
+    float* part;                 // [batch][n_kv][n_rb][n_splits][rows a block][d + 4]: max, sum, -, -, O
     unsigned* tickets;           // [batch][n_kv][n_rb]
     float* scores;               // [batch][n_kv][capacity][s_ld] (log2 units) or null
     float2* stats;               // [batch][n_kv][T * group] (max in log2 units, 1 / sum)
@@ -65,7 +65,7 @@ DKV_DEV void q8_store2(const Q8AttnArgs& a, int b, int h, int gr, int n_tok, int
 // loads up to kMergeQ splits.
 template <int D, int RB>
 DKV_DEV void q8_merge_splits(const Q8AttnArgs& a, size_t bhr, int b, int h, int rbase, int R, int n_tok) {
-    constexpr int PS = D + 2, kMergeQ = 16;
+    constexpr int PS = D + 4, kMergeQ = 16;
     __shared__ int is_last;
     __syncthreads();                     // the CTA's partials are stored
     if (threadIdx.x == 0) {
@@ -91,7 +91,7 @@ DKV_DEV void q8_merge_splits(const Q8AttnArgs& a, size_t bhr, int b, int h, int 
                 if (q0 + k < ns) {
                     const float* at = parts + ((size_t)(q0 + k) * RB + r) * PS;
                     ml[k] = __ldcg(reinterpret_cast<const float2*>(at));
-                    y[k] = __ldcg(reinterpret_cast<const float2*>(at + 2 + e));
+                    y[k] = __ldcg(reinterpret_cast<const float2*>(at + 4 + e));
                 }
             }
             float m = M;

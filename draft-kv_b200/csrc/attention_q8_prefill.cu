@@ -12,8 +12,7 @@
 //     query tile t, O_t += P_t(j-1) V(j-1), then S_t(j) = Q_t K_j^T;
 //   warps 0-3 / 4-7 -- softmax of query tiles A / B, one row a thread.
 // The order of a contraction is free, so both operands of each product take the
-// order in which a lane's bytes lie: dims are permuted alike in Q and K
-// (qp_dim), keys alike in S, P and V (qp_key: a tile's column c belongs to the
+// order in which a lane's bytes lie: dims are permuted alike in Q and K, keys alike in S, P and V (qp_key: a tile's column c belongs to the
 // 16-token group (c >> 6) * 4 + ((c >> 2) & 3)).
 // Block scales never touch the operands: K's multiplies the fp32 score, V's
 // (over the largest of the CTA's key range) is added to the exponent of the
@@ -46,11 +45,9 @@ constexpr float kQpLazy = 8.f;
 constexpr int kQpBias = 6;
 constexpr int kQpDown = -20;            // V block exponents below the largest that probabilities carry
 
-// Dim of element i (0..7) of a row's 16-byte unit u (of the d / 8): what lane
-// t = (u & 7) >> 1 of a fragment of block 2 (u >> 3) + (u & 1) holds.
-__host__ __device__ constexpr int qp_dim(int u, int i) {
-    return (2 * (u >> 3) + (u & 1)) * 32 + (i >> 2) * 16 + ((i >> 1) & 1) * 8 + 2 * ((u & 7) >> 1) + (i & 1);
-}
+// Element i (0..7) of a row's 16-byte unit u (of the d / 8) is dim
+// 32 (2 (u >> 3) + (u & 1)) + 16 (i >> 2) + 8 ((i >> 1) & 1) + 2 ((u & 7) >> 1) + (i & 1):
+// what lane t = (u & 7) >> 1 of a fragment of that 32-dim block holds.
 // Key (0..127) of a tile's column c: 16-byte unit 2 t + pair of a 64-key half,
 // 4 tokens of each of the pair's groups.
 __host__ __device__ constexpr int qp_key(int c) {
@@ -75,6 +72,10 @@ DKV_DEV uint32_t h2(float lo, float hi) {
     __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&v);
 }
+DKV_DEV uint32_t pack_bf2(float lo, float hi) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+}
 // Four codes times f (a power of two up to 1), rounded to codes again.
 DKV_DEV uint32_t rescaled(uint32_t w, float f) {
     uint32_t lo, hi;
@@ -86,7 +87,7 @@ DKV_DEV uint32_t rescaled(uint32_t w, float f) {
 template <int D>
 __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_constant__ Q8AttnArgs a) {
     using Geo = QpGeo<D>;
-    constexpr int PS = D + 2;
+    constexpr int PS = D + 4;
     extern __shared__ uint8_t qp_raw[];
     uint8_t* sm = qp_raw + ((1024u - (smem_u32(qp_raw) & 1023u)) & 1023u);
     __shared__ __align__(8) uint64_t k_full[kQpNst], k_empty[kQpNst], v_full[kQpNst], v_empty[kQpNst];
@@ -349,33 +350,33 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t sb = lanes + (uint32_t)(t * 256), ob = sb + 128;
         const bool mine = cr < R && gr / G < n_tok;
-        float c;                                                  // scores = S * c * (K scale), log2 units
+        float c = 1.f;                                            // scores = S * c * (K scale), log2 units
         {
-            // the row of Q as f16 of q * log2 e / sqrt(d) * 2^-x, x the row's exponent
-            const float* qrow =
-                mine ? a.q + (((size_t)b * a.T + gr / G) * v.n_kv * G + h * G + gr % G) * D : nullptr;
-            float am = 0.f;
-            if (qrow)
-#pragma unroll 8
-                for (int u = 0; u < D / 4; ++u) {
-                    const float4 x = __ldg(reinterpret_cast<const float4*>(qrow + 4 * u));
-                    am = fmaxf(fmaxf(am, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
-                }
-            const int ex = min(max((int)(__float_as_uint(am * a.scale) >> 23) - 127, -100), 126);
-            const float f = a.scale * q8_pow2(-ex);
-            c = q8_pow2(ex);
+            // the warp's 32 rows of Q as f16 of q * log2 e / sqrt(d) * 2^-x, x the
+            // row's exponent: D / 4 lanes a row, 16 bytes each
+            constexpr int LPR = D / 4, RPI = 32 / LPR;            // lanes a row, rows a step
+            const int li = lane % LPR;
             uint8_t* qt = sm + t * Geo::QT;
 #pragma unroll 4
-            for (int u = 0; u < D / 8; ++u) {
-                uint32_t o[4] = {0u, 0u, 0u, 0u};
-                if (qrow)
+            for (int i = 0; i < LPR; ++i) {
+                const int wr = i * RPI + lane / LPR, row = (warp & 3) * 32 + wr, qr = r0 + t * kQpTile + row;
+                const bool there = t * kQpTile + row < R && qr / G < n_tok;
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (there)
+                    x = __ldg(reinterpret_cast<const float4*>(
+                        a.q + (((size_t)b * a.T + qr / G) * v.n_kv * G + h * G + qr % G) * D + 4 * li));
+                float am = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float2 x = __ldg(reinterpret_cast<const float2*>(qrow + qp_dim(u, 2 * i)));
-                        o[i] = h2(x.x * f, x.y * f);
-                    }
-                *reinterpret_cast<uint4*>(qt + (u >> 3) * 16384 + rt * 128 + (((u & 7) ^ (rt & 7)) << 4)) =
-                    make_uint4(o[0], o[1], o[2], o[3]);
+                for (int o = 1; o < LPR; o <<= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
+                const int ex = min(max((int)(__float_as_uint(am * a.scale) >> 23) - 127, -100), 126);
+                const float f = a.scale * q8_pow2(-ex);
+                const int mx = __shfl_sync(0xffffffffu, ex, (lane % RPI) * LPR);
+                if (lane / RPI == i) c = q8_pow2(mx);             // (this thread's own row: lane = i * RPI + ..)
+                // dims 4 li .. + 3 are two pairs: block li / 8, half li / 4 % 2, t = 2 li % 4, + 1
+                const int blk = li >> 3, u = (blk >> 1) * 8 + (blk & 1) + 2 * ((2 * li) & 3), in = ((li >> 2) & 1) * 8 + ((li >> 1) & 1) * 4;
+                uint8_t* at = qt + (u >> 3) * 16384 + row * 128 + in;
+                *reinterpret_cast<uint32_t*>(at + (((u & 7) ^ (row & 7)) << 4)) = h2(x.x * f, x.y * f);
+                *reinterpret_cast<uint32_t*>(at + ((((u + 2) & 7) ^ (row & 7)) << 4)) = h2(x.z * f, x.w * f);
             }
             fence_async_shared();
             named_sync(1, kQpSoft + 32);
@@ -502,6 +503,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
         // O is in units of 2^(evm - bias), l in units of 2^-bias
         const float un = q8_pow2(evm);
         const float f = alone ? (live ? un / l : 0.f) : un * q8_pow2(-kQpBias);
+        const size_t out_at = (((size_t)b * a.T + gr / G) * v.n_kv * G + h * G + gr % G) * D;
         if (__all_sync(0xffffffffu, ok)) {
 #pragma unroll 1
             for (int c0 = 0; c0 < D; c0 += 32) {
@@ -510,12 +512,19 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
                 tmem_wait_ld();
                 if (!mine) continue;
 #pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    const float x0 = live ? __uint_as_float(o[e]) * f : 0.f, x1 = live ? __uint_as_float(o[e + 1]) * f : 0.f;
-                    if (alone)
-                        q8_store2<D>(a, b, h, gr, n_tok, c0 + e, x0, x1);
-                    else if (live)
-                        *reinterpret_cast<float2*>(mypart + 2 + c0 + e) = make_float2(x0, x1);
+                for (int e = 0; e < 32; ++e) o[e] = live ? __float_as_uint(__uint_as_float(o[e]) * f) : 0u;
+                if (!alone || a.out_dtype == DKV_F32) {
+                    if (!alone && !live) continue;
+                    float* to = alone ? reinterpret_cast<float*>(a.out) + out_at + c0 : mypart + 4 + c0;
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        *reinterpret_cast<uint4*>(to + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                } else {
+                    uint16_t* to = reinterpret_cast<uint16_t*>(a.out) + out_at + c0;
+                    auto bf2 = [&](int e) { return pack_bf2(__uint_as_float(o[e]), __uint_as_float(o[e + 1])); };
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8)
+                        *reinterpret_cast<uint4*>(to + e) = make_uint4(bf2(e), bf2(e + 2), bf2(e + 4), bf2(e + 6));
                 }
             }
         }
@@ -551,7 +560,7 @@ int prefill_split(dkv_dims dims, int n_rb, int capacity) {
 size_t prefill_layout(dkv_dims dims, int group, int T, int capacity, Q8AttnArgs* a, Arena* ar) {
     const int R = T * group, n_rb = (R + kQpRows - 1) / kQpRows;
     const int split = prefill_split(dims, n_rb, capacity), ns = std::max(1, (capacity + split - 1) / split);
-    const size_t part = ns == 1 ? 0 : (size_t)dims.batch * dims.n_kv * n_rb * ns * kQpRows * (dims.d + 2);
+    const size_t part = ns == 1 ? 0 : (size_t)dims.batch * dims.n_kv * n_rb * ns * kQpRows * (dims.d + 4);
     if (a) {
         a->split = split;
         a->n_splits = ns;
