@@ -259,139 +259,409 @@ DKV_DEV int evict_keep(const Q8EvictArgs& a, int b, int* n_out) {
 }
 
 constexpr int kSelThreads = 1024;
+constexpr int kSelBits = 11, kSelBins = 1 << kSelBits;
+constexpr int kSelMaxCluster = 8;
+constexpr int kSelSmemKeys = 48 * 1024;         // keys of a CTA's slice that shared memory holds
+constexpr size_t kSelSmem = 3 * kSelBins * sizeof(unsigned);      // its histograms, one a pass
 
-// Which entries stay: per (sequence, head) the `drop` lowest (mass, index)
-// of the unprotected entries go.  The drop-th smallest mass is found by a
-// radix select (four passes of 8 bits over the masses), then one ordered pass
-// counts the entries that stay and writes their indices, masses and positions.
-__global__ void __launch_bounds__(kSelThreads) q8_select_kernel(Q8EvictArgs a) {
-    __shared__ unsigned hist[256];
-    __shared__ unsigned s_prefix, s_need;
-    __shared__ int wsum_lt[32], wsum_eq[32];
-    const int h = blockIdx.x, b = blockIdx.y;
+DKV_DEV uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+    return r;
+}
+DKV_DEV void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+DKV_DEV void cluster_arrive_all() { asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory"); }
+DKV_DEV void cluster_wait_all() { asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory"); }
+// Two words of the CTA `rank`'s shared memory at this CTA's address p
+DKV_DEV uint2 dsmem_ld2(const void* p, uint32_t rank) {
+    uint2 v;
+    asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %2, %3;\n ld.shared::cluster.v2.u32 {%0, %1}, [a];\n}\n"
+        : "=r"(v.x), "=r"(v.y)
+        : "r"(smem_u32(p)), "r"(rank));
+    return v;
+}
+DKV_DEV unsigned warp_scan(unsigned v) {      // inclusive
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned y = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += y;
+    }
+    return v;
+}
+
+// Which entries stay: per (sequence, head) the `drop` lowest (mass, index) of
+// the unprotected entries go.  A cluster of CTAs takes a (sequence, head), each
+// CTA a contiguous slice of the entries whose order-preserving keys it keeps in
+// shared memory (slices that do not fit are read from global memory again).
+// Radix select of the drop-th smallest key in three passes (11, 11, 10 bits):
+// each CTA's histogram is summed over the cluster through distributed shared
+// memory (one cluster barrier a pass: every pass has a histogram of its own), so
+// every CTA finds the same bin.  Plain shared-memory atomics: grouping a warp's
+// equal bins first (match) took 200 cycles a warp, more than 32 atomics to one
+// address.  The counts below and at the key give each slice its place, and one
+// ordered pass over it (a warp a contiguous part) writes the kept indices,
+// masses and positions: order and result are fixed.
+__global__ void __launch_bounds__(kSelThreads) q8_select_kernel(Q8EvictArgs a, int cluster, int smem_keys) {
+    extern __shared__ __align__(16) unsigned sel_sm[];
+    unsigned* keys_s = sel_sm + 3 * kSelBins;      // (histograms [3][kSelBins] first)
+    __shared__ unsigned wsum[32], wbelow[32], wcnt[64], s_bin, s_below;
+    __shared__ __align__(8) uint2 counts;
+    const uint32_t rank = cluster > 1 ? cluster_rank() : 0u;
+    const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    for (int i = tid; i < 3 * kSelBins; i += kSelThreads) sel_sm[i] = 0u;
+    pdl_trigger();
+    pdl_wait();
     int n;
     const int keep = evict_keep(a, b, &n);
-    if (threadIdx.x == 0 && (a.n[b] > a.v.capacity() || a.n[b] < 0 ||
-                             keep < min(n, max(a.budget[b], a.sink + a.recent))))
+    if (rank == 0 && tid == 0 && (a.n[b] > a.v.capacity() || a.n[b] < 0 ||
+                                  keep < min(n, max(a.budget[b], a.sink + a.recent))))
         atomicOr(a.err, kErrQ8Page);
-    const size_t cap = a.v.capacity(), row = ((size_t)b * a.v.n_kv + h);
+    const size_t cap = a.v.capacity(), row = (size_t)b * a.v.n_kv + h;
     const float* mass = a.mass + row * cap;
     const int out_cap = a.out_pages << a.v.page_shift;
-    int32_t* kept = a.kept + row * out_cap;
     const int f0 = min(a.sink, n), f1 = max(n - a.recent, f0);     // unprotected entries [f0, f1)
     const int drop = min(n - keep, f1 - f0);
-    // radix select of the drop-th smallest key
-    unsigned prefix = 0, need = (unsigned)drop;
+    // this CTA's slice [i0, i1): a multiple of 32 entries a warp
+    const int slice = ((n + cluster - 1) / cluster + kSelThreads - 1) / kSelThreads * kSelThreads;
+    const int i0 = min((int)rank * slice, n), i1 = min(i0 + slice, n);
+    const bool staged = slice <= smem_keys;
+    // key of entry i, 0xffffffff for protected ones (which never go)
+    auto key_of = [&](int i, float m) { return i >= f0 && i < f1 ? mass_key(m) : 0xffffffffu; };
+    if (staged && drop > 0) {
+#pragma unroll 8
+        for (int i = i0 + tid; i < i1; i += kSelThreads) keys_s[i - i0] = key_of(i, __ldg(mass + i));
+    }
+    auto key_at = [&](int i) { return staged ? keys_s[i - i0] : key_of(i, __ldg(mass + i)); };
+    __syncthreads();
+
+    unsigned prefix = 0, need = (unsigned)drop, below = 0, equal = 0;      // below, equal: this slice's counts
     if (drop > 0) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = threadIdx.x; i < 256; i += kSelThreads) hist[i] = 0;
-            __syncthreads();
-            const unsigned hi_mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-            for (int i = f0 + threadIdx.x; i < f1; i += kSelThreads) {
-                const unsigned key = mass_key(mass[i]);
-                if ((key & hi_mask) == prefix) atomicAdd(&hist[(key >> shift) & 255u], 1u);
+        for (int pass = 0; pass < 3; ++pass) {
+            unsigned* hist = sel_sm + pass * kSelBins;
+            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : kSelBits;
+            const unsigned mask = pass == 0 ? 0u : 0xffffffffu << (shift + bits);
+            const int from = max(i0, f0), to = min(i1, f1);
+#pragma unroll 4
+            for (int i = from + tid; i < to; i += kSelThreads) {
+                const unsigned key = key_at(i);
+                if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & ((1u << bits) - 1u)], 1u);
             }
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                unsigned left = need;
-                int bin = 0;
-                while (bin < 255 && hist[bin] < left) left -= hist[bin++];
-                s_prefix = prefix | ((unsigned)bin << shift);
-                s_need = left;
+            if (cluster > 1)
+                cluster_sync_all();
+            else
+                __syncthreads();
+            // the cluster's sums, thread i's bins 2 i and 2 i + 1, and their prefix sums
+            const uint2 own = *reinterpret_cast<const uint2*>(hist + 2 * tid);
+            uint2 c = own;
+            if (cluster > 1) {
+                uint2 part[kSelMaxCluster];
+#pragma unroll
+                for (int r = 0; r < kSelMaxCluster; ++r) {
+                    part[r] = make_uint2(0u, 0u);
+                    if (r < cluster) part[r] = dsmem_ld2(hist + 2 * tid, r);
+                }
+                c = make_uint2(0u, 0u);
+#pragma unroll
+                for (int r = 0; r < kSelMaxCluster; ++r) c.x += part[r].x, c.y += part[r].y;
             }
+            const unsigned run = warp_scan(c.x + c.y);
+            if (lane == 31) wsum[warp] = run;
             __syncthreads();
-            prefix = s_prefix;
-            need = s_need;                 // how many entries equal to the key found so far go
+            const unsigned w = wsum[lane], upto = warp_scan(w);
+            const unsigned before = __shfl_sync(0xffffffffu, upto - w, warp);
+            const unsigned e0 = before + run - c.x - c.y, e1 = e0 + c.x;      // entries in bins below
+            if (e0 < need && need <= e0 + c.x) s_bin = 2 * tid, s_below = e0;
+            if (e1 < need && need <= e1 + c.y) s_bin = 2 * tid + 1, s_below = e1;
             __syncthreads();
+            // this slice's entries in bins below the one found
+            const unsigned bin = s_bin;
+            unsigned mine = (2u * tid < bin ? own.x : 0u) + (2u * tid + 1u < bin ? own.y : 0u);
+            prefix |= bin << shift;
+            need -= s_below;
+            equal = hist[bin];
+            mine = (unsigned)warp_sum_i((int)mine);
+            if (lane == 0) wbelow[warp] = mine;
+            __syncthreads();
+            below += (unsigned)warp_sum_i((int)wbelow[lane]);
         }
     }
-    // ordered pass: an unprotected entry goes if its key is below `prefix`, or
-    // equal with fewer than `need` equal ones before it
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int done_gone = 0, done_eq = 0;
-    for (int c0 = 0; c0 < n; c0 += kSelThreads) {
-        const int i = c0 + threadIdx.x;
-        const bool in = i < n, open = in && i >= f0 && i < f1 && drop > 0;
-        const float mval = in ? mass[i] : 0.f;
-        const unsigned key = open ? mass_key(mval) : 0xffffffffu;
-        const bool eq = open && key == prefix;
-        const unsigned beq = __ballot_sync(0xffffffffu, eq);
-        if (lane == 0) wsum_eq[warp] = __popc(beq);
-        __syncthreads();
-        int eq_before = done_eq + __popc(beq & ((1u << lane) - 1u)), eq_all = 0;
-        for (int w = 0; w < kSelThreads / 32; ++w) {
-            if (w < warp) eq_before += wsum_eq[w];
-            eq_all += wsum_eq[w];
+    // entries that go before this slice: all below the key, and the first `need` equal ones
+    unsigned gone_before = 0, eq_before = 0;
+    if (cluster > 1) {
+        if (tid == 0) counts = make_uint2(below, equal);
+        cluster_sync_all();
+        for (uint32_t r = 0; r < rank; ++r) {
+            const uint2 c = dsmem_ld2(&counts, r);
+            gone_before += c.x;
+            eq_before += c.y;
         }
-        const bool gone = open && (key < prefix || (eq && eq_before < (int)need));
-        const unsigned bg = __ballot_sync(0xffffffffu, gone);
-        if (lane == 0) wsum_lt[warp] = __popc(bg);
+        gone_before += min(eq_before, need);
+        cluster_arrive_all();                      // (waited for at the end: shared memory outlives its readers)
+    }
+
+    int32_t* kept = a.kept + row * out_cap;
+    if (i0 < i1) {
+        // a warp a contiguous part of the slice: its equal and gone counts, then its place, then its entries
+        const int part = slice / 32, p0 = i0 + warp * part, p1 = min(p0 + part, i1);
+        unsigned my_eq = 0, my_lt = 0;
+        if (drop > 0)
+#pragma unroll 4
+            for (int i = max(p0, f0) + lane; i < min(p1, f1); i += 32) {
+                const unsigned k = key_at(i);
+                my_eq += k == prefix;
+                my_lt += k < prefix;
+            }
+        my_eq = (unsigned)warp_sum_i((int)my_eq);
+        my_lt = (unsigned)warp_sum_i((int)my_lt);
+        if (lane == 0) wcnt[warp] = my_eq, wcnt[32 + warp] = my_lt;
         __syncthreads();
-        int gone_before = done_gone + __popc(bg & ((1u << lane) - 1u)), gone_all = 0;
-        for (int w = 0; w < kSelThreads / 32; ++w) {
-            if (w < warp) gone_before += wsum_lt[w];
-            gone_all += wsum_lt[w];
-        }
-        if (in && !gone) {
-            const int o = i - gone_before;
-            if (o < out_cap) {
-                kept[o] = i;
-                a.mass_out[row * cap + o] = mval;
-                if (a.pos_out) a.pos_out[row * cap + o] = a.pos[row * cap + i];
+        const unsigned we = wcnt[lane], wl = wcnt[32 + lane];
+        const unsigned se = warp_scan(we) - we, sl = warp_scan(wl) - wl;
+        unsigned eq = eq_before + __shfl_sync(0xffffffffu, se, warp);
+        unsigned gone = gone_before + __shfl_sync(0xffffffffu, sl, warp) + (min(eq, need) - min(eq_before, need));
+        constexpr int U = 4;                       // 32-entry groups whose loads are in flight together
+        for (int c0 = p0; c0 < p1; c0 += 32 * U) {
+            float m[U];
+            int32_t p[U], o[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int i = c0 + 32 * u + lane;
+                const bool in = i < p1;
+                m[u] = in ? __ldg(mass + i) : 0.f;
+                p[u] = in && a.pos_out ? __ldg(a.pos + row * cap + i) : 0;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int i = c0 + 32 * u + lane;
+                const bool in = i < p1, open = in && i >= f0 && i < f1 && drop > 0;
+                const unsigned k = open ? mass_key(m[u]) : 0xffffffffu;
+                const bool is_eq = open && k == prefix;
+                const unsigned beq = __ballot_sync(0xffffffffu, is_eq);
+                const bool goes = open && (k < prefix || (is_eq && eq + __popc(beq & ((1u << lane) - 1u)) < need));
+                const unsigned bg = __ballot_sync(0xffffffffu, goes);
+                o[u] = in && !goes ? i - (int)(gone + __popc(bg & ((1u << lane) - 1u))) : out_cap;
+                eq += __popc(beq);
+                gone += __popc(bg);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (o[u] >= out_cap) continue;
+                kept[o[u]] = c0 + 32 * u + lane;
+                a.mass_out[row * cap + o[u]] = m[u];
+                if (a.pos_out) a.pos_out[row * cap + o[u]] = p[u];
             }
         }
-        done_eq += eq_all;
-        done_gone += gone_all;
-        __syncthreads();
     }
-    const int left = min(n - drop, out_cap);
-    for (int i = left + threadIdx.x; i < out_cap; i += kSelThreads) kept[i] = -1;
-    for (size_t i = left + threadIdx.x; i < cap; i += kSelThreads) {
+    // behind the kept entries, the cluster's threads together
+    const int left = min(n - drop, out_cap), stride = kSelThreads * cluster;
+    for (int i = left + (int)rank * kSelThreads + tid; i < out_cap; i += stride) kept[i] = -1;
+    for (size_t i = left + (size_t)rank * kSelThreads + tid; i < cap; i += stride) {
         a.mass_out[row * cap + i] = 0.f;
         if (a.pos_out) a.pos_out[row * cap + i] = -1;
     }
+    if (cluster > 1) cluster_wait_all();
 }
 
-// The kept rows of one output page, head and side: gathered as fp32 values
-// (exact: an e4m3 code times a power of two), then written under the smallest
-// scale that holds them, as an append of those values to an empty page would.
-__global__ void __launch_bounds__(kQ8Threads) q8_gather_kernel(Q8EvictArgs a) {
-    extern __shared__ __align__(16) float stage[];
-    __shared__ float red[32];
+// The kept rows of one output page and head, K (warps 0-3) and V (warps 4-7): a
+// thread makes 16-byte fragments of the output.  A K fragment holds two rows
+// (words 0, 2 and 1, 3), a V fragment a byte of four rows in each word; the
+// sources are the fragments of those rows' tiles at the same dims, loaded whole
+// and picked apart in registers.  The page's scale is the smallest that holds
+// the values (as an append of them to an empty page gives), so the fragments
+// wait in registers for the largest magnitude, and codes whose scale changes
+// are rounded once.  What it reads: the sectors the kept rows touch (half of a
+// tile's K sectors for 4 kept rows of 16, nearly all of V's, whose rows are the
+// bytes of every word).
+struct GatherRow {
+    const uint8_t* tile;       // the row's 16-token tile of K in its page (V: + a side), null: bad page or not there
+    int k;                     // row in the tile, -1: not there
+};
+
+// Four codes times f, rounded to codes again.
+DKV_DEV uint32_t times4(uint32_t w, float f) {
+    uint32_t lo, hi;
+    q8_decode4(w, lo, hi);
+    const float2 x = __half22float2(*reinterpret_cast<__half2*>(&lo)), y = __half22float2(*reinterpret_cast<__half2*>(&hi));
+    return q8_encode2(x.x * f, x.y * f) | (q8_encode2(y.x * f, y.y * f) << 16);
+}
+// 2^(e_src - e_dst); codes that are not zero fit below 2^18, so 2^32 is enough above
+DKV_DEV float shift_factor(int e_src, int e_dst) { return q8_pow2(min(max(e_src - e_dst, -126), 32)); }
+
+// Loads go out in three rounds: kept indices, page ids, then data and scales
+// together (whose largest magnitude needs the scales only at the end).
+template <int D, int TILES>
+__global__ void __launch_bounds__(256) q8_gather_kernel(Q8EvictArgs a) {
+    constexpr int NJ = D / 32, N_BLK = TILES * NJ, FR = (N_BLK + 3) / 4;      // 512-byte blocks of a side; fragments a thread
+    __shared__ GatherRow rows[TILES * 16];
+    __shared__ int exps[2][TILES * 16], emax[2];
     const Q8View& v = a.v;
-    const int b = blockIdx.z >> 1, i = blockIdx.z & 1, h = blockIdx.y, pg = blockIdx.x;
+    const int b = blockIdx.z, h = blockIdx.y, pg = blockIdx.x, tid = threadIdx.x;
+    const int warp = tid >> 5, lane = tid & 31, side = warp >> 2, w4 = warp & 3;
+    pdl_trigger();
+    pdl_wait();
+    const int pid = __ldg(a.out_table + (size_t)b * a.out_pages + pg);
+    const int src = tid < TILES * 16 ? a.kept[(((size_t)b * v.n_kv + h) * a.out_pages + pg) * v.page + tid] : -1;
     int n;
     const int keep = evict_keep(a, b, &n);
     const int cnt = min(keep - (pg << v.page_shift), v.page);
     if (cnt <= 0) return;
-    const int pid = a.out_table[(size_t)b * a.out_pages + pg];
-    const int32_t* kept = a.kept + (((size_t)b * v.n_kv + h) * a.out_pages + pg) * v.page;
     if (!v.ok(pid)) {
-        if (threadIdx.x == 0) atomicOr(a.err, kErrQ8Page);
+        if (tid == 0) atomicOr(a.err, kErrQ8Page);
         return;
     }
-    const int d = v.d, ld = stage_ld(d);
-    const int32_t* tab = v.row(b);
-    float amax = 0.f;
-    for (int c = threadIdx.x; c < cnt * d; c += kQ8Threads) {
-        const int r = c / d, x = c % d;
-        const int src = kept[r];
-        const int sp = src >= 0 ? tab[src >> v.page_shift] : -1;
-        float val = 0.f;
-        if (v.ok(sp)) {
-            const int k = src & (v.page - 1);
-            const int byte = i ? q8_v_byte(d, k, x) : q8_k_byte(d, k, x);
-            val = q8_decode(v.side(sp, h, i)[byte]) * v.scale[v.scale_at(sp, h, i)];
-        } else {
-            atomicOr(a.err, kErrQ8Page);
+    if (tid < 2) emax[tid] = kQ8ExpMin;
+    int sp = -1;
+    if (tid < TILES * 16) {
+        GatherRow r{nullptr, tid < cnt ? 0 : -1};
+        if (tid < cnt) {
+            if (src >= 0 && src < n) sp = __ldg(v.row(b) + (src >> v.page_shift));
+            if (v.ok(sp)) {
+                r.tile = v.side(sp, h, 0) + (size_t)((src & (v.page - 1)) >> 4) * 16 * D;
+                r.k = src & 15;
+            } else {
+                sp = -1;
+                atomicOr(a.err, kErrQ8Page);              // (its values count as zeros)
+            }
         }
-        amax = fmaxf(amax, fabsf(val));
-        stage[r * ld + x] = val;
+        rows[tid] = r;
     }
-    amax = block_max(amax, red);
-    const int e = q8_exp_of(amax);
-    if (threadIdx.x == 0) v.scale[v.scale_at(pid, h, i)] = q8_pow2(e);
-    encode_side(v.side(pid, h, i), stage, d, v.page, i != 0, 0, cnt, e, e);
+    __syncthreads();
+    const int g = lane >> 2, t = lane & 3;
+    auto row_of = [&](int tile, int i) {                  // K: rows g, g + 8; V: tokens 2t, 2t + 1, 2t + 8, 2t + 9
+        return tile * 16 + (side ? 2 * t + (i & 1) + 8 * (i >> 1) : g + 8 * i);
+    };
+    float2 sc = make_float2(1.f, 1.f);
+    if (sp >= 0) sc = __ldg(reinterpret_cast<const float2*>(v.scale + v.scale_at(sp, h, 0)));
+    const size_t v_off = (size_t)v.page * D;
+    // fragment x of this warp: block x * 4 + w4 of the page side = tile block / NJ, dims block block % NJ;
+    // big: the largest magnitudes, byte i of row i
+    uint4 fr[FR];
+    uint32_t big[FR];
+#pragma unroll
+    for (int x = 0; x < FR; ++x) {
+        const int blk = x * 4 + w4, tile = blk / NJ, j = blk % NJ;
+        fr[x] = make_uint4(0u, 0u, 0u, 0u);
+        big[x] = 0u;
+        if (blk >= N_BLK || tile * 16 >= cnt) continue;
+        uint32_t w[4] = {0u, 0u, 0u, 0u};
+        if (side == 0) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const GatherRow r = rows[row_of(tile, i)];
+                if (r.tile == nullptr) continue;
+                const uint4 s = __ldg(reinterpret_cast<const uint4*>(r.tile + j * 512 + ((r.k & 7) * 4 + t) * 16));
+                w[i] = r.k & 8 ? s.y : s.x;
+                w[2 + i] = r.k & 8 ? s.w : s.z;
+                uint32_t m = __vmaxu4(w[i] & 0x7f7f7f7fu, w[2 + i] & 0x7f7f7f7fu);
+                m = __vmaxu4(m, m >> 16);
+                big[x] |= (__vmaxu4(m, m >> 8) & 0xffu) << (8 * i);
+            }
+        } else {
+            uint4 s[4];
+            int sh[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const GatherRow r = rows[row_of(tile, i)];
+                sh[i] = ((r.k >> 3 & 1) * 2 + (r.k & 1)) * 8;
+                s[i] = r.tile == nullptr ? make_uint4(0u, 0u, 0u, 0u)
+                                         : __ldg(reinterpret_cast<const uint4*>(r.tile + v_off + j * 512 + (g * 4 + ((r.k & 7) >> 1)) * 16));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[0] |= ((s[i].x >> sh[i]) & 0xffu) << (8 * i);
+                w[1] |= ((s[i].y >> sh[i]) & 0xffu) << (8 * i);
+                w[2] |= ((s[i].z >> sh[i]) & 0xffu) << (8 * i);
+                w[3] |= ((s[i].w >> sh[i]) & 0xffu) << (8 * i);
+            }
+            big[x] = __vmaxu4(__vmaxu4(w[0] & 0x7f7f7f7fu, w[1] & 0x7f7f7f7fu), __vmaxu4(w[2] & 0x7f7f7f7fu, w[3] & 0x7f7f7f7fu));
+        }
+        fr[x] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    if (tid < TILES * 16) {
+        exps[0][tid] = min(max(q8_scale_exp(sc.x), kQ8ExpMin), kQ8ExpMax);
+        exps[1][tid] = min(max(q8_scale_exp(sc.y), kQ8ExpMin), kQ8ExpMax);
+    }
+    __syncthreads();
+    int e = kQ8ExpMin;
+#pragma unroll
+    for (int x = 0; x < FR; ++x) {
+        const int tile = (x * 4 + w4) / NJ;
+        if (big[x] == 0u) continue;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (side || i < 2)
+                e = max(e, q8_exp_of(q8_decode((big[x] >> (8 * i)) & 0xffu) * q8_pow2(exps[side][row_of(tile, i)])));
+    }
+    e = warp_max_i(e);
+    if (lane == 0) atomicMax(&emax[side], e);
+    __syncthreads();
+    e = emax[side];
+    if (tid < 2) v.scale[v.scale_at(pid, h, tid)] = q8_pow2(emax[tid]);
+    uint8_t* out = v.side(pid, h, side);
+#pragma unroll
+    for (int x = 0; x < FR; ++x) {
+        const int blk = x * 4 + w4, tile = blk / NJ;
+        if (blk >= N_BLK || tile * 16 >= cnt) continue;
+        uint32_t w[4] = {fr[x].x, fr[x].y, fr[x].z, fr[x].w};
+        uint4* at = reinterpret_cast<uint4*>(out + (size_t)blk * 512 + lane * 16);
+        const bool whole = tile * 16 + 16 <= cnt;
+        const uint4 was = whole ? make_uint4(0u, 0u, 0u, 0u) : *at;
+        const uint32_t old[4] = {was.x, was.y, was.z, was.w};
+        if (side == 0) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int r = row_of(tile, i), er = exps[0][r];
+                if (r >= cnt) {
+                    w[i] = old[i], w[2 + i] = old[2 + i];
+                } else if (er != e) {
+                    const float f = shift_factor(er, e);
+                    w[i] = times4(w[i], f), w[2 + i] = times4(w[2 + i], f);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = row_of(tile, i), er = exps[1][r];
+                const uint32_t m = 0xffu << (8 * i);
+                if (r >= cnt) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) w[q] = (w[q] & ~m) | (old[q] & m);
+                } else if (er != e) {
+                    // the row's four bytes through one word
+                    uint32_t y = 0u;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) y |= ((w[q] >> (8 * i)) & 0xffu) << (8 * q);
+                    y = times4(y, shift_factor(er, e));
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) w[q] = (w[q] & ~m) | (((y >> (8 * q)) & 0xffu) << (8 * i));
+                }
+            }
+        }
+        *at = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+// CTAs a (sequence, head)'s selection is spread over: one wave of the GPU's SMs,
+// each CTA with 2048 entries at least, and its keys in shared memory.
+int select_cluster(int batch, int n_kv, int capacity) {
+    int c = 1;
+    while (c < kSelMaxCluster && ((capacity / (2 * c) >= 2048 && (long long)batch * n_kv * 2 * c <= 148) ||
+                                  capacity / c > kSelSmemKeys))
+        c *= 2;
+    return c;
+}
+
+template <int D>
+cudaError_t launch_gather(const Q8EvictArgs& a, dim3 grid, cudaStream_t st) {
+    switch (a.v.page) {
+        case 16: return launch_pdl(q8_gather_kernel<D, 1>, grid, dim3(256), 0, st, a);
+        case 32: return launch_pdl(q8_gather_kernel<D, 2>, grid, dim3(256), 0, st, a);
+        case 64: return launch_pdl(q8_gather_kernel<D, 4>, grid, dim3(256), 0, st, a);
+        default: return launch_pdl(q8_gather_kernel<D, 8>, grid, dim3(256), 0, st, a);
+    }
 }
 
 size_t stage_bytes(int page, int d) { return (size_t)page * (d + 8) * sizeof(float); }
@@ -478,10 +748,25 @@ extern "C" int dkv_q8_evict(const dkv_q8_cache* cache, dkv_dims dims, int layer,
     a.err = device_error_word();
     DKV_REQUIRE(a.err, "dkv_q8_evict: device error word unavailable");
     cudaStream_t st = (cudaStream_t)stream;
-    q8_select_kernel<<<dim3(dims.n_kv, dims.batch), kSelThreads, 0, st>>>(a);
-    DKV_LAUNCHED();
-    DKV_CUDA(allow_smem_max_once<q8_gather_kernel>());
-    q8_gather_kernel<<<dim3(out_pages, dims.n_kv, dims.batch * 2), kQ8Threads, stage_bytes(a.v.page, dims.d), st>>>(a);
-    DKV_LAUNCHED();
+    const int cap = a.v.capacity(), cl = select_cluster(dims.batch, dims.n_kv, cap);
+    const int per = ((cap + cl - 1) / cl + kSelThreads - 1) / kSelThreads * kSelThreads;
+    const int smem_keys = per <= kSelSmemKeys ? per : 0;
+    DKV_CUDA(allow_smem_max_once<q8_select_kernel>());
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)cl, (unsigned)dims.n_kv, (unsigned)dims.batch);
+    cfg.blockDim = dim3(kSelThreads);
+    cfg.dynamicSmemBytes = kSelSmem + (size_t)smem_keys * sizeof(unsigned);
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)cl;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    DKV_CUDA(cudaLaunchKernelEx(&cfg, q8_select_kernel, a, cl, smem_keys));
+    const dim3 grid((unsigned)out_pages, (unsigned)dims.n_kv, (unsigned)dims.batch);
+    DKV_CUDA(dims.d == 128 ? launch_gather<128>(a, grid, st) : launch_gather<64>(a, grid, st));
     return DKV_OK;
 }
