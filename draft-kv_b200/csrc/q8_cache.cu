@@ -465,45 +465,80 @@ __global__ void __launch_bounds__(kSelThreads) q8_select_kernel(Q8EvictArgs a, i
     if (cluster > 1) cluster_wait_all();
 }
 
-// The kept rows of one output page and head, K (warps 0-3) and V (warps 4-7): a
-// thread makes 16-byte fragments of the output.  A K fragment holds two rows
-// (words 0, 2 and 1, 3), a V fragment a byte of four rows in each word; the
-// sources are the fragments of those rows' tiles at the same dims, loaded whole
-// and picked apart in registers.  The page's scale is the smallest that holds
-// the values (as an append of them to an empty page gives), so the fragments
-// wait in registers for the largest magnitude, and codes whose scale changes
-// are rounded once.  What it reads: the sectors the kept rows touch (half of a
-// tile's K sectors for 4 kept rows of 16, nearly all of V's, whose rows are the
-// bytes of every word).
+// The kept rows of one output page and head, K or V: a thread makes 16-byte
+// fragments of the output.  A K fragment holds two rows (words 0, 2 and 1, 3), a
+// V fragment a byte of four rows in each word; the sources are the fragments of
+// those rows' tiles at the same dims, loaded whole and picked apart in
+// registers.  The page's scale is the smallest that holds the values (as an
+// append of them to an empty page gives), so the fragments wait in registers for
+// the largest magnitude, and codes whose scale changes are rounded once.  What
+// bounds it: the sectors the kept rows touch (half of a tile's K sectors for 4
+// kept rows of 16, nearly all of V's, whose rows are the bytes of every word):
+// 4 x 8 heads, 8192 of 32768 rows of d 128: 215 MB read and 45 MB written in 71 us.
 struct GatherRow {
     const uint8_t* tile;       // the row's 16-token tile of K in its page (V: + a side), null: bad page or not there
     int k;                     // row in the tile, -1: not there
 };
 
-// Four codes times f, rounded to codes again.
-DKV_DEV uint32_t times4(uint32_t w, float f) {
+DKV_DEV __half2 as_h2(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
+DKV_DEV uint32_t as_u32(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
+// Largest magnitude of four codes (as f16, exact).
+DKV_DEV __half largest4(uint32_t w) {
     uint32_t lo, hi;
     q8_decode4(w, lo, hi);
-    const float2 x = __half22float2(*reinterpret_cast<__half2*>(&lo)), y = __half22float2(*reinterpret_cast<__half2*>(&hi));
-    return q8_encode2(x.x * f, x.y * f) | (q8_encode2(y.x * f, y.y * f) << 16);
+    const __half2 m = __hmax2(__habs2(as_h2(lo)), __habs2(as_h2(hi)));
+    return __hmax(__low2half(m), __high2half(m));
 }
-// 2^(e_src - e_dst); codes that are not zero fit below 2^18, so 2^32 is enough above
-DKV_DEV float shift_factor(int e_src, int e_dst) { return q8_pow2(min(max(e_src - e_dst, -126), 32)); }
+// 2^(e_src - e_dst) as two f16 factors: codes that are not zero fit below 2^18,
+// and below 2^-28 every product rounds to zero.  What ends as a code other than
+// zero (2^-10 and more) is exact after each factor.
+struct Shift {
+    __half2 a, b;
+};
+DKV_DEV Shift shift_of(int e_src, int e_dst) {
+    const int d = min(max(e_src - e_dst, -28), 18), x = d / 2;
+    return {__float2half2_rn(q8_pow2(x)), __float2half2_rn(q8_pow2(d - x))};
+}
+DKV_DEV uint32_t times4(uint32_t w, Shift f) {
+    uint32_t lo, hi;
+    q8_decode4(w, lo, hi);
+    lo = as_u32(__hmul2(__hmul2(as_h2(lo), f.a), f.b));
+    hi = as_u32(__hmul2(__hmul2(as_h2(hi), f.a), f.b));
+    uint32_t r;
+    asm("{\n .reg .b16 a, b;\n cvt.rn.satfinite.e4m3x2.f16x2 a, %1;\n cvt.rn.satfinite.e4m3x2.f16x2 b, %2;\n mov.b32 %0, {a, b};\n}\n"
+        : "=r"(r)
+        : "r"(lo), "r"(hi));
+    return r;
+}
+// Bytes i of word q <-> bytes q of word i.
+DKV_DEV void transpose4(uint32_t (&w)[4]) {
+    const uint32_t a = __byte_perm(w[0], w[1], 0x5140), b = __byte_perm(w[2], w[3], 0x5140);      // 0: w0.0 w1.0 w0.1 w1.1
+    const uint32_t c = __byte_perm(w[0], w[1], 0x7362), d = __byte_perm(w[2], w[3], 0x7362);
+    w[0] = __byte_perm(a, b, 0x5410);
+    w[1] = __byte_perm(a, b, 0x7632);
+    w[2] = __byte_perm(c, d, 0x5410);
+    w[3] = __byte_perm(c, d, 0x7632);
+}
 
-// Loads go out in three rounds: kept indices, page ids, then data and scales
-// together (whose largest magnitude needs the scales only at the end).
-template <int D, int TILES>
-__global__ void __launch_bounds__(256) q8_gather_kernel(Q8EvictArgs a) {
-    constexpr int NJ = D / 32, N_BLK = TILES * NJ, FR = (N_BLK + 3) / 4;      // 512-byte blocks of a side; fragments a thread
+// A CTA makes one side of a page, a thread a fragment (two or more for the
+// largest pages).  Loads go out in three rounds: kept indices, page ids, then
+// data and scales together (the largest magnitude needs the scales only at the
+// end).
+constexpr int gather_threads(int d, int tiles) { return d * tiles < 512 ? d * tiles : 512; }
+
+template <int D, int TILES>              // tiles a page
+__global__ void __launch_bounds__(gather_threads(D, TILES)) q8_gather_kernel(Q8EvictArgs a) {
+    constexpr int NT = gather_threads(D, TILES), WS = NT / 32, NJ = D / 32, FR = TILES * NJ / WS;
+    static_assert(NT >= TILES * 16, "a thread for every row");
     __shared__ GatherRow rows[TILES * 16];
-    __shared__ int exps[2][TILES * 16], emax[2];
+    __shared__ int exps[TILES * 16], emax;
     const Q8View& v = a.v;
-    const int b = blockIdx.z, h = blockIdx.y, pg = blockIdx.x, tid = threadIdx.x;
-    const int warp = tid >> 5, lane = tid & 31, side = warp >> 2, w4 = warp & 3;
+    const int b = blockIdx.z >> 1, side = blockIdx.z & 1, h = blockIdx.y, pg = blockIdx.x, tid = threadIdx.x;
+    const int wi = tid >> 5, lane = tid & 31;
     pdl_trigger();
     pdl_wait();
-    const int pid = __ldg(a.out_table + (size_t)b * a.out_pages + pg);
     const int src = tid < TILES * 16 ? a.kept[(((size_t)b * v.n_kv + h) * a.out_pages + pg) * v.page + tid] : -1;
+    const int pid = __ldg(a.out_table + (size_t)b * a.out_pages + pg);
     int n;
     const int keep = evict_keep(a, b, &n);
     const int cnt = min(keep - (pg << v.page_shift), v.page);
@@ -512,14 +547,14 @@ __global__ void __launch_bounds__(256) q8_gather_kernel(Q8EvictArgs a) {
         if (tid == 0) atomicOr(a.err, kErrQ8Page);
         return;
     }
-    if (tid < 2) emax[tid] = kQ8ExpMin;
+    if (tid == 0) emax = kQ8ExpMin;
     int sp = -1;
     if (tid < TILES * 16) {
         GatherRow r{nullptr, tid < cnt ? 0 : -1};
         if (tid < cnt) {
             if (src >= 0 && src < n) sp = __ldg(v.row(b) + (src >> v.page_shift));
             if (v.ok(sp)) {
-                r.tile = v.side(sp, h, 0) + (size_t)((src & (v.page - 1)) >> 4) * 16 * D;
+                r.tile = v.side(sp, h, side) + (size_t)((src & (v.page - 1)) >> 4) * 16 * D;
                 r.k = src & 15;
             } else {
                 sp = -1;
@@ -533,114 +568,85 @@ __global__ void __launch_bounds__(256) q8_gather_kernel(Q8EvictArgs a) {
     auto row_of = [&](int tile, int i) {                  // K: rows g, g + 8; V: tokens 2t, 2t + 1, 2t + 8, 2t + 9
         return tile * 16 + (side ? 2 * t + (i & 1) + 8 * (i >> 1) : g + 8 * i);
     };
-    float2 sc = make_float2(1.f, 1.f);
-    if (sp >= 0) sc = __ldg(reinterpret_cast<const float2*>(v.scale + v.scale_at(sp, h, 0)));
-    const size_t v_off = (size_t)v.page * D;
-    // fragment x of this warp: block x * 4 + w4 of the page side = tile block / NJ, dims block block % NJ;
-    // big: the largest magnitudes, byte i of row i
-    uint4 fr[FR];
-    uint32_t big[FR];
+    float sc = 1.f;
+    if (sp >= 0) sc = __ldg(v.scale + v.scale_at(sp, h, side));
+    // fragment x of this warp: block x * WS + wi of the side = tile block / NJ, dims
+    // block block % NJ, as words of one row each (K: rows g, g + 8, g, g + 8; V: a
+    // word a row, turned at the end); big: their largest magnitudes
+    uint32_t w[FR][4];
+    __half2 big[FR][2];
 #pragma unroll
     for (int x = 0; x < FR; ++x) {
-        const int blk = x * 4 + w4, tile = blk / NJ, j = blk % NJ;
-        fr[x] = make_uint4(0u, 0u, 0u, 0u);
-        big[x] = 0u;
-        if (blk >= N_BLK || tile * 16 >= cnt) continue;
-        uint32_t w[4] = {0u, 0u, 0u, 0u};
-        if (side == 0) {
+        const int blk = x * WS + wi, tile = blk / NJ, j = blk % NJ;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const GatherRow r = rows[row_of(tile, i)];
-                if (r.tile == nullptr) continue;
-                const uint4 s = __ldg(reinterpret_cast<const uint4*>(r.tile + j * 512 + ((r.k & 7) * 4 + t) * 16));
-                w[i] = r.k & 8 ? s.y : s.x;
-                w[2 + i] = r.k & 8 ? s.w : s.z;
-                uint32_t m = __vmaxu4(w[i] & 0x7f7f7f7fu, w[2 + i] & 0x7f7f7f7fu);
-                m = __vmaxu4(m, m >> 16);
-                big[x] |= (__vmaxu4(m, m >> 8) & 0xffu) << (8 * i);
-            }
-        } else {
-            uint4 s[4];
-            int sh[4];
+        for (int q = 0; q < 4; ++q) w[x][q] = 0u;
+        if (tile * 16 < cnt) {
+            if (side == 0) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const GatherRow r = rows[row_of(tile, i)];
-                sh[i] = ((r.k >> 3 & 1) * 2 + (r.k & 1)) * 8;
-                s[i] = r.tile == nullptr ? make_uint4(0u, 0u, 0u, 0u)
-                                         : __ldg(reinterpret_cast<const uint4*>(r.tile + v_off + j * 512 + (g * 4 + ((r.k & 7) >> 1)) * 16));
-            }
+                for (int i = 0; i < 2; ++i) {
+                    const GatherRow r = rows[row_of(tile, i)];
+                    if (r.tile == nullptr) continue;
+                    const uint4 s = __ldg(reinterpret_cast<const uint4*>(r.tile + j * 512 + ((r.k & 7) * 4 + t) * 16));
+                    w[x][i] = r.k & 8 ? s.y : s.x;
+                    w[x][2 + i] = r.k & 8 ? s.w : s.z;
+                }
+            } else {
+                uint4 s[4];
+                uint32_t pick[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                w[0] |= ((s[i].x >> sh[i]) & 0xffu) << (8 * i);
-                w[1] |= ((s[i].y >> sh[i]) & 0xffu) << (8 * i);
-                w[2] |= ((s[i].z >> sh[i]) & 0xffu) << (8 * i);
-                w[3] |= ((s[i].w >> sh[i]) & 0xffu) << (8 * i);
+                for (int i = 0; i < 4; ++i) {
+                    const GatherRow r = rows[row_of(tile, i)];
+                    pick[i] = 0x40u + 0x11u * (uint32_t)((r.k >> 3 & 1) * 2 + (r.k & 1));      // that byte of both words
+                    s[i] = r.tile == nullptr ? make_uint4(0u, 0u, 0u, 0u)
+                                             : __ldg(reinterpret_cast<const uint4*>(r.tile + j * 512 +
+                                                                                    (g * 4 + ((r.k & 7) >> 1)) * 16));
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    w[x][i] = __byte_perm(__byte_perm(s[i].x, s[i].y, pick[i]), __byte_perm(s[i].z, s[i].w, pick[i]), 0x5410);
             }
-            big[x] = __vmaxu4(__vmaxu4(w[0] & 0x7f7f7f7fu, w[1] & 0x7f7f7f7fu), __vmaxu4(w[2] & 0x7f7f7f7fu, w[3] & 0x7f7f7f7fu));
         }
-        fr[x] = make_uint4(w[0], w[1], w[2], w[3]);
+        big[x][0] = __halves2half2(largest4(w[x][0]), largest4(w[x][1]));
+        big[x][1] = __halves2half2(largest4(w[x][2]), largest4(w[x][3]));
     }
-    if (tid < TILES * 16) {
-        exps[0][tid] = min(max(q8_scale_exp(sc.x), kQ8ExpMin), kQ8ExpMax);
-        exps[1][tid] = min(max(q8_scale_exp(sc.y), kQ8ExpMin), kQ8ExpMax);
-    }
+    if (tid < TILES * 16) exps[tid] = min(max(q8_scale_exp(sc), kQ8ExpMin), kQ8ExpMax);
     __syncthreads();
-    int e = kQ8ExpMin;
+    float amax = 0.f;
 #pragma unroll
     for (int x = 0; x < FR; ++x) {
-        const int tile = (x * 4 + w4) / NJ;
-        if (big[x] == 0u) continue;
+        const int tile = (x * WS + wi) / NJ;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (side || i < 2)
-                e = max(e, q8_exp_of(q8_decode((big[x] >> (8 * i)) & 0xffu) * q8_pow2(exps[side][row_of(tile, i)])));
+        for (int q = 0; q < 4; ++q) {
+            const __half m = q & 1 ? __high2half(big[x][q >> 1]) : __low2half(big[x][q >> 1]);
+            amax = fmaxf(amax, __half2float(m) * q8_pow2(exps[row_of(tile, side ? q : q & 1)]));
+        }
     }
-    e = warp_max_i(e);
-    if (lane == 0) atomicMax(&emax[side], e);
+    int e = warp_max_i(q8_exp_of(amax));
+    if (lane == 0) atomicMax(&emax, e);
     __syncthreads();
-    e = emax[side];
-    if (tid < 2) v.scale[v.scale_at(pid, h, tid)] = q8_pow2(emax[tid]);
+    e = emax;
+    if (tid == 0) v.scale[v.scale_at(pid, h, side)] = q8_pow2(e);
     uint8_t* out = v.side(pid, h, side);
 #pragma unroll
     for (int x = 0; x < FR; ++x) {
-        const int blk = x * 4 + w4, tile = blk / NJ;
-        if (blk >= N_BLK || tile * 16 >= cnt) continue;
-        uint32_t w[4] = {fr[x].x, fr[x].y, fr[x].z, fr[x].w};
+        const int blk = x * WS + wi, tile = blk / NJ;
+        if (tile * 16 >= cnt) continue;
         uint4* at = reinterpret_cast<uint4*>(out + (size_t)blk * 512 + lane * 16);
+        uint32_t old[4] = {0u, 0u, 0u, 0u};
         const bool whole = tile * 16 + 16 <= cnt;
-        const uint4 was = whole ? make_uint4(0u, 0u, 0u, 0u) : *at;
-        const uint32_t old[4] = {was.x, was.y, was.z, was.w};
-        if (side == 0) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int r = row_of(tile, i), er = exps[0][r];
-                if (r >= cnt) {
-                    w[i] = old[i], w[2 + i] = old[2 + i];
-                } else if (er != e) {
-                    const float f = shift_factor(er, e);
-                    w[i] = times4(w[i], f), w[2 + i] = times4(w[2 + i], f);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = row_of(tile, i), er = exps[1][r];
-                const uint32_t m = 0xffu << (8 * i);
-                if (r >= cnt) {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) w[q] = (w[q] & ~m) | (old[q] & m);
-                } else if (er != e) {
-                    // the row's four bytes through one word
-                    uint32_t y = 0u;
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) y |= ((w[q] >> (8 * i)) & 0xffu) << (8 * q);
-                    y = times4(y, shift_factor(er, e));
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) w[q] = (w[q] & ~m) | (((y >> (8 * q)) & 0xffu) << (8 * i));
-                }
-            }
+        if (!whole) {
+            const uint4 was = *at;
+            old[0] = was.x, old[1] = was.y, old[2] = was.z, old[3] = was.w;
+            if (side) transpose4(old);
         }
-        *at = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int r = row_of(tile, side ? q : q & 1), er = exps[r];
+            if (er != e) w[x][q] = times4(w[x][q], shift_of(er, e));
+            if (!whole && r >= cnt) w[x][q] = old[q];
+        }
+        if (side) transpose4(w[x]);
+        *at = make_uint4(w[x][0], w[x][1], w[x][2], w[x][3]);
     }
 }
 
@@ -654,13 +660,18 @@ int select_cluster(int batch, int n_kv, int capacity) {
     return c;
 }
 
+template <int D, int TILES>
+cudaError_t launch_gather(const Q8EvictArgs& a, int batch, cudaStream_t st) {
+    const dim3 grid((unsigned)a.out_pages, (unsigned)a.v.n_kv, (unsigned)batch * 2);
+    return launch_pdl(q8_gather_kernel<D, TILES>, grid, dim3((unsigned)gather_threads(D, TILES)), 0, st, a);
+}
 template <int D>
-cudaError_t launch_gather(const Q8EvictArgs& a, dim3 grid, cudaStream_t st) {
+cudaError_t launch_gather_page(const Q8EvictArgs& a, int batch, cudaStream_t st) {
     switch (a.v.page) {
-        case 16: return launch_pdl(q8_gather_kernel<D, 1>, grid, dim3(256), 0, st, a);
-        case 32: return launch_pdl(q8_gather_kernel<D, 2>, grid, dim3(256), 0, st, a);
-        case 64: return launch_pdl(q8_gather_kernel<D, 4>, grid, dim3(256), 0, st, a);
-        default: return launch_pdl(q8_gather_kernel<D, 8>, grid, dim3(256), 0, st, a);
+        case 16: return launch_gather<D, 1>(a, batch, st);
+        case 32: return launch_gather<D, 2>(a, batch, st);
+        case 64: return launch_gather<D, 4>(a, batch, st);
+        default: return launch_gather<D, 8>(a, batch, st);
     }
 }
 
@@ -766,7 +777,6 @@ extern "C" int dkv_q8_evict(const dkv_q8_cache* cache, dkv_dims dims, int layer,
     cfg.attrs = at;
     cfg.numAttrs = 2;
     DKV_CUDA(cudaLaunchKernelEx(&cfg, q8_select_kernel, a, cl, smem_keys));
-    const dim3 grid((unsigned)out_pages, (unsigned)dims.n_kv, (unsigned)dims.batch);
-    DKV_CUDA(dims.d == 128 ? launch_gather<128>(a, grid, st) : launch_gather<64>(a, grid, st));
+    DKV_CUDA(dims.d == 128 ? launch_gather_page<128>(a, dims.batch, st) : launch_gather_page<64>(a, dims.batch, st));
     return DKV_OK;
 }
