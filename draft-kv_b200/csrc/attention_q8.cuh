@@ -121,5 +121,7 @@ DKV_DEV void q8_merge_splits(const Q8AttnArgs& a, size_t bhr, int b, int h, int 
 
 int attn_q8_prefill(Q8AttnArgs& a, dkv_dims dims, void* work, size_t work_bytes, cudaStream_t st);
 size_t attn_q8_prefill_work(dkv_dims dims, int group, int T, int capacity);
+// Scratch for every T up to max_T (a shorter prompt chunk may take more splits).
+size_t attn_q8_work_upto(dkv_dims dims, int group, int max_T, int capacity, bool mass);
 
 }  // namespace dkv

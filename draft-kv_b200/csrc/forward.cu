@@ -6,6 +6,7 @@
 // captured into one CUDA graph per (shape, config).
 #include <algorithm>
 
+#include "attention_q8.cuh"
 #include "attn_common.cuh"
 
 namespace dkv {
@@ -26,8 +27,10 @@ using namespace dkv;
 
 static int round128(int x) { return (x + 127) / 128 * 128; }
 
-size_t dkv::forward_work(const dkv_model* m, int batch, int T, int max_ctx, int comp_cap, size_t* attn_bytes,
-                         size_t* gemm_bytes) {
+// q8_mass < 0: a full or drafter cache; else the 8-bit cache of max_ctx entries
+// a sequence (1: with the attention mass).
+static size_t work_layout(const dkv_model* m, int batch, int T, int max_ctx, int comp_cap, int q8_mass,
+                          size_t* attn_bytes, size_t* gemm_bytes) {
     const int N = batch * T;
     const int elem = m->dtype == DKV_F32 ? 4 : 2;
     const int HD = m->n_heads * m->d_head, KD = m->n_kv * m->d_head;
@@ -45,8 +48,9 @@ size_t dkv::forward_work(const dkv_model* m, int batch, int T, int max_ctx, int 
     // kPromptMinSplit keys, far fewer partials
     const int G = m->n_heads / m->n_kv;
     const int sk = m->split_keys > 0 ? m->split_keys : 512;
-    size_t a = dkv_attn_work_bytes(dims, G, std::min(T, std::max(1, 64 / G)), max_ctx, sk, comp_cap);
-    if (T * G > 64) {
+    size_t a = q8_mass >= 0 ? attn_q8_work_upto(dims, G, T, max_ctx, q8_mass != 0)
+                            : dkv_attn_work_bytes(dims, G, std::min(T, std::max(1, 64 / G)), max_ctx, sk, comp_cap);
+    if (q8_mass < 0 && T * G > 64) {
         const int sk_rows = m->dtype == DKV_BF16 ? std::max(kPromptMinSplit, (sk + 127) / 128 * 128) : sk;
         a = std::max(a, dkv_attn_work_bytes(dims, G, T, max_ctx, sk_rows, comp_cap));
     }
@@ -65,20 +69,29 @@ size_t dkv::forward_work(const dkv_model* m, int batch, int T, int max_ctx, int 
     return b + align_up(g, 256) + align_up(a, 256) + 4096;
 }
 
+size_t dkv::forward_work(const dkv_model* m, int batch, int T, int max_ctx, int comp_cap, size_t* attn_bytes,
+                         size_t* gemm_bytes) {
+    return work_layout(m, batch, T, max_ctx, comp_cap, -1, attn_bytes, gemm_bytes);
+}
+
 extern "C" size_t dkv_forward_work_bytes(const dkv_model* m, int batch, int T, int max_ctx, int comp_cap) {
     if (!m) return 0;
     return forward_work(m, batch, T, max_ctx, comp_cap, nullptr, nullptr);
 }
 
-extern "C" int dkv_forward(const dkv_model* m, const dkv_full_cache* full, const dkv_comp_cache* comp,
-                           const dkv_step* st, void* stream) {
-    DKV_REQUIRE(m && st && m->layers && st->tokens && st->pos0, "dkv_forward: bad arguments");
-    DKV_REQUIRE(comp || (full && full->k_pool && full->page_table),
-                "dkv_forward: a full-cache forward needs the full cache");
-    DKV_REQUIRE(m->n_heads % m->n_kv == 0, "dkv_forward: n_heads %% n_kv != 0");
-    DKV_REQUIRE(!comp || st->T == 1, "dkv_forward: draft steps have T == 1");
-    DKV_REQUIRE(st->max_T >= st->T && st->T >= 0, "dkv_forward: T %d > max_T %d", st->T, st->max_T);
-    DKV_REQUIRE(!full || m->dtype == full->dtype, "dkv_forward: model and cache dtypes differ");
+namespace {
+// The 8-bit cache of a forward: its entries per token 0, and per layer (host
+// arrays, either may be null) the mass and positions kept beside it.
+struct Q8Target {
+    const dkv_q8_cache* cache;
+    const int32_t* entry0;
+    float* const* mass;
+    int32_t* const* pos;
+};
+}  // namespace
+
+static int forward_layers(const dkv_model* m, const dkv_full_cache* full, const dkv_comp_cache* comp, const Q8Target* q8,
+                          const dkv_step* st, void* stream) {
     const int N = st->batch * st->T;
     if (N == 0) return DKV_OK;
     const int dm = m->d_model, D = m->d_head, H = m->n_heads, KV = m->n_kv;
@@ -88,8 +101,8 @@ extern "C" int dkv_forward(const dkv_model* m, const dkv_full_cache* full, const
     size_t attn_bytes = 0, gemm_bytes = 0;
     // the arena layout depends on (batch, max_T, max_ctx, cap) only, so the
     // ticket regions stay at fixed offsets across calls with different T
-    const size_t need = forward_work(m, st->batch, st->max_T, st->max_ctx, comp ? comp->cap : 0, &attn_bytes,
-                                     &gemm_bytes);
+    const size_t need = work_layout(m, st->batch, st->max_T, q8 ? q8->cache->max_pages * q8->cache->page_size : st->max_ctx,
+                                    comp ? comp->cap : 0, q8 ? q8->mass != nullptr : -1, &attn_bytes, &gemm_bytes);
     DKV_REQUIRE(st->work && st->work_bytes >= need, "dkv_forward: work buffer %zu < %zu bytes", st->work_bytes, need);
     const size_t NM = (size_t)st->batch * st->max_T;
     Arena ar(st->work, st->work_bytes);
@@ -143,7 +156,7 @@ extern "C" int dkv_forward(const dkv_model* m, const dkv_full_cache* full, const
         e.rope_cos = llama ? m->rope_cos : nullptr;
         e.rope_sin = llama ? m->rope_sin : nullptr;
         e.q_out = q;
-        e.kv_stage = comp ? stage : nullptr;
+        e.kv_stage = comp || q8 ? stage : nullptr;
         e.full = full;
         e.layer = L;
         e.n_layers = m->n_layers;
@@ -208,6 +221,15 @@ extern "C" int dkv_forward(const dkv_model* m, const dkv_full_cache* full, const
             DKV_TRY(dkv_comp_append(comp, full, dims, L, 1, stage, m->dtype, 1, st->pos0, nullptr, nullptr, L == 0 ? 1 : 0,
                                     stream));
             DKV_TRY(dkv_attn_comp(comp, dims, L, group, q, st->pos0, x, m->dtype, awork, attn_bytes, stream));
+        } else if (q8) {
+            // rows of the stage: [token][kv head][K, V][d]
+            const int32_t* e0 = q8->entry0 ? q8->entry0 : st->pos0;
+            const int64_t row = 2ll * KD;
+            float* mass = q8->mass ? q8->mass[L] : nullptr;
+            DKV_TRY(dkv_q8_append(q8->cache, dims, L, stage, stage + (size_t)D * elem, m->dtype, st->T, row * st->T, row, 2 * D,
+                                  e0, nullptr, st->pos0, mass, q8->pos ? q8->pos[L] : nullptr, stream));
+            DKV_TRY(dkv_q8_attn(q8->cache, dims, L, group, st->T, q, e0, nullptr, x, m->dtype, 0, mass, awork, attn_bytes,
+                                stream));
         } else {
             DKV_TRY(dkv_attn_full(full, dims, L, group, st->T, q, st->pos0, x, m->dtype, m->split_keys, awork,
                                   attn_bytes, stream));
@@ -225,4 +247,35 @@ extern "C" int dkv_forward(const dkv_model* m, const dkv_full_cache* full, const
     const dkv_epilogue eh = head_epi();
     DKV_TRY(dkv_gemm(xin, m->dtype, m->w_head, m->dtype, m->vocab_pad, N, dm, &eh, gwork, gemm_bytes, stream));
     return DKV_OK;
+}
+
+extern "C" int dkv_forward(const dkv_model* m, const dkv_full_cache* full, const dkv_comp_cache* comp,
+                           const dkv_step* st, void* stream) {
+    DKV_REQUIRE(m && st && m->layers && st->tokens && st->pos0, "dkv_forward: bad arguments");
+    DKV_REQUIRE(comp || (full && full->k_pool && full->page_table),
+                "dkv_forward: a full-cache forward needs the full cache");
+    DKV_REQUIRE(m->n_heads % m->n_kv == 0, "dkv_forward: n_heads %% n_kv != 0");
+    DKV_REQUIRE(!comp || st->T == 1, "dkv_forward: draft steps have T == 1");
+    DKV_REQUIRE(st->max_T >= st->T && st->T >= 0, "dkv_forward: T %d > max_T %d", st->T, st->max_T);
+    DKV_REQUIRE(!full || m->dtype == full->dtype, "dkv_forward: model and cache dtypes differ");
+    return forward_layers(m, full, comp, nullptr, st, stream);
+}
+
+extern "C" size_t dkv_forward_q8_work_bytes(const dkv_model* m, int batch, int max_T, int capacity, int note_mass) {
+    if (!m || batch < 1 || max_T < 1 || capacity < 1) return 0;
+    return work_layout(m, batch, max_T, capacity, 0, note_mass ? 1 : 0, nullptr, nullptr);
+}
+
+extern "C" int dkv_forward_q8(const dkv_model* m, const dkv_q8_cache* cache, const dkv_step* st, const int32_t* entry0,
+                              float* const* mass, int32_t* const* pos, void* stream) {
+    DKV_REQUIRE(m && st && m->layers && st->tokens && st->pos0, "dkv_forward_q8: bad arguments");
+    DKV_REQUIRE(m->n_heads % m->n_kv == 0, "dkv_forward_q8: n_heads %% n_kv != 0");
+    DKV_REQUIRE(st->batch >= 1 && st->max_T >= st->T && st->T >= 0, "dkv_forward_q8: batch %d, T %d > max_T %d", st->batch,
+                st->T, st->max_T);
+    Q8View v;
+    DKV_TRY(q8_view("dkv_forward_q8", cache, dkv_dims{m->n_layers, m->n_kv, m->d_head, st->batch}, 0, &v));
+    DKV_UNSUPPORTED(!mass || st->T * (m->n_heads / m->n_kv) <= kQ8MaxRows,
+                    "dkv_forward_q8: the mass of %d query rows a head (at most %d)", st->T * (m->n_heads / m->n_kv), kQ8MaxRows);
+    const Q8Target q8{cache, entry0, mass, pos};
+    return forward_layers(m, nullptr, nullptr, &q8, st, stream);
 }

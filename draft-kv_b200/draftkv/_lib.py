@@ -119,6 +119,8 @@ _SIGS = {
                              vp, vp, vp, vp, vp, vp, vp, C.c_size_t, vp]),
     "dkv_sample_work_bytes": (C.c_size_t, [C.c_int, C.c_int]),
     "dkv_forward_work_bytes": (C.c_size_t, [C.POINTER(ModelS), C.c_int, C.c_int, C.c_int, C.c_int]),
+    "dkv_forward_q8_work_bytes": (C.c_size_t, [C.POINTER(ModelS), C.c_int, C.c_int, C.c_int, C.c_int]),
+    "dkv_forward_q8": (C.c_int, [C.POINTER(ModelS), C.POINTER(Q8CacheS), C.POINTER(StepS), vp, vp, vp, vp]),
     "dkv_forward": (C.c_int, [C.POINTER(ModelS), C.POINTER(FullCacheS), C.POINTER(CompCacheS),
                               C.POINTER(StepS), vp]),
 }

@@ -34,6 +34,7 @@ from .compress import CompressedKVCache
 from .config import CompressionConfig, layer_cfgs
 from .controller import Controller, FixedPolicy
 from .paged import PagedKVCache
+from .q8 import MASS_ROWS, Q8KVCache
 
 try:
     import torch
@@ -123,7 +124,7 @@ class _Batch:
     def workspace(self):
         cap = self.comp.cap if self.comp is not None else 0
         if self.work is None or self._cap != cap:
-            self.work = self.m.work(self.B, self.G + 1, self.full.capacity_tokens, cap)
+            self.work = self.m.work(self.B, self.G + 1, self.full.capacity_tokens, cap, self.full)
             self._cap = cap
         return self.work
 
@@ -182,12 +183,14 @@ class DraftKVEngine:
         lens = [len(p) - 1 for p in prompts]
         L = max(lens) if lens else 0
         CH = max(self.prefill_chunk, self.prefill_tokens // max(B, 1)) if L >= 1024 else 64
+        if isinstance(st.full, Q8KVCache) and st.full.track_mass:
+            CH = max(1, min(CH, MASS_ROWS // m.n_rep))      # every prompt token adds to the mass
         tok = torch.zeros((B, max(L, 1)), dtype=torch.int32)
         for b, p in enumerate(prompts):
             if lens[b] > 0:
                 tok[b, :lens[b]] = torch.tensor(p[:-1], dtype=torch.int32)
         tok = tok.to(m.device)
-        work = m.work(B, CH, st.full.capacity_tokens, 0)
+        work = m.work(B, CH, st.full.capacity_tokens, 0, st.full)
         for b in range(B):
             st.full.ensure(b, lens[b] + st.G + 2)
         for c0 in range(0, L, CH):
@@ -286,6 +289,9 @@ class DraftKVEngine:
     # -------------------------------------------------------- device round
     def _new_comp(self, st: _Batch, cfg) -> CompressedKVCache:
         m = self.model
+        if isinstance(st.full, Q8KVCache):
+            raise NotImplementedError("the drafter cache is built from a bf16 / fp32 full cache; an 8-bit cache decodes "
+                                      "without drafts (generate_baseline)")
         arms = getattr(self.controller, "arms", None) or [cfg]
         cfgs = [c for a in arms for c in layer_cfgs(a, m.n_layers)] + layer_cfgs(cfg, m.n_layers)
         max_bits = max(c.bits for c in cfgs)

@@ -21,6 +21,7 @@ import numpy as np
 
 from . import _lib
 from .paged import PagedKVCache, dtype_code, torch_dtype
+from .q8 import MASS_ROWS, Q8KVCache
 
 try:
     import torch
@@ -141,18 +142,25 @@ class DeviceDecoder:
         if self.arch == _lib.ARCH_GPT2 and n > self.max_pos:
             raise ValueError(f"position {n - 1} beyond the learned position table ({self.max_pos})")
 
-    def work(self, batch: int, max_T: int, max_ctx: int, comp_cap: int) -> "torch.Tensor":
-        key = (batch, max_T, max_ctx, comp_cap)
+    def work(self, batch: int, max_T: int, max_ctx: int, comp_cap: int, cache=None) -> "torch.Tensor":
+        """The forward's scratch; `cache` tells whether it runs over an 8-bit
+        cache (Q8KVCache), whose attention takes scratch of its own size."""
+        q8 = None if not isinstance(cache, Q8KVCache) else bool(cache.track_mass and cache.mass is not None)
+        key = (batch, max_T, max_ctx, comp_cap, q8)
         w = self._work_cache.get(key)
         if w is None:
-            n = _lib.load().dkv_forward_work_bytes(C.byref(self._s), batch, max_T, max_ctx, comp_cap)
+            if q8 is None:
+                n = _lib.load().dkv_forward_work_bytes(C.byref(self._s), batch, max_T, max_ctx, comp_cap)
+            else:
+                n = _lib.load().dkv_forward_q8_work_bytes(C.byref(self._s), batch, max_T, max_ctx, 1 if q8 else 0)
             w = torch.zeros(int(n), dtype=torch.uint8, device=self.device)
             self._work_cache[key] = w
         return w
 
     # ------------------------------------------------------------ forward
     def forward_raw(self, full, comp, tokens_ptr: int, tok_stride: int, pos0: "torch.Tensor", batch: int, T: int,
-                    logits: "torch.Tensor", work: "torch.Tensor", max_T: int, max_ctx: int, graph: bool = True) -> None:
+                    logits: "torch.Tensor", work: "torch.Tensor", max_T: int, max_ctx: int, graph: bool = True,
+                    entry0: "torch.Tensor | None" = None) -> None:
         """One native forward for `batch` sequences x T tokens (device pointers);
         `logits` None runs no final norm and head (a prefill chunk).
 
@@ -162,13 +170,26 @@ class DeviceDecoder:
         calls replay it.  The token, position and cache contents are read at
         replay time; only the launch parameters are frozen.  `graph` False
         launches eagerly (prompt chunks: a capture syncs the device and costs
-        more than the few launches a replay would save)."""
+        more than the few launches a replay would save).
+
+        `full` may be a Q8KVCache; entry0 [batch] then gives the entries token 0
+        of each sequence gets (pos0 while nothing was evicted).  A cache that
+        tracks the mass takes at most 64 query rows a KV head."""
         step = _lib.StepS(batch, T, tokens_ptr, tok_stride, pos0.data_ptr(), None if logits is None else logits.data_ptr(),
                           work.data_ptr(), work.numel(), max_ctx, max_T)
         fs = None if full is None else full.struct()        # (syncs a changed page table first)
         cs = None if comp is None else comp.struct()
+        q8 = isinstance(full, Q8KVCache)
+        if q8 and comp is not None:
+            raise TypeError("draft steps run over a CompressedKVCache alone")
+        kept = full.layer_arrays() if q8 else ((), ())
 
         def run():
+            if q8:
+                mass, pos = ((C.c_void_p * len(a))(*a) if a else None for a in kept)
+                _lib.call("dkv_forward_q8", C.byref(self._s), C.byref(fs), C.byref(step), _lib.ptr(entry0), mass, pos,
+                          _lib.stream_ptr())
+                return
             _lib.call("dkv_forward", C.byref(self._s), None if fs is None else C.byref(fs),
                       None if cs is None else C.byref(cs), C.byref(step), _lib.stream_ptr())
 
@@ -178,7 +199,7 @@ class DeviceDecoder:
         key = (tuple(getattr(step, f) for f, _ in step._fields_),
                None if fs is None else tuple(getattr(fs, f) for f, _ in fs._fields_),
                None if cs is None else (tuple(getattr(cs, f) for f, _ in cs._fields_[:12]), tuple(comp.cfgs)),
-               _lib.stream_ptr())
+               _lib.stream_ptr()) + ((kept, _lib.ptr(entry0)) if q8 else ())
         g = self._graphs.get(key)
         if g is not None:
             g.replay()
@@ -210,8 +231,8 @@ class DeviceDecoder:
 
     def forward(self, tokens, cache, start_pos: int):
         """Run `tokens` at positions [start_pos, start_pos + T) against `cache`
-        (a device FullKVCache / PagedKVCache, or a CompressedKVCache for a
-        draft step) and return fp32 logits (T, V) on the device."""
+        (a device FullKVCache / PagedKVCache / Q8KVCache, or a CompressedKVCache
+        for a draft step) and return fp32 logits (T, V) on the device."""
         from .compress import CompressedKVCache, FullKVCache
         toks = np.asarray(tokens, dtype=np.int64).reshape(-1)
         T = int(toks.shape[0])
@@ -230,6 +251,8 @@ class DeviceDecoder:
         if isinstance(cache, FullKVCache):
             cache.materialize(self.n_kv_heads, self.d_head, self.dtype)
             cache.grow(start_pos + T)
+        if isinstance(cache, Q8KVCache):
+            return self._forward_q8(toks, cache, start_pos, logits)
         if not isinstance(cache, PagedKVCache):
             raise TypeError("device models need a device cache (FullKVCache / PagedKVCache / CompressedKVCache)")
         if cache.dtype != self.dtype:
@@ -246,6 +269,38 @@ class DeviceDecoder:
             self.forward_raw(cache, None, tok.data_ptr() + 4 * c0, c1 - c0, pos0, 1, c1 - c0, logits[c0:c1], w, CH,
                              cache.capacity_tokens)
             cache.set_length(0, start_pos + c1)
+        return logits
+
+
+    def _forward_q8(self, toks, cache, start_pos: int, logits):
+        """`forward` over sequence 0 of an 8-bit cache.  start_pos is the
+        position (RoPE, learned embeddings) of the first token, which after an
+        eviction runs ahead of the entry it gets; a cache that tracks the mass
+        is fed in chunks of at most 64 query rows a KV head, so that every token
+        adds to it."""
+        if cache.n_layers != self.n_layers or cache.n_heads != self.n_kv_heads or cache.d_head != self.d_head:
+            raise TypeError("the cache's layers, KV heads or head size are not the model's")
+        if cache.pool is None:
+            raise TypeError("a cache over external storage has no block allocator: use forward_raw")
+        n = cache.length
+        if any(c != n for c in cache.counts[0]):
+            raise ValueError("the layers hold different numbers of entries (evict all of them alike)")
+        if cache.next_pos[0] != start_pos:
+            raise ValueError(f"the cache continues at position {cache.next_pos[0]}, start_pos {start_pos}")
+        T = int(toks.shape[0])
+        if T == 0:
+            return logits
+        cache.ensure(0, n + T)
+        tok = torch.tensor(toks, dtype=torch.int32, device=self.device)
+        CH = self.api_chunk if not cache.track_mass else max(1, min(self.api_chunk, MASS_ROWS // self.n_rep))
+        w = self.work(cache.batch, CH, cache.capacity_tokens, 0, cache)
+        for c0 in range(0, T, CH):
+            c1 = min(T, c0 + CH)
+            pos0 = torch.tensor([start_pos + c0], dtype=torch.int32, device=self.device)
+            e0 = torch.tensor([n + c0], dtype=torch.int32, device=self.device)
+            self.forward_raw(cache, None, tok.data_ptr() + 4 * c0, c1 - c0, pos0, 1, c1 - c0, logits[c0:c1], w, CH,
+                             cache.capacity_tokens, entry0=e0, graph=False)
+            cache.set_length(0, n + c1)
         return logits
 
 

@@ -122,6 +122,12 @@ class Q8KVCache(PagedKVCache):
         self.sync_table()
         return self._struct
 
+    def layer_arrays(self):
+        """Device addresses of the layers' mass and positions (empty: not kept)."""
+        if not self.track_mass or self.mass is None:
+            return (), ()
+        return tuple(t.data_ptr() for t in self.mass[:-1]), tuple(t.data_ptr() for t in self.pos_t[:-1])
+
     @property
     def host_resident(self) -> bool:
         return False
@@ -287,8 +293,9 @@ class Q8KVCache(PagedKVCache):
         n, start = k.shape[0], self.counts[0][layer]
         if n == 0:
             return
-        if not np.array_equal(pos, np.arange(pos[0], pos[0] + n)) or pos[0] < start:
-            raise ValueError("appended positions must be consecutive and not below the entry they get")
+        if not np.array_equal(pos, np.arange(pos[0], pos[0] + n)) or pos[0] < start \
+                or (pos[0] != start and not self.track_mass):
+            raise ValueError("appended positions must be consecutive and continue the cache's")
         self._ensure_layer(0, layer, start + n)
         kv = torch.from_numpy(np.ascontiguousarray(np.stack([k, v])[:, None])).to(self.device)
         rows = torch.zeros((self.batch,), dtype=torch.int32)
@@ -338,7 +345,8 @@ class Q8KVCache(PagedKVCache):
         emptied block stays until the block is written from its start again."""
         before = self.counts[b][0]
         super().truncate_seq(b, n_pos)
-        self.next_pos[b] -= before - self.counts[b][0]
+        left = self.counts[b][0]
+        self.next_pos[b] = self.next_pos[b] - (before - left) if left else 0
 
     def set_length(self, b: int, n: int) -> None:
         self.next_pos[b] += n - self.counts[b][0]

@@ -482,6 +482,17 @@ DKV_API size_t dkv_forward_work_bytes(const dkv_model* m, int batch, int max_T, 
 DKV_API int dkv_forward(const dkv_model* m, const dkv_full_cache* full, const dkv_comp_cache* comp,
                 const dkv_step* st, void* stream);
 
+/* The same forward over the 8-bit cache (no counterpart in the reference): each
+ * layer's K/V rows are quantized into entries entry0[b] .. (pos0[b] .. when
+ * entry0 is NULL) and attended by dkv_q8_attn; st->pos0 gives the positions
+ * (RoPE, learned embeddings), st->max_ctx is not read.  mass, pos: host arrays of
+ * n_layers device pointers ([batch][n_kv][capacity] each; NULL: not kept), as
+ * dkv_q8_append and dkv_q8_attn take them; with mass T * group <= 64.
+ * Logits NULL as in dkv_forward.  Heads of 64 or 128; f32 and bf16 models. */
+DKV_API size_t dkv_forward_q8_work_bytes(const dkv_model* m, int batch, int max_T, int capacity, int note_mass);
+DKV_API int dkv_forward_q8(const dkv_model* m, const dkv_q8_cache* cache, const dkv_step* st, const int32_t* d_entry0,
+                           float* const* mass, int32_t* const* pos, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
