@@ -40,7 +40,7 @@ constexpr int kQdUnit = 4096;          // bytes of a unit
 constexpr int kQdDepth = 3;            // units of a warp's ring
 constexpr int kQdThreads = 32 * kQdKG;
 constexpr size_t kQdSmem = (size_t)kQdKG * kQdDepth * kQdUnit;
-constexpr int kQdMinBytes = 1 << 18;   // codes a split streams where the library picks it, at least
+constexpr int kQdMinBytes = 1 << 17;   // codes a split streams where the library picks it, at least
 constexpr float kQdLazy = 8.f;         // growth of the max that forces a rescale (log2 units)
 constexpr int kQdBias = 6;             // probabilities enter as p * 2^6: f16 keeps 2^-30 of the max
 
@@ -116,17 +116,17 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
     };
     const int first_pid = load_pid(0);
     const int qr = lane >> 2, qc = lane & 3;
-    float2 xq[NT > 1 ? 1 : KS][2];
+    float2 xq[NT][KS][2];
     auto load_q = [&](int nt, int kk, int u) {
         const int r = nt * 8 + (PAIR ? qr & 3 : qr), gr = rbase + r;      // this lane's operand row
         return r < R ? __ldg(reinterpret_cast<const float2*>(
                            a.q + (((size_t)b * a.T + gr / G) * v.n_kv * G + h * G + gr % G) * D + kk * 16 + u * 8 + 2 * qc))
                      : make_float2(0.f, 0.f);
     };
-    if (NT == 1) {
 #pragma unroll
-        for (int kk = 0; kk < KS; ++kk) xq[NT > 1 ? 0 : kk][0] = load_q(0, kk, 0), xq[NT > 1 ? 0 : kk][1] = load_q(0, kk, 1);
-    }
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk) xq[nt][kk][0] = load_q(nt, kk, 0), xq[nt][kk][1] = load_q(nt, kk, 1);
     const int n_tok = a.n_rows ? min(a.n_rows[b], a.T) : a.T;
     const int e0 = a.entry0[b];
     // the block's last token decides what is read
@@ -195,13 +195,12 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
     int lim[NT][2];                                    // last visible entry of them
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        float2 x[KS][2];
+        float2(&x)[KS][2] = xq[nt];
         float am = 0.f;
 #pragma unroll
         for (int kk = 0; kk < KS; ++kk)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                x[kk][u] = NT == 1 ? xq[NT > 1 ? 0 : kk][u] : load_q(nt, kk, u);
                 x[kk][u].x *= a.scale;
                 x[kk][u].y *= a.scale;
                 am = fmaxf(am, fmaxf(fabsf(x[kk][u].x), fabsf(x[kk][u].y)));
@@ -264,46 +263,20 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
     // entries up to here are seen by every row of the block that is there
     const int all_see = min(e0 + rbase / G, kend - 1);
 
-    int slot = 0;
-    uint32_t phase = 0;
-    for (int u = 0; u < mine; ++u) {
-        const int ub = u % UPB;
-        if (ub == 0) {
-            if (u > 0) cur = nxt;
-            nxt.pid = check_pid(u + UPB, load_pid(u + UPB));
-        } else if (ub == UPB / 2) {
-            load_scale(nxt.pid, nxt.ks, nxt.vs);
-        }
-        const uint8_t* st = ring + slot * kQdUnit + lane * 16;
-        if (!__all_sync(0xffffffffu, mbar_wait(&full[slot], phase, a.err))) {
-            // a copy never came (error word 0x80): wait, bounded, for those still in flight
-            if (lane == 0) {
-                failed = 1;
-                for (int w = u + 1; w < min(mine, u + kQdDepth); ++w)
-                    mbar_wait(&full[w % kQdDepth], (uint32_t)((w / kQdDepth) & 1), nullptr);
-            }
-            __syncwarp();
-            break;
-        }
-        const int key0 = key_of(u);
-        float ks[TPU], vs[TPU];
-        bool whole = key0 + UT - 1 <= all_see;         // every key of the unit is there for every row
+    // ---- S^T of a unit, not yet scaled: keys qr (+8), columns 2qc, 2qc + 1 of
+    // each row tile.  Two chains of products (the halves of each 32-dim block)
+    // and the queries' lower parts apart, added in one order
+    auto products = [&](const uint8_t* st, float (&sh)[TPU][NT][4]) {
 #pragma unroll
         for (int tt = 0; tt < TPU; ++tt) {
-            ks[tt] = __shfl_sync(0xffffffffu, cur.ks, ub * TPU + tt);
-            vs[tt] = __shfl_sync(0xffffffffu, cur.vs, ub * TPU + tt);
-            whole = whole && ks[tt] >= 0.f;
-        }
-        // ---- S^T: keys qr (+8), columns 2qc, 2qc + 1 of each row tile
-        float sh[TPU][NT][4];
-        bool grow = false;
-#pragma unroll
-        for (int tt = 0; tt < TPU; ++tt) {
-            float sl[NT][4];
+            float x0[NT][4], x1[NT][4], y0[PAIR ? 1 : NT][4], y1[PAIR ? 1 : NT][4];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sh[tt][nt][e] = sl[nt][e] = 0.f;
+                for (int e = 0; e < 4; ++e) {
+                    x0[nt][e] = x1[nt][e] = 0.f;
+                    if (!PAIR) y0[nt][e] = y1[nt][e] = 0.f;
+                }
 #pragma unroll
             for (int j = 0; j < D / 32; ++j) {
                 const uint4 w = *reinterpret_cast<const uint4*>(st + tt * 32 * D + j * 512);
@@ -315,27 +288,80 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     const uint2 q0 = query(0, 2 * j, nt), q1 = query(0, 2 * j + 1, nt);
-                    mma_f16_16816(sh[tt][nt], a0, q0.x, q0.y);
+                    mma_f16_16816(x0[nt], a0, q0.x, q0.y);
+                    mma_f16_16816(x1[nt], a1, q1.x, q1.y);
                     if (!PAIR) {
-                        const uint2 p0 = query(1, 2 * j, nt);
-                        mma_f16_16816(sl[nt], a0, p0.x, p0.y);
-                    }
-                    mma_f16_16816(sh[tt][nt], a1, q1.x, q1.y);
-                    if (!PAIR) {
-                        const uint2 p1 = query(1, 2 * j + 1, nt);
-                        mma_f16_16816(sl[nt], a1, p1.x, p1.y);
+                        const uint2 p0 = query(1, 2 * j, nt), p1 = query(1, 2 * j + 1, nt);
+                        mma_f16_16816(y0[nt], a0, p0.x, p0.y);
+                        mma_f16_16816(y1[nt], a1, p1.x, p1.y);
                     }
                 }
-            }
-            if (PAIR) {                                // lane qc holds columns 2qc, + 1; qc + 2 their lower parts
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sl[0][e] = __shfl_xor_sync(0xffffffffu, sh[tt][0][e], 2);
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sh[tt][nt][e] = (sh[tt][nt][e] + sl[nt][e]) * (cs[nt][e & 1] * ks[tt]);
+                for (int e = 0; e < 4; ++e) {
+                    const float hi = x0[nt][e] + x1[nt][e];
+                    // paired: lane qc holds columns 2qc, + 1; qc + 2 their lower parts
+                    const float lo = PAIR ? __shfl_xor_sync(0xffffffffu, hi, 2) : y0[PAIR ? 0 : nt][e] + y1[PAIR ? 0 : nt][e];
+                    sh[tt][nt][e] = hi + lo;
+                }
         }
+    };
+    auto arrived = [&](int u, int slot, uint32_t phase) {
+        if (__all_sync(0xffffffffu, mbar_wait(&full[slot], phase, a.err))) return true;
+        // a copy never came (error word 0x80): wait, bounded, for those still in flight
+        if (lane == 0) {
+            failed = 1;
+            for (int w = u + 1; w < min(mine, u + kQdDepth); ++w)
+                mbar_wait(&full[w % kQdDepth], (uint32_t)((w / kQdDepth) & 1), nullptr);
+        }
+        __syncwarp();
+        return false;
+    };
+
+    // One row tile of d 128 (a unit of d 64 has two tiles to overlap): the next unit's scores are computed among this one's
+    // probabilities and V products (a warp's own chain of latencies, not issue
+    // slots, is what a unit takes)
+    constexpr bool AHEAD = NT == 1 && D == 128;
+    float sn[TPU][NT][4];
+    int slot = 0;
+    uint32_t phase = 0;
+    bool go = mine > 0;
+    if (AHEAD && go) {
+        go = arrived(0, 0, 0u);
+        products(ring + lane * 16, sn);
+    }
+    for (int u = 0; u < mine && go; ++u) {
+        const int ub = u % UPB;
+        if (ub == 0) {
+            if (u > 0) cur = nxt;
+            nxt.pid = check_pid(u + UPB, load_pid(u + UPB));
+        } else if (ub == UPB / 2) {
+            load_scale(nxt.pid, nxt.ks, nxt.vs);
+        }
+        const uint8_t* st = ring + slot * kQdUnit + lane * 16;
+        const int slot1 = slot + 1 == kQdDepth ? 0 : slot + 1;
+        const uint32_t phase1 = slot1 == 0 ? phase ^ 1u : phase;
+        if (AHEAD ? u + 1 < mine && !arrived(u + 1, slot1, phase1) : !arrived(u, slot, phase)) break;
+        const int key0 = key_of(u);
+        float ks[TPU], vs[TPU];
+        bool whole = key0 + UT - 1 <= all_see;         // every key of the unit is there for every row
+#pragma unroll
+        for (int tt = 0; tt < TPU; ++tt) {
+            ks[tt] = __shfl_sync(0xffffffffu, cur.ks, ub * TPU + tt);
+            vs[tt] = __shfl_sync(0xffffffffu, cur.vs, ub * TPU + tt);
+            whole = whole && ks[tt] >= 0.f;
+        }
+        float sh[TPU][NT][4];
+        bool grow = false;
+        if (!AHEAD) products(st, sn);
+#pragma unroll
+        for (int tt = 0; tt < TPU; ++tt)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sh[tt][nt][e] = sn[tt][nt][e] * (cs[nt][e & 1] * ks[tt]);
         if (!whole) {
 #pragma unroll
             for (int tt = 0; tt < TPU; ++tt)
@@ -407,6 +433,8 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o[nt][md][e] *= dn;
         }
+        // (past the last unit: over stale bytes, unused)
+        if (AHEAD) products(ring + slot1 * kQdUnit + lane * 16, sn);
 #pragma unroll
         for (int tt = 0; tt < TPU; ++tt) {
             const float vf = q8_pow2(max(q8_scale_exp(vs[tt]) - eo + kQdBias, -126));
@@ -464,7 +492,8 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
         __syncwarp();
         const int un = u + kQdDepth;
         if (un < mine) issue(un, slot, ub + kQdDepth < UPB ? cur.pid : nxt.pid);
-        if (++slot == kQdDepth) slot = 0, phase ^= 1u;
+        slot = slot1;
+        phase = phase1;
     }
     __syncwarp();
 

@@ -69,11 +69,13 @@ DKV_DEV void q8_merge_splits(const Q8AttnArgs& a, size_t bhr, int b, int h, int 
     __shared__ int is_last;
     __syncthreads();                     // the CTA's partials are stored
     if (threadIdx.x == 0) {
+        // release and acquire on the device, cumulative over the barriers: the
+        // CTA's stores before, the other CTAs' partials after
         unsigned* tk = a.tickets + bhr;
-        __threadfence();                 // (cumulative: the other threads' stores too, by the barrier)
-        is_last = atomicAdd(tk, 1u) == (unsigned)(a.n_splits - 1);
+        unsigned before;
+        asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;\n" : "=r"(before) : "l"(tk) : "memory");
+        is_last = before == (unsigned)(a.n_splits - 1);
         if (is_last) *tk = 0u;
-        __threadfence();
     }
     __syncthreads();
     if (!is_last) return;
