@@ -169,7 +169,9 @@ prof_active = False
 def call(name: str, *args) -> None:
     global prof_active
     lib = load()
-    check(getattr(lib, name)(*args), name)
+    status = getattr(lib, name)(*args)
+    if status != OK:
+        check(status, name)
     if name == "dkv_prof_start":
         prof_active = True
     elif name == "dkv_prof_stop":

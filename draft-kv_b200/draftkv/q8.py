@@ -17,7 +17,7 @@ from __future__ import annotations
 import numpy as np
 
 from . import _lib
-from .paged import BlockPool, BlockPoolExhausted, PagedKVCache, dtype_code
+from .paged import BlockPoolExhausted, PagedKVCache
 
 try:
     import torch
@@ -26,6 +26,7 @@ except ImportError:  # pragma: no cover
 
 BLOCK_SIZES = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128)
+_CODES = {} if torch is None else {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 MASS_ROWS = 64          # query rows a KV head up to which attention can add up the mass
 
 
@@ -155,10 +156,12 @@ class Q8KVCache(PagedKVCache):
                 self._work[key] = w
         return w
 
-    def _on_device(self):
-        """The cache's device as the current one (launches go there)."""
+    def _stream(self) -> int:
+        """The current stream, of the cache's device (which has to be the current
+        one: launches go there)."""
         if torch.cuda.current_device() != self.device.index:
             raise ValueError(f"the cache is on {self.device}, the current device is cuda:{torch.cuda.current_device()}")
+        return _lib.stream_ptr()
 
     # ------------------------------------------------------ device calls
     def write(self, layer: int, k, v, entry0, n_rows=None, pos0=None, mass=None, pos=None) -> None:
@@ -167,14 +170,14 @@ class Q8KVCache(PagedKVCache):
         dimension contiguous (the same for both); entry0, n_rows, pos0: int32
         [batch].  mass / pos ([batch, n_kv, capacity]): reset for the new
         entries.  The pages must be in the table (`ensure`)."""
-        self._on_device()
-        if k.dim() != 4 or k.shape[0] != self.batch or k.shape[2] != self.n_heads or k.shape[3] != self.d_head:
-            raise ValueError(f"k must be [{self.batch}, rows, {self.n_heads}, {self.d_head}], got {tuple(k.shape)}")
-        if v.shape != k.shape or v.dtype != k.dtype or v.stride() != k.stride():
+        stream, shape, strides, code = self._stream(), k.shape, k.stride(), _CODES.get(k.dtype)
+        if len(shape) != 4 or shape[0] != self.batch or shape[2] != self.n_heads or shape[3] != self.d_head:
+            raise ValueError(f"k must be [{self.batch}, rows, {self.n_heads}, {self.d_head}], got {tuple(shape)}")
+        if v.shape != shape or v.dtype is not k.dtype or v.stride() != strides:
             raise ValueError("k and v must have one shape, dtype and strides")
         if k.device != self.device or v.device != self.device:
             raise ValueError(f"k and v must be on {self.device}")
-        if k.dtype not in (torch.bfloat16, torch.float32) or k.stride(3) != 1:
+        if code is None or strides[3] != 1:
             raise ValueError("k and v must be bf16 or fp32 with a contiguous last dimension")
         _check_i32("entry0", entry0, (self.batch,), self.device)
         for name, t in (("n_rows", n_rows), ("pos0", pos0)):
@@ -183,13 +186,12 @@ class Q8KVCache(PagedKVCache):
         self._check_mass(mass)
         if pos is not None:
             _check_i32("pos", pos, self._mass_shape(), self.device)
-        rows = k.shape[1]
+        rows = shape[1]
         if rows == 0:
             return
-        sb, st, sh, _ = k.stride()
-        _lib.call("dkv_q8_append", self.struct(), self._dims, layer, k.data_ptr(), v.data_ptr(), dtype_code(k.dtype), rows,
-                  sb, st, sh, entry0.data_ptr(), _lib.ptr(n_rows), _lib.ptr(pos0), _lib.ptr(mass), _lib.ptr(pos),
-                  _lib.stream_ptr())
+        _lib.call("dkv_q8_append", self.struct(), self._dims, layer, k.data_ptr(), v.data_ptr(), code, rows, strides[0],
+                  strides[1], strides[2], entry0.data_ptr(), _lib.ptr(n_rows), _lib.ptr(pos0), _lib.ptr(mass),
+                  _lib.ptr(pos), stream)
 
     def _mass_shape(self):
         return (self.batch, self.n_heads, self.capacity_tokens)
@@ -211,34 +213,31 @@ class Q8KVCache(PagedKVCache):
         scratch of `dkv_q8_attn_work_bytes` (zero when first used) for a caller
         that runs or replays calls side by side; by default the cache keeps one
         per stream and call shape."""
-        self._on_device()
-        if q.dim() != 4 or q.shape[0] != self.batch or q.shape[3] != self.d_head or q.shape[2] % self.n_heads \
-                or q.shape[2] == 0:
-            raise ValueError(f"q must be [{self.batch}, T, a multiple of {self.n_heads} heads, {self.d_head}], "
-                             f"got {tuple(q.shape)}")
-        if q.dtype != torch.float32 or not q.is_contiguous() or q.device != self.device:
+        stream, shape, kv = self._stream(), q.shape, self.n_heads
+        if len(shape) != 4 or shape[0] != self.batch or shape[3] != self.d_head or shape[2] % kv or not shape[2]:
+            raise ValueError(f"q must be [{self.batch}, T, a multiple of {kv} heads, {self.d_head}], got {tuple(shape)}")
+        if q.dtype is not torch.float32 or q.device != self.device or not q.is_contiguous():
             raise ValueError(f"q must be a contiguous float32 tensor on {self.device}")
         _check_i32("entry0", entry0, (self.batch,), self.device)
         if n_rows is not None:
             _check_i32("n_rows", n_rows, (self.batch,), self.device)
         self._check_mass(mass)
-        T, group = q.shape[1], q.shape[2] // self.n_heads
+        T, group = shape[1], shape[2] // kv
         if out is None:
             make = torch.empty if n_rows is None else torch.zeros
-            out = make(q.shape, dtype=out_dtype or torch.bfloat16, device=self.device)
-        elif out.shape != q.shape or not out.is_contiguous() or out.device != self.device \
-                or (out_dtype is not None and out.dtype != out_dtype):
+            out = make(shape, dtype=out_dtype or torch.bfloat16, device=self.device)
+        elif out.shape != shape or not out.is_contiguous() or out.device != self.device \
+                or (out_dtype is not None and out.dtype is not out_dtype):
             raise ValueError("out must be contiguous and shaped like q")
-        if out.dtype not in (torch.bfloat16, torch.float32):
+        code = _CODES.get(out.dtype)
+        if code is None:
             raise ValueError("attention writes bf16 or fp32")
         if T == 0:
             return out
-        stream = _lib.stream_ptr()
         if work is None:
             work = self._workspace(T, group, split_keys, mass is not None, stream)
         _lib.call("dkv_q8_attn", self.struct(), self._dims, layer, group, T, q.data_ptr(), entry0.data_ptr(),
-                  _lib.ptr(n_rows), out.data_ptr(), dtype_code(out.dtype), split_keys, _lib.ptr(mass), work.data_ptr(),
-                  work.numel(), stream)
+                  _lib.ptr(n_rows), out.data_ptr(), code, split_keys, _lib.ptr(mass), work.data_ptr(), work.numel(), stream)
         return out
 
     def evict_rows(self, layer: int, n, budget, out_table, mass, pos=None, sink: int = 0, recent: int = 0,
@@ -250,7 +249,7 @@ class Q8KVCache(PagedKVCache):
         which must be in no row of the page table.  Returns (kept [batch, n_kv,
         out_pages * block_size] int32 entry indices, -1 behind; mass_out;
         pos_out or None)."""
-        self._on_device()
+        stream = self._stream()
         _check_i32("n", n, (self.batch,), self.device)
         _check_i32("budget", budget, (self.batch,), self.device)
         if out_table.dim() != 2:
@@ -273,15 +272,15 @@ class Q8KVCache(PagedKVCache):
         kept = torch.empty((self.batch, self.n_heads, out_pages * self.block_size), dtype=torch.int32, device=self.device)
         _lib.call("dkv_q8_evict", self.struct(), self._dims, layer, n.data_ptr(), budget.data_ptr(), sink, recent,
                   mass.data_ptr(), _lib.ptr(pos), out_table.data_ptr(), out_pages, mass_out.data_ptr(), _lib.ptr(pos_out),
-                  kept.data_ptr(), _lib.stream_ptr())
+                  kept.data_ptr(), stream)
         return kept, mass_out, pos_out
 
     def read_rows(self, layer: int, n: int, b: int = 0):
         """Entries [0, n) of one sequence, dequantized: fp32 [n, n_kv, 2, d] on
         the device."""
-        self._on_device()
+        stream = self._stream()
         out = torch.empty((n, self.n_heads, 2, self.d_head), dtype=torch.float32, device=self.device)
-        _lib.call("dkv_q8_read", self.struct(), self._dims, b, layer, n, out.data_ptr(), _lib.stream_ptr())
+        _lib.call("dkv_q8_read", self.struct(), self._dims, b, layer, n, out.data_ptr(), stream)
         return out
 
     # ---------------------------------------------------- cache protocol
