@@ -282,6 +282,13 @@ DKV_DEV uint2 dsmem_ld2(const void* p, uint32_t rank) {
         : "r"(smem_u32(p)), "r"(rank));
     return v;
 }
+DKV_DEV unsigned dsmem_ld(const void* p, uint32_t rank) {
+    unsigned v;
+    asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %1, %2;\n ld.shared::cluster.u32 %0, [a];\n}\n"
+                 : "=r"(v)
+                 : "r"(smem_u32(p)), "r"(rank));
+    return v;
+}
 DKV_DEV unsigned warp_scan(unsigned v) {      // inclusive
     const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -291,14 +298,23 @@ DKV_DEV unsigned warp_scan(unsigned v) {      // inclusive
     }
     return v;
 }
+// Inclusive sums over the block's threads in order (all 32 warps; a barrier inside).
+DKV_DEV unsigned block_scan(unsigned v, unsigned* wsum) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const unsigned run = warp_scan(v);
+    if (lane == 31) wsum[warp] = run;
+    __syncthreads();
+    const unsigned w = wsum[lane], upto = warp_scan(w);
+    return run + __shfl_sync(0xffffffffu, upto - w, warp);
+}
 
 // Which entries stay: per (sequence, head) the `drop` lowest (mass, index) of
 // the unprotected entries go.  A cluster of CTAs takes a (sequence, head), each
 // CTA a contiguous slice of the entries whose order-preserving keys it keeps in
 // shared memory (slices that do not fit are read from global memory again).
 // Radix select of the drop-th smallest key in three passes (11, 11, 10 bits):
-// each CTA's histogram is summed over the cluster through distributed shared
-// memory (one cluster barrier a pass: every pass has a histogram of its own), so
+// the CTAs' histograms are summed over the cluster through distributed shared
+// memory, a part of the bins a CTA (every pass has a histogram of its own), and
 // every CTA finds the same bin.  Plain shared-memory atomics: grouping a warp's
 // equal bins first (match) took 200 cycles a warp, more than 32 atomics to one
 // address.  The counts below and at the key give each slice its place, and one
@@ -307,7 +323,7 @@ DKV_DEV unsigned warp_scan(unsigned v) {      // inclusive
 __global__ void __launch_bounds__(kSelThreads) q8_select_kernel(Q8EvictArgs a, int cluster, int smem_keys) {
     extern __shared__ __align__(16) unsigned sel_sm[];
     unsigned* keys_s = sel_sm + 3 * kSelBins;      // (histograms [3][kSelBins] first)
-    __shared__ unsigned wsum[32], wbelow[32], wcnt[64], s_bin, s_below;
+    __shared__ unsigned part_s[kSelThreads], wsum[32], wbelow[32], wcnt[64], s_bin, s_below;
     __shared__ __align__(8) uint2 counts;
     const uint32_t rank = cluster > 1 ? cluster_rank() : 0u;
     const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -344,7 +360,7 @@ __global__ void __launch_bounds__(kSelThreads) q8_select_kernel(Q8EvictArgs a, i
             const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : kSelBits;
             const unsigned mask = pass == 0 ? 0u : 0xffffffffu << (shift + bits);
             const int from = max(i0, f0), to = min(i1, f1);
-#pragma unroll 4
+#pragma unroll 8
             for (int i = from + tid; i < to; i += kSelThreads) {
                 const unsigned key = key_at(i);
                 if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & ((1u << bits) - 1u)], 1u);
@@ -353,28 +369,40 @@ __global__ void __launch_bounds__(kSelThreads) q8_select_kernel(Q8EvictArgs a, i
                 cluster_sync_all();
             else
                 __syncthreads();
-            // the cluster's sums, thread i's bins 2 i and 2 i + 1, and their prefix sums
             const uint2 own = *reinterpret_cast<const uint2*>(hist + 2 * tid);
-            uint2 c = own;
-            if (cluster > 1) {
-                uint2 part[kSelMaxCluster];
+            if (cluster == 1) {
+                // thread i's bins 2 i and 2 i + 1, and the prefix sums over all
+                const unsigned before = block_scan(own.x + own.y, wsum) - own.x - own.y;
+                const unsigned e1 = before + own.x;                           // entries in bins below
+                if (before < need && need <= e1) s_bin = 2 * tid, s_below = before;
+                if (e1 < need && need <= e1 + own.y) s_bin = 2 * tid + 1, s_below = e1;
+            } else {
+                // a CTA sums a part of the bins over the cluster and scans it; every
+                // CTA then finds the part that holds the bin, and the bin in it
+                const int part = kSelBins / cluster;
+                unsigned c = 0;
+                if (tid < part) {
+                    unsigned x[kSelMaxCluster];
 #pragma unroll
-                for (int r = 0; r < kSelMaxCluster; ++r) {
-                    part[r] = make_uint2(0u, 0u);
-                    if (r < cluster) part[r] = dsmem_ld2(hist + 2 * tid, r);
+                    for (int r = 0; r < kSelMaxCluster; ++r)
+                        x[r] = r < cluster ? dsmem_ld(hist + (int)rank * part + tid, r) : 0u;
+#pragma unroll
+                    for (int r = 0; r < kSelMaxCluster; ++r) c += x[r];
                 }
-                c = make_uint2(0u, 0u);
-#pragma unroll
-                for (int r = 0; r < kSelMaxCluster; ++r) c.x += part[r].x, c.y += part[r].y;
+                const unsigned upto = block_scan(c, wsum);
+                part_s[tid] = upto;
+                cluster_sync_all();
+                const unsigned tot = lane < cluster ? dsmem_ld(part_s + part - 1, lane) : 0u;
+                const unsigned end = warp_scan(tot);
+                const unsigned hit = __ballot_sync(0xffffffffu, end - tot < need && need <= end);
+                const int owner = __ffs(hit) - 1;
+                const unsigned start = __shfl_sync(0xffffffffu, end - tot, owner);
+                if (tid < part) {
+                    const unsigned hi = start + dsmem_ld(part_s + tid, owner);
+                    const unsigned lo = tid ? start + dsmem_ld(part_s + tid - 1, owner) : start;
+                    if (lo < need && need <= hi) s_bin = owner * part + tid, s_below = lo;
+                }
             }
-            const unsigned run = warp_scan(c.x + c.y);
-            if (lane == 31) wsum[warp] = run;
-            __syncthreads();
-            const unsigned w = wsum[lane], upto = warp_scan(w);
-            const unsigned before = __shfl_sync(0xffffffffu, upto - w, warp);
-            const unsigned e0 = before + run - c.x - c.y, e1 = e0 + c.x;      // entries in bins below
-            if (e0 < need && need <= e0 + c.x) s_bin = 2 * tid, s_below = e0;
-            if (e1 < need && need <= e1 + c.y) s_bin = 2 * tid + 1, s_below = e1;
             __syncthreads();
             // this slice's entries in bins below the one found
             const unsigned bin = s_bin;
@@ -408,7 +436,7 @@ __global__ void __launch_bounds__(kSelThreads) q8_select_kernel(Q8EvictArgs a, i
         const int part = slice / 32, p0 = i0 + warp * part, p1 = min(p0 + part, i1);
         unsigned my_eq = 0, my_lt = 0;
         if (drop > 0)
-#pragma unroll 4
+#pragma unroll 8
             for (int i = max(p0, f0) + lane; i < min(p1, f1); i += 32) {
                 const unsigned k = key_at(i);
                 my_eq += k == prefix;
@@ -422,22 +450,14 @@ __global__ void __launch_bounds__(kSelThreads) q8_select_kernel(Q8EvictArgs a, i
         const unsigned se = warp_scan(we) - we, sl = warp_scan(wl) - wl;
         unsigned eq = eq_before + __shfl_sync(0xffffffffu, se, warp);
         unsigned gone = gone_before + __shfl_sync(0xffffffffu, sl, warp) + (min(eq, need) - min(eq_before, need));
-        constexpr int U = 4;                       // 32-entry groups whose loads are in flight together
+        constexpr int U = 8;                       // 32-entry groups whose loads are in flight together
         for (int c0 = p0; c0 < p1; c0 += 32 * U) {
-            float m[U];
-            int32_t p[U], o[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int i = c0 + 32 * u + lane;
-                const bool in = i < p1;
-                m[u] = in ? __ldg(mass + i) : 0.f;
-                p[u] = in && a.pos_out ? __ldg(a.pos + row * cap + i) : 0;
-            }
+            int32_t o[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int i = c0 + 32 * u + lane;
                 const bool in = i < p1, open = in && i >= f0 && i < f1 && drop > 0;
-                const unsigned k = open ? mass_key(m[u]) : 0xffffffffu;
+                const unsigned k = open ? key_at(i) : 0xffffffffu;
                 const bool is_eq = open && k == prefix;
                 const unsigned beq = __ballot_sync(0xffffffffu, is_eq);
                 const bool goes = open && (k < prefix || (is_eq && eq + __popc(beq & ((1u << lane) - 1u)) < need));
@@ -445,6 +465,15 @@ __global__ void __launch_bounds__(kSelThreads) q8_select_kernel(Q8EvictArgs a, i
                 o[u] = in && !goes ? i - (int)(gone + __popc(bg & ((1u << lane) - 1u))) : out_cap;
                 eq += __popc(beq);
                 gone += __popc(bg);
+            }
+            float m[U];
+            int32_t p[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int i = c0 + 32 * u + lane;
+                const bool stays = o[u] < out_cap;
+                m[u] = stays ? __ldg(mass + i) : 0.f;
+                p[u] = stays && a.pos_out ? __ldg(a.pos + row * cap + i) : 0;
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {

@@ -537,6 +537,24 @@ def test_evict_order_of_hard_masses(kind):
     run_evict(mk, r, [1270], [511], 3, 70, mass)
 
 
+@pytest.mark.parametrize("kv,pages,n,budget,kind", [
+    (1, 72, [9001], [2300], "lognormal"), (2, 160, [20000], [5000], "ties"), (1, 330, [42000], [40001], "lognormal"),
+    (1, 330, [700], [333], "ties"), (1, 3136, [401000], [2000], "ties"), (3, 330, [42240], [1], "equal")])
+def test_evict_from_long_sequences(kv, pages, n, budget, kind):
+    """Selections over several CTAs (clusters of 2, 4 and 8), a short sequence in a
+    long capacity, and slices that shared memory does not hold."""
+    mk = Made(1, 1, kv, 64, 128, pages, seed=4, spare=pages)
+    rng = np.random.default_rng(n[0])
+    mk.codes.copy_(torch.randint(0, 127, mk.codes.shape, dtype=torch.uint8, device="cuda"))      # any finite codes
+    mk.scale.copy_(torch.ldexp(torch.ones(mk.scale.shape, device="cuda"), torch.randint(-9, 3, mk.scale.shape, device="cuda")))
+    mass = np.exp(2 * rng.standard_normal((1, kv, mk.cap))).astype(np.float32)
+    if kind == "ties":
+        mass = np.round(mass * 2).astype(np.float32)
+    elif kind == "equal":
+        mass[:] = 1.5
+    run_evict(mk, mk.reference(), n, budget, 4, 64, mass)
+
+
 def test_evict_into_too_small_a_table_is_reported():
     mk = Made(1, 1, 1, 64, 16, 4, seed=2, spare=8)
     rng = np.random.default_rng(1)
