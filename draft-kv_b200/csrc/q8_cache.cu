@@ -503,36 +503,34 @@ __global__ void __launch_bounds__(kSelThreads) q8_select_kernel(Q8EvictArgs a, i
 // the largest magnitude, and codes whose scale changes are rounded once.  What
 // bounds it: the sectors the kept rows touch (half of a tile's K sectors for 4
 // kept rows of 16, nearly all of V's, whose rows are the bytes of every word):
-// 4 x 8 heads, 8192 of 32768 rows of d 128: 215 MB read and 45 MB written in 71 us.
-struct GatherRow {
-    const uint8_t* tile;       // the row's 16-token tile of K in its page (V: + a side), null: bad page or not there
-    int k;                     // row in the tile, -1: not there
+// 4 x 8 heads, 8192 of 32768 rows of d 128: 215 MB read and 45 MB written in 63 us.
+struct __align__(16) GatherRow {
+    const uint4* at;      // its first fragment (null: bad page or not there)
+    uint32_t pick;        // which byte (V, as a byte selector of two words) or word (K) of a fragment is its own
 };
 
 DKV_DEV __half2 as_h2(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
 DKV_DEV uint32_t as_u32(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
-// Largest magnitude of four codes (as f16, exact).
-DKV_DEV __half largest4(uint32_t w) {
+// Largest magnitude of four codes (exact).
+DKV_DEV float largest4(uint32_t w) {
     uint32_t lo, hi;
     q8_decode4(w, lo, hi);
     const __half2 m = __hmax2(__habs2(as_h2(lo)), __habs2(as_h2(hi)));
-    return __hmax(__low2half(m), __high2half(m));
+    return __half2float(__hmax(__low2half(m), __high2half(m)));
 }
-// 2^(e_src - e_dst) as two f16 factors: codes that are not zero fit below 2^18,
-// and below 2^-28 every product rounds to zero.  What ends as a code other than
-// zero (2^-10 and more) is exact after each factor.
-struct Shift {
-    __half2 a, b;
-};
-DKV_DEV Shift shift_of(int e_src, int e_dst) {
+// 2^(e_src - e_dst) as two f16 factors (each twice): codes that are not zero fit
+// below 2^18, and below 2^-28 every product rounds to zero.  What ends as a code
+// other than zero (2^-10 and more) is exact after each factor.
+DKV_DEV uint2 shift_of(int e_src, int e_dst) {
     const int d = min(max(e_src - e_dst, -28), 18), x = d / 2;
-    return {__float2half2_rn(q8_pow2(x)), __float2half2_rn(q8_pow2(d - x))};
+    return make_uint2(as_u32(__float2half2_rn(q8_pow2(x))), as_u32(__float2half2_rn(q8_pow2(d - x))));
 }
-DKV_DEV uint32_t times4(uint32_t w, Shift f) {
+// Four codes times such a factor, rounded to codes again.
+DKV_DEV uint32_t times4(uint32_t w, uint2 f) {
     uint32_t lo, hi;
     q8_decode4(w, lo, hi);
-    lo = as_u32(__hmul2(__hmul2(as_h2(lo), f.a), f.b));
-    hi = as_u32(__hmul2(__hmul2(as_h2(hi), f.a), f.b));
+    lo = as_u32(__hmul2(__hmul2(as_h2(lo), as_h2(f.x)), as_h2(f.y)));
+    hi = as_u32(__hmul2(__hmul2(as_h2(hi), as_h2(f.x)), as_h2(f.y)));
     uint32_t r;
     asm("{\n .reg .b16 a, b;\n cvt.rn.satfinite.e4m3x2.f16x2 a, %1;\n cvt.rn.satfinite.e4m3x2.f16x2 b, %2;\n mov.b32 %0, {a, b};\n}\n"
         : "=r"(r)
@@ -559,8 +557,12 @@ template <int D, int TILES>              // tiles a page
 __global__ void __launch_bounds__(gather_threads(D, TILES)) q8_gather_kernel(Q8EvictArgs a) {
     constexpr int NT = gather_threads(D, TILES), WS = NT / 32, NJ = D / 32, FR = TILES * NJ / WS;
     static_assert(NT >= TILES * 16, "a thread for every row");
+    // per row: where its bytes are, its scale, the factors that bring its codes to
+    // the new scale
     __shared__ GatherRow rows[TILES * 16];
-    __shared__ int exps[TILES * 16], emax;
+    __shared__ uint2 factors[TILES * 16];
+    __shared__ float scales[TILES * 16];
+    __shared__ int emax;
     const Q8View& v = a.v;
     const int b = blockIdx.z >> 1, side = blockIdx.z & 1, h = blockIdx.y, pg = blockIdx.x, tid = threadIdx.x;
     const int wi = tid >> 5, lane = tid & 31;
@@ -579,12 +581,14 @@ __global__ void __launch_bounds__(gather_threads(D, TILES)) q8_gather_kernel(Q8E
     if (tid == 0) emax = kQ8ExpMin;
     int sp = -1;
     if (tid < TILES * 16) {
-        GatherRow r{nullptr, tid < cnt ? 0 : -1};
+        GatherRow r{nullptr, 0x40u};
         if (tid < cnt) {
             if (src >= 0 && src < n) sp = __ldg(v.row(b) + (src >> v.page_shift));
             if (v.ok(sp)) {
-                r.tile = v.side(sp, h, side) + (size_t)((src & (v.page - 1)) >> 4) * 16 * D;
-                r.k = src & 15;
+                const int k = src & 15;
+                r.at = reinterpret_cast<const uint4*>(v.side(sp, h, side)) + ((src & (v.page - 1)) >> 4) * D +
+                       (side ? (k & 7) >> 1 : (k & 7) * 4);
+                r.pick = side ? 0x40u + 0x11u * (uint32_t)((k >> 3) * 2 + (k & 1)) : (uint32_t)(k >> 3);
             } else {
                 sp = -1;
                 atomicOr(a.err, kErrQ8Page);              // (its values count as zeros)
@@ -601,78 +605,86 @@ __global__ void __launch_bounds__(gather_threads(D, TILES)) q8_gather_kernel(Q8E
     if (sp >= 0) sc = __ldg(v.scale + v.scale_at(sp, h, side));
     // fragment x of this warp: block x * WS + wi of the side = tile block / NJ, dims
     // block block % NJ, as words of one row each (K: rows g, g + 8, g, g + 8; V: a
-    // word a row, turned at the end); big: their largest magnitudes
+    // word a row, turned at the end)
     uint32_t w[FR][4];
-    __half2 big[FR][2];
 #pragma unroll
     for (int x = 0; x < FR; ++x) {
         const int blk = x * WS + wi, tile = blk / NJ, j = blk % NJ;
 #pragma unroll
         for (int q = 0; q < 4; ++q) w[x][q] = 0u;
-        if (tile * 16 < cnt) {
-            if (side == 0) {
+        if (tile * 16 >= cnt) continue;
+        if (side == 0) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const GatherRow r = rows[row_of(tile, i)];
-                    if (r.tile == nullptr) continue;
-                    const uint4 s = __ldg(reinterpret_cast<const uint4*>(r.tile + j * 512 + ((r.k & 7) * 4 + t) * 16));
-                    w[x][i] = r.k & 8 ? s.y : s.x;
-                    w[x][2 + i] = r.k & 8 ? s.w : s.z;
-                }
-            } else {
-                uint4 s[4];
-                uint32_t pick[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const GatherRow r = rows[row_of(tile, i)];
-                    pick[i] = 0x40u + 0x11u * (uint32_t)((r.k >> 3 & 1) * 2 + (r.k & 1));      // that byte of both words
-                    s[i] = r.tile == nullptr ? make_uint4(0u, 0u, 0u, 0u)
-                                             : __ldg(reinterpret_cast<const uint4*>(r.tile + j * 512 +
-                                                                                    (g * 4 + ((r.k & 7) >> 1)) * 16));
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    w[x][i] = __byte_perm(__byte_perm(s[i].x, s[i].y, pick[i]), __byte_perm(s[i].z, s[i].w, pick[i]), 0x5410);
+            for (int i = 0; i < 2; ++i) {
+                const GatherRow r = rows[row_of(tile, i)];
+                if (r.at == nullptr) continue;
+                const uint4 s = __ldg(r.at + j * 32 + t);
+                w[x][i] = r.pick ? s.y : s.x;
+                w[x][2 + i] = r.pick ? s.w : s.z;
             }
+        } else {
+            uint4 s[4];
+            uint32_t pick[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const GatherRow r = rows[row_of(tile, i)];
+                pick[i] = r.pick;
+                s[i] = r.at == nullptr ? make_uint4(0u, 0u, 0u, 0u) : __ldg(r.at + j * 32 + g * 4);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                w[x][i] = __byte_perm(__byte_perm(s[i].x, s[i].y, pick[i]), __byte_perm(s[i].z, s[i].w, pick[i]), 0x5410);
         }
-        big[x][0] = __halves2half2(largest4(w[x][0]), largest4(w[x][1]));
-        big[x][1] = __halves2half2(largest4(w[x][2]), largest4(w[x][3]));
     }
-    if (tid < TILES * 16) exps[tid] = min(max(q8_scale_exp(sc), kQ8ExpMin), kQ8ExpMax);
+    int er = 0;
+    if (tid < TILES * 16) {
+        er = min(max(q8_scale_exp(sc), kQ8ExpMin), kQ8ExpMax);
+        scales[tid] = q8_pow2(er);
+    }
     __syncthreads();
     float amax = 0.f;
 #pragma unroll
     for (int x = 0; x < FR; ++x) {
         const int tile = (x * WS + wi) / NJ;
+        if (side == 0) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const __half m = q & 1 ? __high2half(big[x][q >> 1]) : __low2half(big[x][q >> 1]);
-            amax = fmaxf(amax, __half2float(m) * q8_pow2(exps[row_of(tile, side ? q : q & 1)]));
+            for (int i = 0; i < 2; ++i)
+                amax = fmaxf(amax, fmaxf(largest4(w[x][i]), largest4(w[x][2 + i])) * scales[row_of(tile, i)]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) amax = fmaxf(amax, largest4(w[x][i]) * scales[row_of(tile, i)]);
         }
     }
-    int e = warp_max_i(q8_exp_of(amax));
-    if (lane == 0) atomicMax(&emax, e);
+    amax = warp_max(amax);
+    if (lane == 0) atomicMax(&emax, q8_exp_of(amax));
     __syncthreads();
-    e = emax;
+    const int e = emax;
+    if (tid < TILES * 16) factors[tid] = shift_of(er, e);
     if (tid == 0) v.scale[v.scale_at(pid, h, side)] = q8_pow2(e);
+    __syncthreads();
     uint8_t* out = v.side(pid, h, side);
 #pragma unroll
     for (int x = 0; x < FR; ++x) {
         const int blk = x * WS + wi, tile = blk / NJ;
         if (tile * 16 >= cnt) continue;
         uint4* at = reinterpret_cast<uint4*>(out + (size_t)blk * 512 + lane * 16);
-        uint32_t old[4] = {0u, 0u, 0u, 0u};
-        const bool whole = tile * 16 + 16 <= cnt;
-        if (!whole) {
-            const uint4 was = *at;
-            old[0] = was.x, old[1] = was.y, old[2] = was.z, old[3] = was.w;
-            if (side) transpose4(old);
-        }
+        if (side == 0) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int r = row_of(tile, side ? q : q & 1), er = exps[r];
-            if (er != e) w[x][q] = times4(w[x][q], shift_of(er, e));
-            if (!whole && r >= cnt) w[x][q] = old[q];
+            for (int i = 0; i < 2; ++i) {
+                const uint2 f = factors[row_of(tile, i)];
+                w[x][i] = times4(w[x][i], f), w[x][2 + i] = times4(w[x][2 + i], f);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[x][i] = times4(w[x][i], factors[row_of(tile, i)]);
+        }
+        if (tile * 16 + 16 > cnt) {                       // rows that are not there keep their bytes
+            const uint4 was = *at;
+            uint32_t old[4] = {was.x, was.y, was.z, was.w};
+            if (side) transpose4(old);
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (row_of(tile, side ? q : q & 1) >= cnt) w[x][q] = old[q];
         }
         if (side) transpose4(w[x]);
         *at = make_uint4(w[x][0], w[x][1], w[x][2], w[x][3]);
