@@ -112,14 +112,14 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
     // page id of tile `lane` of the batch that starts at this warp's unit u0 (-1 beyond the table)
     auto load_pid = [&](int u0) {
         const int pg = (key_of(u0 + lane / TPU) + (lane % TPU) * 16) >> v.page_shift;
-        return pg < v.max_pages ? __ldg(tab + pg) : -1;
+        return pg < v.max_pages ? q8_ld(tab + pg) : -1;
     };
     const int first_pid = load_pid(0);
     const int qr = lane >> 2, qc = lane & 3;
     float2 xq[NT][KS][2];
     auto load_q = [&](int nt, int kk, int u) {
         const int r = nt * 8 + (PAIR ? qr & 3 : qr), gr = rbase + r;      // this lane's operand row
-        return r < R ? __ldg(reinterpret_cast<const float2*>(
+        return r < R ? q8_ld(reinterpret_cast<const float2*>(
                            a.q + (((size_t)b * a.T + gr / G) * v.n_kv * G + h * G + gr % G) * D + kk * 16 + u * 8 + 2 * qc))
                      : make_float2(0.f, 0.f);
     };
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
     };
     auto load_scale = [&](int pid, float& ks, float& vs) {
         float2 sc = make_float2(-1.f, 1.f);
-        if (pid >= 0) sc = __ldg(reinterpret_cast<const float2*>(v.scale + v.scale_at(pid, h, 0)));
+        if (pid >= 0) sc = q8_ld(reinterpret_cast<const float2*>(v.scale + v.scale_at(pid, h, 0)));
         ks = sc.x;
         vs = sc.y;
     };

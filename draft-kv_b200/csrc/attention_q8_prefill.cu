@@ -161,12 +161,12 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
     // per 16-key group of the key range: page id and scales; keys of a bad page are not seen
     const int n_grp = (kend - k0 + 15) / 16;
     for (int i = threadIdx.x; i < ntiles * 8; i += kQpThreads) {
-        const int pid = i < n_grp ? __ldg(v.row(b) + ((k0 + i * 16) >> v.page_shift)) : -1;
+        const int pid = i < n_grp ? q8_ld(v.row(b) + ((k0 + i * 16) >> v.page_shift)) : -1;
         const bool ok = v.ok(pid);
         float2 sc = make_float2(1.f, 1.f);
         int ev = kQ8ExpMin;
         if (ok) {
-            sc = __ldg(reinterpret_cast<const float2*>(v.scale + v.scale_at(pid, h, 0)));
+            sc = q8_ld(reinterpret_cast<const float2*>(v.scale + v.scale_at(pid, h, 0)));
             ev = min(max(q8_scale_exp(sc.y), kQ8ExpMin), kQ8ExpMax);
             atomicMax(&emax_s, ev);
         } else if (i < n_grp) {
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
                 const uint8_t* at = v.side(max(pid, 0), h, i) + (size_t)((k0 + grp * 16) & (v.page - 1)) * D + lane * 16;
 #pragma unroll
                 for (int x = 0; x < NJ; ++x)
-                    r[gb][x] = pid >= 0 ? __ldg(reinterpret_cast<const uint4*>(at + x * 512)) : make_uint4(0u, 0u, 0u, 0u);
+                    r[gb][x] = pid >= 0 ? q8_ld(reinterpret_cast<const uint4*>(at + x * 512)) : make_uint4(0u, 0u, 0u, 0u);
             }
         };
         // row of key g (+8: row + 2) of group 2 w + gb, see qp_key; unit 2 t + (x & 1) of the 64-dim half x >> 1
@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
                 const bool there = t * kQpTile + row < R && qr / G < n_tok;
                 float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (there)
-                    x = __ldg(reinterpret_cast<const float4*>(
+                    x = q8_ld(reinterpret_cast<const float4*>(
                         a.q + (((size_t)b * a.T + qr / G) * v.n_kv * G + h * G + qr % G) * D + 4 * li));
                 float am = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
 #pragma unroll

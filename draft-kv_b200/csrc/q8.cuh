@@ -56,6 +56,35 @@ DKV_DEV int q8_exp_of(float amax) {
     return min(max(e, kQ8ExpMin), kQ8ExpMax);
 }
 
+// Loads of what an earlier kernel of the stream may write.  Not the read-only
+// path: this kernel's start and the earlier one's end overlap (pdl_wait), so
+// the memory is not read-only while it runs, and a load must not pass the wait.
+DKV_DEV uint4 q8_ld(const uint4* p) {
+    uint4 x;
+    asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "l"(p));
+    return x;
+}
+DKV_DEV float4 q8_ld(const float4* p) {
+    float4 x;
+    asm volatile("ld.global.v4.f32 {%0,%1,%2,%3}, [%4];\n" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "l"(p));
+    return x;
+}
+DKV_DEV float2 q8_ld(const float2* p) {
+    float2 x;
+    asm volatile("ld.global.v2.f32 {%0,%1}, [%2];\n" : "=f"(x.x), "=f"(x.y) : "l"(p));
+    return x;
+}
+DKV_DEV float q8_ld(const float* p) {
+    float x;
+    asm volatile("ld.global.f32 %0, [%1];\n" : "=f"(x) : "l"(p));
+    return x;
+}
+DKV_DEV int32_t q8_ld(const int32_t* p) {
+    int32_t x;
+    asm volatile("ld.global.s32 %0, [%1];\n" : "=r"(x) : "l"(p));
+    return x;
+}
+
 // Two fp32 values to two e4m3 codes (low byte = a), nearest even, saturating.
 DKV_DEV uint32_t q8_encode2(float a, float b) {
     uint16_t r;

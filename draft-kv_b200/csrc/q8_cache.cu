@@ -156,11 +156,11 @@ __global__ void __launch_bounds__(kQ8Threads) q8_append_kernel(Q8AppendArgs a) {
             const int64_t o = off + r * a.st + x;
             float e[8];
             if (a.src_dtype == DKV_F32) {
-                const float4 p = __ldg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(src) + o));
-                const float4 q = __ldg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(src) + o + 4));
+                const float4 p = q8_ld(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(src) + o));
+                const float4 q = q8_ld(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(src) + o + 4));
                 e[0] = p.x, e[1] = p.y, e[2] = p.z, e[3] = p.w, e[4] = q.x, e[5] = q.y, e[6] = q.z, e[7] = q.w;
             } else {
-                const uint4 p = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(src) + o));
+                const uint4 p = q8_ld(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(src) + o));
                 const uint32_t w[4] = {p.x, p.y, p.z, p.w};
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
@@ -348,9 +348,9 @@ __global__ void __launch_bounds__(kSelThreads) q8_select_kernel(Q8EvictArgs a, i
     auto key_of = [&](int i, float m) { return i >= f0 && i < f1 ? mass_key(m) : 0xffffffffu; };
     if (staged && drop > 0) {
 #pragma unroll 8
-        for (int i = i0 + tid; i < i1; i += kSelThreads) keys_s[i - i0] = key_of(i, __ldg(mass + i));
+        for (int i = i0 + tid; i < i1; i += kSelThreads) keys_s[i - i0] = key_of(i, q8_ld(mass + i));
     }
-    auto key_at = [&](int i) { return staged ? keys_s[i - i0] : key_of(i, __ldg(mass + i)); };
+    auto key_at = [&](int i) { return staged ? keys_s[i - i0] : key_of(i, q8_ld(mass + i)); };
     __syncthreads();
 
     unsigned prefix = 0, need = (unsigned)drop, below = 0, equal = 0;      // below, equal: this slice's counts
@@ -472,8 +472,8 @@ __global__ void __launch_bounds__(kSelThreads) q8_select_kernel(Q8EvictArgs a, i
             for (int u = 0; u < U; ++u) {
                 const int i = c0 + 32 * u + lane;
                 const bool stays = o[u] < out_cap;
-                m[u] = stays ? __ldg(mass + i) : 0.f;
-                p[u] = stays && a.pos_out ? __ldg(a.pos + row * cap + i) : 0;
+                m[u] = stays ? q8_ld(mass + i) : 0.f;
+                p[u] = stays && a.pos_out ? q8_ld(a.pos + row * cap + i) : 0;
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(gather_threads(D, TILES)) q8_gather_kernel(Q8E
     pdl_trigger();
     pdl_wait();
     const int src = tid < TILES * 16 ? a.kept[(((size_t)b * v.n_kv + h) * a.out_pages + pg) * v.page + tid] : -1;
-    const int pid = __ldg(a.out_table + (size_t)b * a.out_pages + pg);
+    const int pid = q8_ld(a.out_table + (size_t)b * a.out_pages + pg);
     int n;
     const int keep = evict_keep(a, b, &n);
     const int cnt = min(keep - (pg << v.page_shift), v.page);
@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(gather_threads(D, TILES)) q8_gather_kernel(Q8E
     if (tid < TILES * 16) {
         GatherRow r{nullptr, 0x40u};
         if (tid < cnt) {
-            if (src >= 0 && src < n) sp = __ldg(v.row(b) + (src >> v.page_shift));
+            if (src >= 0 && src < n) sp = q8_ld(v.row(b) + (src >> v.page_shift));
             if (v.ok(sp)) {
                 const int k = src & 15;
                 r.at = reinterpret_cast<const uint4*>(v.side(sp, h, side)) + ((src & (v.page - 1)) >> 4) * D +
@@ -602,7 +602,7 @@ __global__ void __launch_bounds__(gather_threads(D, TILES)) q8_gather_kernel(Q8E
         return tile * 16 + (side ? 2 * t + (i & 1) + 8 * (i >> 1) : g + 8 * i);
     };
     float sc = 1.f;
-    if (sp >= 0) sc = __ldg(v.scale + v.scale_at(sp, h, side));
+    if (sp >= 0) sc = q8_ld(v.scale + v.scale_at(sp, h, side));
     // fragment x of this warp: block x * WS + wi of the side = tile block / NJ, dims
     // block block % NJ, as words of one row each (K: rows g, g + 8, g, g + 8; V: a
     // word a row, turned at the end)
@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(gather_threads(D, TILES)) q8_gather_kernel(Q8E
             for (int i = 0; i < 2; ++i) {
                 const GatherRow r = rows[row_of(tile, i)];
                 if (r.at == nullptr) continue;
-                const uint4 s = __ldg(r.at + j * 32 + t);
+                const uint4 s = q8_ld(r.at + j * 32 + t);
                 w[x][i] = r.pick ? s.y : s.x;
                 w[x][2 + i] = r.pick ? s.w : s.z;
             }
@@ -629,7 +629,7 @@ __global__ void __launch_bounds__(gather_threads(D, TILES)) q8_gather_kernel(Q8E
             for (int i = 0; i < 4; ++i) {
                 const GatherRow r = rows[row_of(tile, i)];
                 pick[i] = r.pick;
-                s[i] = r.at == nullptr ? make_uint4(0u, 0u, 0u, 0u) : __ldg(r.at + j * 32 + g * 4);
+                s[i] = r.at == nullptr ? make_uint4(0u, 0u, 0u, 0u) : q8_ld(r.at + j * 32 + g * 4);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i)
