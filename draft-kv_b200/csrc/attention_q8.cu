@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
 #pragma unroll
         for (int kk = 0; kk < KS; ++kk) xq[nt][kk][0] = load_q(nt, kk, 0), xq[nt][kk][1] = load_q(nt, kk, 1);
     const int n_tok = a.n_rows ? min(a.n_rows[b], a.T) : a.T;
-    const int e0 = a.entry0[b];
+    const int e0 = a.first(b);
     // the block's last token decides what is read
     const int t_last = min((rbase + R - 1) / G, n_tok - 1);
     const int n_keys = t_last >= rbase / G ? max(0, min(a.n_keys(b), e0 + t_last + 1)) : 0;
@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(kMassThreads) q8_mass_kernel(Q8AttnArgs a, flo
     pdl_trigger();
     pdl_wait();
     const int h = blockIdx.y, b = blockIdx.z, R = a.T * a.group;
-    const int n = a.n_keys(b), e0 = a.entry0[b], key0 = blockIdx.x * kMassThreads * kMassKeys + threadIdx.x;
+    const int n = a.n_keys(b), e0 = a.first(b), key0 = blockIdx.x * kMassThreads * kMassKeys + threadIdx.x;
     if ((int)(blockIdx.x * kMassThreads * kMassKeys) >= n) return;
     const size_t bh = (size_t)b * a.v.n_kv + h, cap = a.v.capacity();
     float old[kMassKeys], sum[kMassKeys];
@@ -634,11 +634,11 @@ int row_block(int R) { return R <= 8 ? 8 : 16; }
 
 // Keys per split (a multiple of 256: whole units of all 8 warps) where the
 // caller names none: one wave of two CTAs an SM over (sequence, head, split),
-// and at least 256 KB of codes a split.  A CTA costs about 8 us apart from its
-// stream (measured on B200 over one sequence of 262144 entries: 37 splits a
-// head 98 us, 256 splits 147 us) and streams 256 KB in about as long.  It
-// depends on the batch, the heads and the capacity only, so a sequence's verify
-// and decode calls share it.
+// and at least 128 KB of codes a split: a CTA costs some microseconds apart
+// from its stream (one sequence of 262144 entries, 8 heads: 37 splits a head
+// 90 us, 256 splits a third longer), and in a capacity far above the length the
+// smaller splits leave the sequence more CTAs.  It depends on the batch, the
+// heads and the capacity only, so a sequence's verify and decode calls share it.
 int default_split(int batch, int n_kv, int d, int capacity) {
     const int ctas = std::max(1, 2 * 148 / std::max(1, batch * n_kv));
     const int keys = (int)(((long long)capacity + ctas - 1) / ctas);
@@ -646,7 +646,8 @@ int default_split(int batch, int n_kv, int d, int capacity) {
 }
 
 int pick_split(dkv_dims dims, int capacity, int split_keys) {
-    return split_keys > 0 ? split_keys : default_split(dims.batch, dims.n_kv, dims.d, capacity);
+    if (split_keys > 0) return std::min(split_keys, (capacity + 127) / 128 * 128);
+    return default_split(dims.batch, dims.n_kv, dims.d, capacity);
 }
 
 size_t decode_work(dkv_dims dims, int R, int capacity, int split, bool mass, Q8AttnArgs* a, Arena* ar) {
@@ -684,7 +685,7 @@ using namespace dkv;
 extern "C" size_t dkv_q8_attn_work_bytes(dkv_dims dims, int group, int T, int capacity, int split_keys, int note_mass) {
     if (dims.batch < 1 || dims.n_kv < 1 || group < 1 || T < 1 || capacity < 1) return 0;
     const long long R = (long long)T * group;
-    if (R > (1 << 24)) return 0;
+    if (R > (1 << 24) || capacity > (1 << 30)) return 0;
     if (R > kQ8MaxRows) return attn_q8_prefill_work(dims, group, T, capacity);
     return decode_work(dims, (int)R, capacity, pick_split(dims, capacity, split_keys), note_mass != 0,
                        nullptr, nullptr);
@@ -730,7 +731,7 @@ extern "C" int dkv_q8_attn(const dkv_q8_cache* cache, dkv_dims dims, int layer, 
     decode_work(dims, R, cap, a.split, mass != nullptr, &a, &ar);
     DKV_REQUIRE(a.tickets && a.part && (!mass || (a.scores && a.stats)), "dkv_q8_attn: work buffer");
     const size_t n_tk = (size_t)dims.batch * dims.n_kv * a.n_rb;
-    DKV_REQUIRE(n_tk <= kQ8Tickets && (size_t)dims.batch * a.n_rb <= 65535,
+    DKV_REQUIRE((a.n_splits == 1 || n_tk <= kQ8Tickets) && (size_t)dims.batch * a.n_rb <= 65535,
                 "dkv_q8_attn: batch x heads x row blocks too large");
     const dim3 grid((unsigned)a.n_splits, (unsigned)dims.n_kv, (unsigned)(dims.batch * a.n_rb));
     ProfScope ps(DKV_PROF_ATTN_FULL, 0.0, st);

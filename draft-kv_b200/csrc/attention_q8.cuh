@@ -7,6 +7,7 @@ namespace dkv {
 
 constexpr int kQ8MaxRows = 64;         // query rows (token x GQA head) of a decode / verify call
 constexpr size_t kQ8Tickets = 16384;   // fixed ticket region at the start of the work buffer
+static_assert(kQ8Tickets * sizeof(unsigned) == 65536, "the 64 KB that callers clear");
 
 struct Q8AttnArgs {
     Q8View v;
@@ -25,6 +26,8 @@ struct Q8AttnArgs {
     int s_ld;
     uint32_t* err;
 
+    // token 0's entry, held to the capacity (entries behind it are recorded by beyond())
+    DKV_DEV int first(int b) const { return min(entry0[b], v.capacity()); }
     // entries the T tokens of sequence b may see at most (its own included)
     DKV_DEV int n_keys(int b) const {
         const int n = n_rows ? min(n_rows[b], T) : T;

@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
 
     pdl_trigger();
     pdl_wait();
-    const int e0 = a.entry0[b];
+    const int e0 = a.first(b);
     const int n_tok = a.n_rows ? min(a.n_rows[b], a.T) : a.T;
     const int t_last = min((r0 + R - 1) / G, n_tok - 1);
     const int n_keys = t_last >= r0 / G ? max(0, min(a.n_keys(b), e0 + t_last + 1)) : 0;
@@ -500,9 +500,10 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
         float* mypart = alone ? nullptr : a.part + ((bhr * a.n_splits + s) * kQpRows + cr) * PS;
         if (l != l && m == -INFINITY) m = 0.f;     // NaN scores have no max: give the row one, so that its NaN comes out
         const bool live = ok && m != -INFINITY;
-        // O is in units of 2^(evm - bias), l in units of 2^-bias
-        const float un = q8_pow2(evm);
-        const float f = alone ? (live ? un / l : 0.f) : un * q8_pow2(-kQpBias);
+        // O is in units of 2^(evm - bias), l in units of 2^-bias.  (Apart from the
+        // sum: 2^evm / l may be too small for fp32 where their result is not.)
+        const float un = alone ? q8_pow2(evm) : q8_pow2(evm - kQpBias);
+        const float f = alone && live ? 1.f / l : 1.f;
         const size_t out_at = (((size_t)b * a.T + gr / G) * v.n_kv * G + h * G + gr % G) * D;
         if (__all_sync(0xffffffffu, ok)) {
 #pragma unroll 1
@@ -512,7 +513,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
                 tmem_wait_ld();
                 if (!mine) continue;
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = live ? __float_as_uint(__uint_as_float(o[e]) * f) : 0u;
+                for (int e = 0; e < 32; ++e) o[e] = live ? __float_as_uint(__uint_as_float(o[e]) * f * un) : 0u;
                 if (!alone || a.out_dtype == DKV_F32) {
                     if (!alone && !live) continue;
                     float* to = alone ? reinterpret_cast<float*>(a.out) + out_at + c0 : mypart + 4 + c0;
@@ -582,7 +583,7 @@ int attn_q8_prefill(Q8AttnArgs& a, dkv_dims dims, void* work, size_t work_bytes,
     prefill_layout(dims, a.group, a.T, a.v.capacity(), &a, &ar);
     DKV_REQUIRE(a.tickets && a.part, "dkv_q8_attn: work buffer");
     const size_t n_tk = (size_t)dims.batch * dims.n_kv * a.n_rb;
-    DKV_REQUIRE(n_tk <= kQ8Tickets && n_tk * a.n_splits <= 0x7fffffffu, "dkv_q8_attn: batch x heads x row blocks too large");
+    DKV_REQUIRE((a.n_splits == 1 || n_tk <= kQ8Tickets) && n_tk * a.n_splits <= 0x7fffffffu, "dkv_q8_attn: batch x heads x row blocks too large");
     ProfScope ps(DKV_PROF_ATTN_FULL, 0.0, st);
     const dim3 grid((unsigned)(n_tk * a.n_splits));
     if (dims.d == 128) {

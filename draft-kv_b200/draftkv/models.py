@@ -293,7 +293,7 @@ class DeviceDecoder:
         cache.ensure(0, n + T)
         tok = torch.tensor(toks, dtype=torch.int32, device=self.device)
         CH = self.api_chunk if not cache.track_mass else max(1, min(self.api_chunk, MASS_ROWS // self.n_rep))
-        w = self.work(cache.batch, CH, cache.capacity_tokens, 0, cache)
+        w = self.work(1, CH, cache.capacity_tokens, 0, cache)
         for c0 in range(0, T, CH):
             c1 = min(T, c0 + CH)
             pos0 = torch.tensor([start_pos + c0], dtype=torch.int32, device=self.device)

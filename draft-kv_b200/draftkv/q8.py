@@ -28,6 +28,7 @@ BLOCK_SIZES = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128)
 _CODES = {} if torch is None else {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 MASS_ROWS = 64          # query rows a KV head up to which attention can add up the mass
+WORK_ZERO_BYTES = 65536  # bytes at the start of an attention's scratch that are zero between calls
 
 
 def tile_bytes(d_head: int):
@@ -59,6 +60,8 @@ class Q8KVCache(PagedKVCache):
         super().__init__(n_layers, n_heads, d_head, block_size=block_size, n_blocks=n_blocks, dtype=np.float32,
                          batch=batch, max_blocks_per_seq=max_blocks_per_seq, device=device)
         self.next_pos = [0] * batch          # position of the next token (entries + evicted)
+        # per sequence and layer: entries from here on are the last positions of every head
+        self._floor = [[0] * n_layers for _ in range(batch)]
 
     @staticmethod
     def _check_shape(d_head: int, block_size: int) -> None:
@@ -142,17 +145,25 @@ class Q8KVCache(PagedKVCache):
         return self.codes.numel() + self.scale.numel() * 4
 
     def _workspace(self, T: int, group: int, split_keys: int, note_mass: bool, stream: int):
-        """The attention scratch of a call shape: zero when made, left ready by
-        each call, one per stream (calls on one stream run in order).  Inside a
-        stream capture a fresh one, cleared by the graph itself, belongs to the
-        graph."""
+        """The attention scratch of a call: one buffer per stream (calls on one
+        stream run in order), grown to the largest call; its tickets are zero
+        when made and left so by each call.  A call that is being captured gets
+        one of its own, cleared by the graph itself: graphs may be replayed side
+        by side."""
+        capturing = torch.cuda.is_current_stream_capturing()
         key = (T, group, split_keys, note_mass, stream)
-        w = self._work.get(key)
+        w = None if capturing else self._work.get(key)
         if w is None:
-            n = int(_lib.load().dkv_q8_attn_work_bytes(self._dims, group, T, self.capacity_tokens, split_keys,
-                                                       1 if note_mass else 0))
-            w = torch.zeros(max(n, 16), dtype=torch.uint8, device=self.device)
-            if not torch.cuda.is_current_stream_capturing():
+            n = max(int(_lib.load().dkv_q8_attn_work_bytes(self._dims, group, T, self.capacity_tokens, split_keys,
+                                                           1 if note_mass else 0)), WORK_ZERO_BYTES)
+            if not capturing:
+                w = next((t for k, t in self._work.items() if k[4] == stream), None)
+            if w is None or w.numel() < n:
+                w = torch.empty(n, dtype=torch.uint8, device=self.device)
+                w[:WORK_ZERO_BYTES].zero_()
+                if not capturing:        # (the smaller one goes)
+                    self._work = {k: t for k, t in self._work.items() if k[4] != stream}
+            if not capturing:
                 self._work[key] = w
         return w
 
@@ -210,9 +221,9 @@ class Q8KVCache(PagedKVCache):
         left as they were (zeros when `out` is made here).  mass (T * n_heads /
         n_kv <= 64): every seen entry's softmax weights are added to it.  A row
         of up to 64 equals the one-token call at that entry bit for bit.  `work`:
-        scratch of `dkv_q8_attn_work_bytes` (zero when first used) for a caller
-        that runs or replays calls side by side; by default the cache keeps one
-        per stream and call shape."""
+        uint8 scratch of `dkv_q8_attn_work_bytes`, the first 64 KB zero when
+        first used, for a caller that keeps its own; by default the cache has one
+        per stream, and a captured call one of its own."""
         stream, shape, kv = self._stream(), q.shape, self.n_heads
         if len(shape) != 4 or shape[0] != self.batch or shape[3] != self.d_head or shape[2] % kv or not shape[2]:
             raise ValueError(f"q must be [{self.batch}, T, a multiple of {kv} heads, {self.d_head}], got {tuple(shape)}")
@@ -236,6 +247,8 @@ class Q8KVCache(PagedKVCache):
             return out
         if work is None:
             work = self._workspace(T, group, split_keys, mass is not None, stream)
+        elif work.dtype is not torch.uint8 or work.device != self.device or not work.is_contiguous():
+            raise ValueError(f"work must be a contiguous uint8 tensor on {self.device}")
         _lib.call("dkv_q8_attn", self.struct(), self._dims, layer, group, T, q.data_ptr(), entry0.data_ptr(),
                   _lib.ptr(n_rows), out.data_ptr(), code, split_keys, _lib.ptr(mass), work.data_ptr(), work.numel(), stream)
         return out
@@ -339,9 +352,22 @@ class Q8KVCache(PagedKVCache):
         pos = self.positions(layer, b)
         return o[:, :, 0], o[:, :, 1], pos[0] if (pos == pos[:1]).all() else pos
 
+    @property
+    def pos(self):
+        """Positions of sequence 0's entries per layer, as `read` gives them."""
+        each = (self.positions(L) for L in range(self.n_layers))
+        return [(p[0] if (p == p[:1]).all() else p).tolist() for p in each]
+
     def truncate_seq(self, b: int, n_pos: int) -> None:
         """Rollback to n_pos entries (paged.py:144-162); the scale of a partly
-        emptied block stays until the block is written from its start again."""
+        emptied block stays until the block is written from its start again.
+        After an eviction a sequence can go back through its recent entries (or
+        to none): before them the heads hold different positions."""
+        floor = max(self._floor[b])
+        if 0 < n_pos < floor:
+            raise ValueError(f"entries before {floor} of sequence {b} hold other positions in each head")
+        if n_pos <= 0:
+            self._floor[b] = [0] * self.n_layers
         before = self.counts[b][0]
         super().truncate_seq(b, n_pos)
         left = self.counts[b][0]
@@ -362,15 +388,22 @@ class Q8KVCache(PagedKVCache):
         if budget < 1 or sink < 0 or recent < 0:
             raise ValueError("evict: budget >= 1, sink >= 0, recent >= 0")
         keep_to = max(budget, sink + recent)
-        out = {}
-        for L in range(self.n_layers) if layers is None else layers:
+        self._stream()
+        plan, free = [], self.pool.n_free
+        for L in dict.fromkeys(range(self.n_layers) if layers is None else layers):
+            if not 0 <= L < self.n_layers:
+                raise ValueError(f"evict: layer {L} of {self.n_layers}")
             n = [self.counts[b][L] for b in range(self.batch)]
             if max(n) <= keep_to:
                 continue
             m = [min(x, keep_to) for x in n]
             pages = [-(-x // self.block_size) for x in m]
-            if sum(pages) > self.pool.n_free:
-                raise BlockPoolExhausted(f"eviction needs {sum(pages)} free blocks, {self.pool.n_free} left")
+            if sum(pages) > free:
+                raise BlockPoolExhausted(f"eviction needs {sum(pages)} free blocks, {free} left")
+            free += sum(len(self.block_tables[b][L]) for b in range(self.batch)) - sum(pages)
+            plan.append((L, n, m, pages))
+        out = {}
+        for L, n, m, pages in plan:
             new = [self.pool.allocate_many(p) for p in pages]
             out_pages = max(max(pages), 1)
             table = torch.full((self.batch, out_pages), -1, dtype=torch.int32)
@@ -388,5 +421,7 @@ class Q8KVCache(PagedKVCache):
                 self.block_tables[b][L] = list(ids)
                 self.table_host[b, L, :len(ids)] = table[b, :len(ids)]
                 self.counts[b][L] = m[b]
+                if n[b] > m[b]:
+                    self._floor[b][L] = max(self._floor[b][L] - (n[b] - m[b]), m[b] - recent)
             self._dirty = True
         return out

@@ -245,6 +245,10 @@ DKV_API size_t dkv_attn_work_bytes(dkv_dims dims, int group, int T, int max_ctx,
  *   K: token g + 8 (w & 1), dims 32j + 16 (w >> 1) + {2t, 2t+1, 2t+8, 2t+9};
  *   V: dim 32j + 16 (w >> 1) + 8 (w & 1) + g, tokens {2t, 2t+1, 2t+8, 2t+9}.
  *
+ * Codes are finite (0x7f and 0xff are never written), scales powers of two.  A
+ * page may stand in several rows of the table to be read; a call that writes it
+ * writes it through one.
+ *
  * A page id outside [0, n_pages) in the table is never followed: nothing is
  * written there, its entries are not seen, and 0x400 is recorded in the device
  * error word, as for entries outside the capacity. */
@@ -287,8 +291,10 @@ DKV_API int dkv_q8_read(const dkv_q8_cache* cache, dkv_dims dims, int b, int lay
  * Up to 64 query rows (T * group) a row's result does not depend on T or on
  * the other rows, bit for bit.  split_keys: keys per split, a multiple of 128,
  * or 0 for a rule on (batch, n_kv, capacity).
- * The work buffer must be zero when first used, is left ready for the next
- * call, and must not serve two calls that may run at the same time (two
+ * batch * n_kv * ceil(T * group / rows of a block: 8, 16 or, above 64, 256) is
+ * at most 16384 where the keys are split (capacity beyond a split).
+ * The first 64 KB of the work buffer must be zero when first used and are left
+ * so; any call may use it, but no two that may run at the same time (two
  * streams, two captured graphs replayed side by side). */
 DKV_API size_t dkv_q8_attn_work_bytes(dkv_dims dims, int group, int T, int capacity, int split_keys, int note_mass);
 DKV_API int dkv_q8_attn(const dkv_q8_cache* cache, dkv_dims dims, int layer, int group, int T, const float* d_q,
@@ -299,8 +305,8 @@ DKV_API int dkv_q8_attn(const dkv_q8_cache* cache, dkv_dims dims, int layer, int
  * n[b] entries of `layer`, min(n, max(budget[b], sink + recent)) stay -- the
  * first `sink`, the last `recent`, and of the others those left after the
  * lowest (mass, index) are dropped.  The kept entries, in order, are written to
- * the pages of out_table [batch][out_pages] (pages that no table row of this
- * call's cache uses) as an append of their values to empty pages would;
+ * the pages of out_table [batch][out_pages] (each once, and none that a table row
+ * of this call's cache uses) as an append of their values to empty pages would;
  * out_pages * page_size must hold them (else fewer stay and 0x400 is recorded).
  * kept [batch][n_kv][out_pages * page_size]: their entry indices, -1 behind.
  * mass_out, pos_out [batch][n_kv][capacity]: mass and pos of the kept entries,

@@ -712,3 +712,171 @@ def test_class_refuses_wrong_tensors():
         c.evict_rows(0, e0, e0, i32([0, 1]), m)
     with pytest.raises(ValueError):
         c.evict_rows(0, e0, e0, i32([[0], [1]]), None)
+
+
+def test_captured_calls_have_scratch_of_their_own():
+    """Two graphs captured on one stream that has run the call before (so that the
+    cache holds scratch for it) are replayed side by side; one eviction inside."""
+    mk = Made(1, 1, 2, 128, 16, 130, seed=7, spare=8)
+    rng = np.random.default_rng(1)
+    mk.fill([2000], rng)
+    e0, n, m, mass = i32([1997]), i32([2000]), i32([64]), torch.rand((1, 2, mk.cap), device="cuda")
+    used = set(mk.table_np.reshape(-1).tolist())
+    table = i32([[p for p in range(mk.codes.shape[0]) if p not in used][:4]])
+    s, side = torch.cuda.Stream(), torch.cuda.Stream()
+    qs = [torch.randn((1, 3, 8, 128), device="cuda") for _ in range(2)]
+    outs = [torch.empty((1, 3, 8, 128), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        want = [mk.cache.attention(0, q, e0) for q in qs]
+        gone = mk.cache.evict_rows(0, n, m, table, mass, None, 2, 16)
+        eager = mk.cache._workspace(3, 4, 0, False, s.cuda_stream)
+    torch.cuda.synchronize()
+    graphs, kept = [], None
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            assert mk.cache._workspace(3, 4, 0, False, s.cuda_stream).data_ptr() != eager.data_ptr()
+            for _ in range(4):
+                mk.cache.attention(0, qs[i], e0, out=outs[i])
+            if i == 0:
+                kept = mk.cache.evict_rows(0, n, m, table, mass, None, 2, 16)
+        graphs.append(g)
+    for _ in range(10):
+        for g, st in zip(graphs, (s, side)):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    assert mk.cache._workspace(3, 4, 0, False, s.cuda_stream) is eager
+    assert all(torch.equal(o, w) for o, w in zip(outs, want))
+    assert torch.equal(kept[0], gone[0]) and torch.equal(kept[1], gone[1])
+
+
+def test_one_scratch_serves_calls_of_any_size():
+    """Decode, verify, mass and prompt calls of one stream in turn, each over what the others left."""
+    mk = Made(1, 1, 2, 64, 16, 1280, seed=3)
+    rng = np.random.default_rng(2)
+    mk.fill([20000], rng, spread=0.5)
+    mass = torch.zeros((1, 2, mk.cap), device="cuda")
+    calls = [(1, False, 0), (40, False, 0), (6, True, 0), (200, False, 0), (8, True, 256), (1, False, 512), (30, True, 0)]
+    q = [torch.randn((1, T, 4, 64), device="cuda") for T, _, _ in calls]
+
+    def run(i, **kw):
+        T, noted, split = calls[i]
+        return mk.cache.attention(0, q[i], i32([20000 - T]), mass=mass if noted else None, split_keys=split, **kw)
+
+    want = []
+    for i, (T, noted, split) in enumerate(calls):      # scratch of its own, cleared as the header asks
+        nb = lib().load().dkv_q8_attn_work_bytes(mk.cache._dims, 2, T, mk.cap, split, int(noted))
+        w = torch.full((nb,), 0xA5, dtype=torch.uint8, device="cuda")
+        w[:65536] = 0
+        want.append(run(i, work=w))
+        assert (w[:65536] == 0).all()
+    for order in (range(len(calls)), reversed(range(len(calls)))):
+        for i in order:
+            assert torch.equal(run(i), want[i]), calls[i]
+    assert len({w.data_ptr() for w in mk.cache._work.values()}) == 1
+
+
+def test_prompt_values_near_the_smallest_scale():
+    """Thousands of entries whose scores stay just below the growth that raises the
+    max, over V at the smallest scale: 2^-120 over the sum (2^26) is far below fp32's
+    normal numbers, the outputs (2^-115) are not."""
+    d, n, T = 64, 8192, 70
+    mk = Made(1, 1, 1, d, 16, n // 16, seed=5)
+    rng = np.random.default_rng(4)
+    k = np.zeros((1, n, 1, d), np.float32)
+    k[:, 128:] = 7.5 * np.log(2) * np.sqrt(d) / d
+    v = np.ldexp(1 + rng.random((1, n, 1, d)), -115).astype(np.float32)
+    r = mk.reference()
+    mk.cache.write(0, torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda(), i32([0]))
+    r.append(0, k, v, [0], [n])
+    kk, vv = r.entries(0, 0, 0, n)
+    assert 7 < (kk[-1].sum() / np.sqrt(d)) / np.log(2) < 8
+    q = np.ones((1, T, 1, d), np.float32)
+    out = mk.cache.attention(0, torch.from_numpy(q).cuda(), i32([n - T]), out_dtype=torch.float32).double().cpu().numpy()
+    want, _, bound = r.attention(0, q, [n - T])
+    # 2^-115 <= v <= 2^-114 (rounded to e4m3 too), so an error of delta x the largest v is 2 delta of the output
+    delta = ref.prompt_tolerance(d, n, bound, 1.0, 0.0)[1]
+    assert (np.abs(out - want) <= 2 * delta * want).all()
+
+
+def test_more_rows_than_tickets_where_the_keys_are_not_split():
+    mk = Made(600, 1, 32, 64, 16, 1, seed=8)
+    rng = np.random.default_rng(3)
+    mk.fill([int(x) for x in rng.integers(1, 17, 600)], rng)
+    q = torch.randn((600, 1, 32, 64), device="cuda")
+    e0 = torch.from_numpy(rng.integers(0, 16, 600).astype(np.int32)).cuda()
+    from draftkv import Q8KVCache
+    out = torch.zeros((600, 1, 32, 64), dtype=torch.bfloat16, device="cuda")
+    n = torch.from_numpy(np.random.default_rng(3).integers(1, 17, 600).astype(np.int32)).cuda()
+    e0 = torch.minimum(e0, n - 1)
+    mk.cache.attention(0, q, e0, out=out)
+    for a in (0, 300):
+        half = Q8KVCache.from_storage(mk.codes, mk.scale, mk.table[a:a + 300].contiguous())
+        assert torch.equal(half.attention(0, q[a:a + 300], e0[a:a + 300]), out[a:a + 300])
+
+
+def test_extreme_entries_and_split_lengths():
+    mk = Made(1, 1, 1, 64, 16, 6, seed=6)
+    mk.fill([96], np.random.default_rng(0))
+    for T in (1, 4, 80):
+        q = torch.randn((1, T, 2, 64), device="cuda")
+        last = mk.cache.attention(0, q, i32([96]))              # every token sees all 96
+        assert device_error() == 0x400
+        for e0 in (97, 2 ** 30, 2 ** 31 - 1):
+            assert torch.equal(mk.cache.attention(0, q, i32([e0])), last)
+            assert device_error() == 0x400
+        assert (mk.cache.attention(0, q, i32([-2 ** 31])) == 0).all()
+        whole = mk.cache.attention(0, q, i32([96 - T]))
+        for split in (128, 2 ** 31 - 128):
+            assert torch.equal(mk.cache.attention(0, q, i32([96 - T]), split_keys=split), whole)
+
+
+def test_evict_plans_all_layers_first():
+    """Too few free blocks, a layer named twice, a layer that is not there, and how
+    far back a sequence can go after an eviction."""
+    from draftkv import BlockPoolExhausted, Q8KVCache
+    c = Q8KVCache(2, 1, 64, block_size=16, n_blocks=10, max_blocks_per_seq=8, track_mass=True)
+    x = np.random.default_rng(0).standard_normal((80, 1, 64)).astype(np.float32)
+    c.append(0, x[:17], x[:17], np.arange(17))
+    c.append(1, x, x, np.arange(80))
+    for m in c.mass:
+        m.copy_(torch.rand_like(m))
+
+    def state():
+        return [c.counts, c.block_tables, c.pool.n_free, c._floor]
+
+    import copy
+    before = copy.deepcopy(state())
+    with pytest.raises(BlockPoolExhausted):        # 4 blocks for layer 1, 3 are free
+        c.evict(64, sink=0, recent=0)
+    with pytest.raises(ValueError):
+        c.evict(8, sink=0, recent=4, layers=[1, -1])
+    with pytest.raises(ValueError):
+        c.evict(8, sink=0, recent=4, layers=[2])
+    assert state() == before
+    c.pool.check_invariants()
+    out = c.evict(8, sink=0, recent=4, layers=[0, 0, 1])
+    assert set(out) == {0, 1} and c.counts == [[8, 8]]
+    c.pool.check_invariants()
+    assert all(p[-4:] == list(range(n - 4, n)) for p, n in zip(c.pos, (17, 80)))
+    c.next_pos[0] = 80
+    with pytest.raises(ValueError):
+        c.truncate(3)
+    c.truncate(5)
+    assert c.length == 5 and c.next_pos == [77]
+    c.truncate(0)
+    assert c.length == 0 and c.next_pos == [0] and c.blocks_in_use == 0
+    c.append(0, x[:3], x[:3], np.arange(3))
+    c.truncate(1)
+
+
+def test_class_refuses_foreign_scratch():
+    mk = Made(1, 1, 1, 64, 16, 4)
+    mk.fill([3], np.random.default_rng(0))
+    q, e0 = torch.zeros((1, 1, 1, 64), device="cuda"), i32([2])
+    for w in (torch.zeros(1 << 20, device="cuda"), torch.zeros(1 << 20, dtype=torch.uint8),
+              torch.zeros(1 << 20, dtype=torch.uint8, device="cuda")[::2]):
+        with pytest.raises(ValueError):
+            mk.cache.attention(0, q, e0, work=w)
