@@ -15,14 +15,21 @@
 // arithmetic gives; probabilities are two f16 numbers for fp32 outputs, one
 // for bf16 outputs; max, sum and O are fp32.
 //
-// One CTA per (key split, KV head, sequence x row block), two an SM.  Its 8
-// warps are on their own until the end: warp w takes units w, w + 8, ... of the
-// split (a unit is 4 KB: the K and V of 16 tokens at d = 128, of 32 at d = 64),
-// lane 0 fetches them with bulk copies into a ring of its warp's, and each warp
-// keeps (max, sum, O), merged in a fixed order.  Split and unit boundaries are
-// absolute key positions and a row's arithmetic does not depend on the other
-// rows of the call, so a verify row equals the decode step at that entry bit
-// for bit.
+// One CTA per (key split, KV head, sequence x row block), two an SM.  A unit is
+// 4 KB: the K and V of 16 tokens at d = 128, of 32 at d = 64; 8 units, one a
+// warp, are a round, and the splits take the rounds in turns, so that a sequence
+// far shorter than the capacity still reaches all its CTAs (4 x 8 heads, 8192
+// entries of 32768: 39 us with a run of keys a split, 21 us in turns; a full one
+// is the same).  A CTA's warps are on their own until the end: lane 0 fetches
+// the warp's units with bulk copies into a ring, and each warp keeps (max, sum,
+// O), merged in a fixed order.  Which split, warp and tile an entry goes to is
+// fixed by its index alone and a row's arithmetic does not depend on the other
+// rows of the call, so a verify row equals the decode step at that entry bit for
+// bit.
+// Measured (d 128, group 4, bf16): a fixed 11 us (launch, first bytes, two
+// merges) and then 6.9 TB/s; a warp needs about 1900 cycles a unit, so one CTA
+// alone streams 27 GB/s, which bounds ragged batches.  6 warps with units of
+// 8 KB (half the overhead a byte) were slower: 262144 entries 95 for 90 us.
 //
 // The running max is raised lazily: only when a score exceeds it by more than
 // 8 (log2 units), which keeps the common tile free of shuffles and rescaling;
@@ -106,13 +113,13 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
     const int b = blockIdx.z / a.n_rb, rb = blockIdx.z % a.n_rb;
     const int G = a.group, R_all = a.T * G;
     const int rbase = rb * RB, R = min(RB, R_all - rbase);
-    const int k0 = s * a.split;
     const int32_t* tab = v.row(b);
-    auto key_of = [&](int u) { return k0 + (u * kQdKG + warp) * UT; };
+    // first key of this warp's unit u: round u * n_splits + s of the sequence
+    auto key_of = [&](int u) { return ((u * a.n_splits + s) * kQdKG + warp) * UT; };
     // page id of tile `lane` of the batch that starts at this warp's unit u0 (-1 beyond the table)
     auto load_pid = [&](int u0) {
-        const int pg = (key_of(u0 + lane / TPU) + (lane % TPU) * 16) >> v.page_shift;
-        return pg < v.max_pages ? q8_ld(tab + pg) : -1;
+        const long long key = (((long long)(u0 + lane / TPU) * a.n_splits + s) * kQdKG + warp) * UT + (lane % TPU) * 16;
+        return key < v.capacity() ? q8_ld(tab + (key >> v.page_shift)) : -1;
     };
     const int first_pid = load_pid(0);
     const int qr = lane >> 2, qc = lane & 3;
@@ -132,15 +139,14 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
     // the block's last token decides what is read
     const int t_last = min((rbase + R - 1) / G, n_tok - 1);
     const int n_keys = t_last >= rbase / G ? max(0, min(a.n_keys(b), e0 + t_last + 1)) : 0;
-    const int kend = min(n_keys, k0 + a.split);
     if (s == 0 && h == 0 && rb == 0 && threadIdx.x == 0 && a.beyond(b)) atomicOr(a.err, kErrQ8Page);
-    const int n_units = kend > k0 ? (kend - k0 + UT - 1) / UT : 0;
-    const int mine = n_units > warp ? (n_units - warp + kQdKG - 1) / kQdKG : 0;      // this warp's units
+    const int before = (n_keys + UT - 1) / UT - (s * kQdKG + warp), every = a.n_splits * kQdKG;
+    const int mine = before > 0 ? (before + every - 1) / every : 0;      // this warp's units
 
     // -1 for tiles past the end and for bad ids (recorded; their keys are not seen)
     auto check_pid = [&](int u0, int pid) {
         const int u = u0 + lane / TPU;
-        if (u >= mine || key_of(u) + (lane % TPU) * 16 >= kend) return -1;
+        if (u >= mine || key_of(u) + (lane % TPU) * 16 >= n_keys) return -1;
         if (v.ok(pid)) return pid;
         atomicOr(a.err, kErrQ8Page);
         return -1;
@@ -261,7 +267,7 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
     }
     float* sc_base = a.scores ? a.scores + (((size_t)b * v.n_kv + h) * v.capacity()) * a.s_ld : nullptr;
     // entries up to here are seen by every row of the block that is there
-    const int all_see = min(e0 + rbase / G, kend - 1);
+    const int all_see = min(e0 + rbase / G, n_keys - 1);
 
     // ---- S^T of a unit, not yet scaled: keys qr (+8), columns 2qc, 2qc + 1 of
     // each row tile.  Two chains of products (the halves of each 32-dim block)
@@ -385,10 +391,10 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
                 for (int nt = 0; nt < NT; ++nt) {
                     const int r = rbase + nt * 8 + 2 * qc, ka = key0 + tt * 16 + qr;
                     if (r < a.s_ld && (!PAIR || qc < 2)) {
-                        if (ka < kend)
+                        if (ka < n_keys)
                             *reinterpret_cast<float2*>(sc_base + (size_t)ka * a.s_ld + r) =
                                 make_float2(sh[tt][nt][0], sh[tt][nt][1]);
-                        if (ka + 8 < kend)
+                        if (ka + 8 < n_keys)
                             *reinterpret_cast<float2*>(sc_base + (size_t)(ka + 8) * a.s_ld + r) =
                                 make_float2(sh[tt][nt][2], sh[tt][nt][3]);
                     }
@@ -464,7 +470,7 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
             if (!whole) {
                 // bytes of keys that are not there (past the end, bad page) as zeros:
                 // their probability is 0, but 0 x NaN would not be
-                const int ke = ks[tt] < 0.f ? 0 : kend - key0 - tt * 16;
+                const int ke = ks[tt] < 0.f ? 0 : n_keys - key0 - tt * 16;
                 const uint32_t vm = (2 * qc < ke ? 0xffu : 0u) | (2 * qc + 1 < ke ? 0xff00u : 0u) |
                                     (2 * qc + 8 < ke ? 0xff0000u : 0u) | (2 * qc + 9 < ke ? 0xff000000u : 0u);
 #pragma unroll
@@ -632,26 +638,18 @@ cudaError_t launch_decode_rows(const Q8AttnArgs& a, int R, dim3 grid, cudaStream
 // Query rows a CTA: 8 or 16.
 int row_block(int R) { return R <= 8 ? 8 : 16; }
 
-// Keys per split (a multiple of 256: whole units of all 8 warps) where the
-// caller names none: one wave of two CTAs an SM over (sequence, head, split),
-// and at least 128 KB of codes a split: a CTA costs some microseconds apart
-// from its stream (one sequence of 262144 entries, 8 heads: 37 splits a head
-// 90 us, 256 splits a third longer), and in a capacity far above the length the
-// smaller splits leave the sequence more CTAs.  It depends on the batch, the
-// heads and the capacity only, so a sequence's verify and decode calls share it.
-int default_split(int batch, int n_kv, int d, int capacity) {
-    const int ctas = std::max(1, 2 * 148 / std::max(1, batch * n_kv));
-    const int keys = (int)(((long long)capacity + ctas - 1) / ctas);
-    return std::max((keys + 255) / 256 * 256, kQdMinBytes / (2 * d));
+// Splits of the key axis.  Where the caller names no length: one wave of two
+// CTAs an SM over (sequence, head, split), and at least 128 KB of codes a split
+// when the capacity is full.  They depend on the batch, the heads and the
+// capacity only, so a sequence's verify and decode calls share them.
+int split_count(dkv_dims dims, int capacity, int split_keys) {
+    if (split_keys > 0) return (int)(((long long)capacity + split_keys - 1) / split_keys);
+    const int ctas = std::max(1, 2 * 148 / std::max(1, dims.batch * dims.n_kv));
+    return (int)std::max(1ll, std::min<long long>(ctas, (long long)capacity * 2 * dims.d / kQdMinBytes));
 }
 
-int pick_split(dkv_dims dims, int capacity, int split_keys) {
-    if (split_keys > 0) return std::min(split_keys, (capacity + 127) / 128 * 128);
-    return default_split(dims.batch, dims.n_kv, dims.d, capacity);
-}
-
-size_t decode_work(dkv_dims dims, int R, int capacity, int split, bool mass, Q8AttnArgs* a, Arena* ar) {
-    const int rb = row_block(R), n_rb = (R + rb - 1) / rb, ns = std::max(1, (capacity + split - 1) / split);
+size_t decode_work(dkv_dims dims, int R, int capacity, int split_keys, bool mass, Q8AttnArgs* a, Arena* ar) {
+    const int rb = row_block(R), n_rb = (R + rb - 1) / rb, ns = split_count(dims, capacity, split_keys);
     const size_t bh = (size_t)dims.batch * dims.n_kv;
     const size_t part = bh * n_rb * ns * rb * (dims.d + 4), s_ld = (size_t)(R + 1) / 2 * 2;
     if (a) {
@@ -687,8 +685,7 @@ extern "C" size_t dkv_q8_attn_work_bytes(dkv_dims dims, int group, int T, int ca
     const long long R = (long long)T * group;
     if (R > (1 << 24) || capacity > (1 << 30)) return 0;
     if (R > kQ8MaxRows) return attn_q8_prefill_work(dims, group, T, capacity);
-    return decode_work(dims, (int)R, capacity, pick_split(dims, capacity, split_keys), note_mass != 0,
-                       nullptr, nullptr);
+    return decode_work(dims, (int)R, capacity, split_keys, note_mass != 0, nullptr, nullptr);
 }
 
 extern "C" int dkv_q8_attn(const dkv_q8_cache* cache, dkv_dims dims, int layer, int group, int T, const float* q,
@@ -724,11 +721,10 @@ extern "C" int dkv_q8_attn(const dkv_q8_cache* cache, dkv_dims dims, int layer, 
                     "dkv_q8_attn: work buffer of %zu bytes is too small", work_bytes);
         return attn_q8_prefill(a, dims, work, work_bytes, st);
     }
-    a.split = pick_split(dims, cap, split_keys);
-    DKV_REQUIRE(work && work_bytes >= decode_work(dims, R, cap, a.split, mass != nullptr, nullptr, nullptr),
+    DKV_REQUIRE(work && work_bytes >= decode_work(dims, R, cap, split_keys, mass != nullptr, nullptr, nullptr),
                 "dkv_q8_attn: work buffer of %zu bytes is too small", work_bytes);
     Arena ar(work, work_bytes);
-    decode_work(dims, R, cap, a.split, mass != nullptr, &a, &ar);
+    decode_work(dims, R, cap, split_keys, mass != nullptr, &a, &ar);
     DKV_REQUIRE(a.tickets && a.part && (!mass || (a.scores && a.stats)), "dkv_q8_attn: work buffer");
     const size_t n_tk = (size_t)dims.batch * dims.n_kv * a.n_rb;
     DKV_REQUIRE((a.n_splits == 1 || n_tk <= kQ8Tickets) && (size_t)dims.batch * a.n_rb <= 65535,

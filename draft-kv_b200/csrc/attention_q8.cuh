@@ -17,7 +17,7 @@ struct Q8AttnArgs {
     const int32_t* n_rows;       // [batch] or null: tokens of the call a sequence has
     void* out;                   // [batch * T][n_kv * group * d]
     int out_dtype;
-    int split, n_splits, n_rb;   // keys per split, splits, row blocks per (sequence, head)
+    int split, n_splits, n_rb;   // keys per split (prompt chunks), splits, row blocks per (sequence, head)
     float scale;                 // log2 e / sqrt(d)
     float* part;                 // [batch][n_kv][n_rb][n_splits][rows a block][d + 4]: max, sum, -, -, O
     unsigned* tickets;           // [batch][n_kv][n_rb]

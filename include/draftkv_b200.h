@@ -289,8 +289,9 @@ DKV_API int dkv_q8_read(const dkv_q8_cache* cache, dkv_dims dims, int b, int lay
  * mass [batch][n_kv][capacity] (NULL: not wanted; T * group <= 64): adds to
  * every seen entry its softmax weights, summed over the call's rows.
  * Up to 64 query rows (T * group) a row's result does not depend on T or on
- * the other rows, bit for bit.  split_keys: keys per split, a multiple of 128,
- * or 0 for a rule on (batch, n_kv, capacity).
+ * the other rows, bit for bit.  split_keys (a multiple of 128): the keys go to
+ * ceil(capacity / split_keys) splits; 0: a rule on (batch, n_kv, capacity).
+ * Above 64 rows the splits are chosen by a rule.
  * batch * n_kv * ceil(T * group / rows of a block: 8, 16 or, above 64, 256) is
  * at most 16384 where the keys are split (capacity beyond a split).
  * The first 64 KB of the work buffer must be zero when first used and are left
