@@ -103,12 +103,14 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
 
     const Q8View& v = a.v;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // row block fastest: the row blocks of a (sequence, head, split) run
-    // together and read the same codes through L2
-    const int rb = (int)(blockIdx.x % a.n_rb);
-    const int s = (int)(blockIdx.x / a.n_rb % a.n_splits);
-    const int h = (int)(blockIdx.x / a.n_rb / a.n_splits % v.n_kv);
-    const int b = (int)(blockIdx.x / a.n_rb / a.n_splits / v.n_kv);
+    // a sequence's last row blocks, which see the most keys, start first, all
+    // heads together (a prompt of 4096 tokens, 8 KV heads, group 4: 298 us with
+    // the row blocks in order, head by head, 255 us so); sequence by sequence, for
+    // long and short ones side by side in the last wave
+    const int h = (int)(blockIdx.x % v.n_kv);
+    const int s = (int)(blockIdx.x / v.n_kv % a.n_splits);
+    const int rb = a.n_rb - 1 - (int)(blockIdx.x / v.n_kv / a.n_splits % a.n_rb);
+    const int b = (int)(blockIdx.x / v.n_kv / a.n_splits / a.n_rb);
     const int G = a.group;
     const int r0 = rb * kQpRows, R = min(kQpRows, a.T * G - r0);
     const size_t bhr = ((size_t)b * v.n_kv + h) * a.n_rb + rb;
