@@ -235,8 +235,8 @@ class Q8KVCache(PagedKVCache):
         self._check_mass(mass)
         T, group = shape[1], shape[2] // kv
         if out is None:
-            make = torch.empty if n_rows is None else torch.zeros
-            out = make(shape, dtype=out_dtype or torch.bfloat16, device=self.device)
+            make = torch.empty_like if n_rows is None else torch.zeros_like
+            out = make(q, dtype=out_dtype or torch.bfloat16)
         elif out.shape != shape or not out.is_contiguous() or out.device != self.device \
                 or (out_dtype is not None and out.dtype is not out_dtype):
             raise ValueError("out must be contiguous and shaped like q")
@@ -282,7 +282,7 @@ class Q8KVCache(PagedKVCache):
         elif pos_out is None:
             pos_out = torch.empty_like(pos)
         out_pages = out_table.shape[1]
-        kept = torch.empty((self.batch, self.n_heads, out_pages * self.block_size), dtype=torch.int32, device=self.device)
+        kept = out_table.new_empty((self.batch, self.n_heads, out_pages * self.block_size))
         _lib.call("dkv_q8_evict", self.struct(), self._dims, layer, n.data_ptr(), budget.data_ptr(), sink, recent,
                   mass.data_ptr(), _lib.ptr(pos), out_table.data_ptr(), out_pages, mass_out.data_ptr(), _lib.ptr(pos_out),
                   kept.data_ptr(), stream)

@@ -495,7 +495,8 @@ DKV_API int dkv_forward(const dkv_model* m, const dkv_full_cache* full, const dk
  * (RoPE, learned embeddings), st->max_ctx is not read.  mass, pos: host arrays of
  * n_layers device pointers ([batch][n_kv][capacity] each; NULL: not kept), as
  * dkv_q8_append and dkv_q8_attn take them; with mass T * group <= 64.
- * Logits NULL as in dkv_forward.  Heads of 64 or 128; f32 and bf16 models. */
+ * Logits NULL as in dkv_forward.  Heads of 64 or 128; f32 and bf16 models.
+ * Every sequence of the batch takes T tokens. */
 DKV_API size_t dkv_forward_q8_work_bytes(const dkv_model* m, int batch, int max_T, int capacity, int note_mass);
 DKV_API int dkv_forward_q8(const dkv_model* m, const dkv_q8_cache* cache, const dkv_step* st, const int32_t* d_entry0,
                            float* const* mass, int32_t* const* pos, void* stream);
