@@ -317,13 +317,16 @@ DKV_DEV unsigned block_scan(unsigned v, unsigned* wsum) {
 // memory, a part of the bins a CTA (every pass has a histogram of its own), and
 // every CTA finds the same bin.  Plain shared-memory atomics: grouping a warp's
 // equal bins first (match) took 200 cycles a warp, more than 32 atomics to one
-// address.  The counts below and at the key give each slice its place, and one
-// ordered pass over it (a warp a contiguous part) writes the kept indices,
-// masses and positions: order and result are fixed.
+// address.  The counts below and at the key give each slice its place, and an
+// ordered pass over it (a warp a contiguous part) writes the kept indices: order
+// and result are fixed.  Their masses and positions follow, spread over all
+// threads (loaded where the indices are made, 256 entries took a warp 6700
+// cycles).  One sequence of 262144 entries, 8 heads: 46 us before, 40 us so;
+// what is left are the cluster barriers and scans of three passes, 9 us of them.
 __global__ void __launch_bounds__(kSelThreads) q8_select_kernel(Q8EvictArgs a, int cluster, int smem_keys) {
     extern __shared__ __align__(16) unsigned sel_sm[];
     unsigned* keys_s = sel_sm + 3 * kSelBins;      // (histograms [3][kSelBins] first)
-    __shared__ unsigned part_s[kSelThreads], wsum[32], wbelow[32], wcnt[64], s_bin, s_below;
+    __shared__ unsigned part_s[kSelThreads], wsum[32], wbelow[32], wcnt[64], s_bin, s_below, s_from, s_upto;
     __shared__ __align__(8) uint2 counts;
     const uint32_t rank = cluster > 1 ? cluster_rank() : 0u;
     const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -347,8 +350,25 @@ __global__ void __launch_bounds__(kSelThreads) q8_select_kernel(Q8EvictArgs a, i
     // key of entry i, 0xffffffff for protected ones (which never go)
     auto key_of = [&](int i, float m) { return i >= f0 && i < f1 ? mass_key(m) : 0xffffffffu; };
     if (staged && drop > 0) {
-#pragma unroll 8
-        for (int i = i0 + tid; i < i1; i += kSelThreads) keys_s[i - i0] = key_of(i, q8_ld(mass + i));
+        constexpr int U = 16;                      // loads in flight a thread
+        for (int c0 = i0 + tid; c0 < i1; c0 += U * kSelThreads) {
+            float m[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) m[u] = c0 + u * kSelThreads < i1 ? q8_ld(mass + c0 + u * kSelThreads) : 0.f;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (c0 + u * kSelThreads < i1) keys_s[c0 + u * kSelThreads - i0] = key_of(c0 + u * kSelThreads, m[u]);
+        }
+    }
+    int32_t* kept = a.kept + row * out_cap;
+    {
+        // behind the kept entries (early: these stores drain while the keys are searched)
+        const int left = min(n - drop, out_cap), stride = kSelThreads * cluster;
+        for (int i = left + (int)rank * kSelThreads + tid; i < out_cap; i += stride) kept[i] = -1;
+        for (size_t i = left + (size_t)rank * kSelThreads + tid; i < cap; i += stride) {
+            a.mass_out[row * cap + i] = 0.f;
+            if (a.pos_out) a.pos_out[row * cap + i] = -1;
+        }
     }
     auto key_at = [&](int i) { return staged ? keys_s[i - i0] : key_of(i, q8_ld(mass + i)); };
     __syncthreads();
@@ -430,66 +450,82 @@ __global__ void __launch_bounds__(kSelThreads) q8_select_kernel(Q8EvictArgs a, i
         cluster_arrive_all();                      // (waited for at the end: shared memory outlives its readers)
     }
 
-    int32_t* kept = a.kept + row * out_cap;
     if (i0 < i1) {
-        // a warp a contiguous part of the slice: its equal and gone counts, then its place, then its entries
-        const int part = slice / 32, p0 = i0 + warp * part, p1 = min(p0 + part, i1);
-        unsigned my_eq = 0, my_lt = 0;
-        if (drop > 0)
+        // A warp a contiguous part of the slice, 32 groups of 32 entries at a time:
+        // lane g holds, as bits, which entries of group g lie below the key and at
+        // it; from the counts of both come the part's place, the groups' places and
+        // with them the kept indices
+        const int part = slice / 32, p0 = min(i0 + warp * part, i1), p1 = min(p0 + part, i1);
+        unsigned lt = 0, at = 0;
+        auto look = [&](int c0) {
+            lt = at = 0;
 #pragma unroll 8
-            for (int i = max(p0, f0) + lane; i < min(p1, f1); i += 32) {
-                const unsigned k = key_at(i);
-                my_eq += k == prefix;
-                my_lt += k < prefix;
+            for (int g = 0; g < 32; ++g) {
+                const int i = c0 + 32 * g + lane;
+                const bool open = drop > 0 && i < p1 && i >= f0 && i < f1;
+                const unsigned k = open ? key_at(i) : 0xffffffffu;
+                const unsigned l = __ballot_sync(0xffffffffu, open && k < prefix);
+                const unsigned e = __ballot_sync(0xffffffffu, open && k == prefix);
+                if (lane == g) lt = l, at = e;
             }
+        };
+        unsigned my_eq = 0, my_lt = 0;
+        for (int c0 = p0; c0 < p1; c0 += 1024) {
+            look(c0);
+            my_eq += __popc(at);
+            my_lt += __popc(lt);
+        }
         my_eq = (unsigned)warp_sum_i((int)my_eq);
         my_lt = (unsigned)warp_sum_i((int)my_lt);
         if (lane == 0) wcnt[warp] = my_eq, wcnt[32 + warp] = my_lt;
         __syncthreads();
         const unsigned we = wcnt[lane], wl = wcnt[32 + lane];
         const unsigned se = warp_scan(we) - we, sl = warp_scan(wl) - wl;
+        // equal entries before the part, and where its first kept entry goes
         unsigned eq = eq_before + __shfl_sync(0xffffffffu, se, warp);
-        unsigned gone = gone_before + __shfl_sync(0xffffffffu, sl, warp) + (min(eq, need) - min(eq_before, need));
-        constexpr int U = 8;                       // 32-entry groups whose loads are in flight together
-        for (int c0 = p0; c0 < p1; c0 += 32 * U) {
-            int32_t o[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int i = c0 + 32 * u + lane;
-                const bool in = i < p1, open = in && i >= f0 && i < f1 && drop > 0;
-                const unsigned k = open ? key_at(i) : 0xffffffffu;
-                const bool is_eq = open && k == prefix;
-                const unsigned beq = __ballot_sync(0xffffffffu, is_eq);
-                const bool goes = open && (k < prefix || (is_eq && eq + __popc(beq & ((1u << lane) - 1u)) < need));
-                const unsigned bg = __ballot_sync(0xffffffffu, goes);
-                o[u] = in && !goes ? i - (int)(gone + __popc(bg & ((1u << lane) - 1u))) : out_cap;
-                eq += __popc(beq);
-                gone += __popc(bg);
+        unsigned to = p0 - (gone_before + __shfl_sync(0xffffffffu, sl, warp) + (min(eq, need) - min(eq_before, need)));
+        if (tid == 0) s_from = to;
+        for (int c0 = p0; c0 < p1; c0 += 1024) {
+            if (part > 1024) look(c0);             // (else the masks are the ones just made)
+            const unsigned n_eq = __popc(at), eq_at = eq + warp_scan(n_eq) - n_eq;
+            const unsigned go = min(need - min(need, eq_at), n_eq);
+            unsigned gone = at;                    // of the equal ones the first `go` go
+            for (unsigned k = n_eq; k > go; --k) gone &= ~(0x80000000u >> __clz(gone));
+            const int there = min(max(p1 - (c0 + 32 * lane), 0), 32);
+            const unsigned stay = (there == 32 ? 0xffffffffu : (1u << there) - 1u) & ~(lt | gone), n_stay = __popc(stay);
+            const unsigned first = to + warp_scan(n_stay) - n_stay;
+#pragma unroll 8
+            for (int g = 0; g < 32; ++g) {
+                const unsigned m = __shfl_sync(0xffffffffu, stay, g);
+                const unsigned o = __shfl_sync(0xffffffffu, first, g) + __popc(m & ((1u << lane) - 1u));
+                if (((m >> lane) & 1u) && o < (unsigned)out_cap) kept[o] = c0 + 32 * g + lane;
             }
+            eq += (unsigned)warp_sum_i((int)n_eq);
+            to += (unsigned)warp_sum_i((int)n_stay);
+        }
+        if (tid == kSelThreads - 1) s_upto = to;
+        __syncthreads();                           // the slice's kept indices are written
+        constexpr int U = 4;
+        const int upto = min((int)s_upto, out_cap);
+        for (int o0 = (int)s_from + tid; o0 < upto; o0 += U * kSelThreads) {
+            int src[U];
             float m[U];
             int32_t p[U];
 #pragma unroll
+            for (int u = 0; u < U; ++u) src[u] = o0 + u * kSelThreads < upto ? q8_ld(kept + o0 + u * kSelThreads) : i0;
+#pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int i = c0 + 32 * u + lane;
-                const bool stays = o[u] < out_cap;
-                m[u] = stays ? q8_ld(mass + i) : 0.f;
-                p[u] = stays && a.pos_out ? q8_ld(a.pos + row * cap + i) : 0;
+                m[u] = q8_ld(mass + src[u]);
+                p[u] = a.pos_out ? q8_ld(a.pos + row * cap + src[u]) : 0;
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (o[u] >= out_cap) continue;
-                kept[o[u]] = c0 + 32 * u + lane;
-                a.mass_out[row * cap + o[u]] = m[u];
-                if (a.pos_out) a.pos_out[row * cap + o[u]] = p[u];
+                const int o = o0 + u * kSelThreads;
+                if (o >= upto) continue;
+                a.mass_out[row * cap + o] = m[u];
+                if (a.pos_out) a.pos_out[row * cap + o] = p[u];
             }
         }
-    }
-    // behind the kept entries, the cluster's threads together
-    const int left = min(n - drop, out_cap), stride = kSelThreads * cluster;
-    for (int i = left + (int)rank * kSelThreads + tid; i < out_cap; i += stride) kept[i] = -1;
-    for (size_t i = left + (size_t)rank * kSelThreads + tid; i < cap; i += stride) {
-        a.mass_out[row * cap + i] = 0.f;
-        if (a.pos_out) a.pos_out[row * cap + i] = -1;
     }
     if (cluster > 1) cluster_wait_all();
 }
