@@ -59,16 +59,85 @@ DKV_DEV void q8_store2(const Q8AttnArgs& a, int b, int h, int gr, int n_tok, int
     else
         *reinterpret_cast<__nv_bfloat162*>(reinterpret_cast<uint16_t*>(a.out) + at) = __floats2bfloat162_rn(x0, x1);
 }
+// Rows r = i / (D / E), E elements from E (i % (D / E)) on, for items i = i0 + u *
+// stride (u < U): online over the splits in order, Q of them at a time, the loads
+// of all U items of a step in flight together.
+template <int D, int RB, int E, int U, int Q>
+DKV_DEV void q8_merge_items(const Q8AttnArgs& a, const float* parts, int b, int h, int rbase, int R, int n_tok, int i0,
+                            int stride) {
+    constexpr int PS = D + 4;
+    float M[U], L[U], x[U][E];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        M[u] = -INFINITY, L[u] = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[u][e] = 0.f;
+    }
+    for (int q0 = 0; q0 < a.n_splits; q0 += Q) {
+        float2 ml[U][Q];
+        float y[U][Q][E];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int k = 0; k < Q; ++k) {
+                const int i = i0 + u * stride;
+                ml[u][k] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+                for (int e = 0; e < E; ++e) y[u][k][e] = 0.f;
+                if (i < R * (D / E) && q0 + k < a.n_splits) {
+                    const float* at = parts + ((size_t)(q0 + k) * RB + i / (D / E)) * PS;
+                    ml[u][k] = __ldcg(reinterpret_cast<const float2*>(at));
+#pragma unroll
+                    for (int e = 0; e < E; e += 2) {
+                        const float2 t = __ldcg(reinterpret_cast<const float2*>(at + 4 + i % (D / E) * E + e));
+                        y[u][k][e] = t.x, y[u][k][e + 1] = t.y;
+                    }
+                }
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float m = M[u];
+#pragma unroll
+            for (int k = 0; k < Q; ++k) m = fmaxf(m, ml[u][k].x);
+            if (m == -INFINITY) continue;
+            const float al = M[u] == -INFINITY ? 0.f : q8_ex2(M[u] - m);
+            M[u] = m;
+            L[u] *= al;
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[u][e] *= al;
+#pragma unroll
+            for (int k = 0; k < Q; ++k) {
+                if (ml[u][k].x == -INFINITY) continue;     // (its O was never written)
+                const float w = q8_ex2(ml[u][k].x - m);
+                L[u] += ml[u][k].y * w;
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[u][e] += y[u][k][e] * w;
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * stride, r = i / (D / E), at = i % (D / E) * E;
+        if (i >= R * (D / E)) continue;
+        const bool none = L[u] == 0.f;
+#pragma unroll
+        for (int e = 0; e < E; e += 2)
+            q8_store2<D>(a, b, h, rbase + r, n_tok, at + e, none ? 0.f : x[u][e] / L[u], none ? 0.f : x[u][e + 1] / L[u]);
+        if (at == 0 && a.stats)
+            a.stats[((size_t)b * a.v.n_kv + h) * (a.T * a.group) + rbase + r] =
+                make_float2(M[u], none || (rbase + r) / a.group >= n_tok ? 0.f : 1.f / L[u]);
+    }
+}
 
 // After a CTA has stored its split's partial rows (max in log2 units, sum,
 // unnormalised O; an empty split has max -infinity and no O) of row block
 // `bhr`, the last CTA to arrive merges all splits and writes the outputs (and
-// the rows' stats).  A thread merges an element pair on its own, online in
-// split order with kMergeQ splits' loads in flight: no barrier, one round of
-// loads up to kMergeQ splits.
+// the rows' stats).  A thread merges an element pair on its own, 16 loads of
+// partials in flight: several splits of one item, or with few splits several
+// items.
 template <int D, int RB>
 DKV_DEV void q8_merge_splits(const Q8AttnArgs& a, size_t bhr, int b, int h, int rbase, int R, int n_tok) {
-    constexpr int PS = D + 4, kMergeQ = 16;
+    constexpr int PS = D + 4;
     __shared__ int is_last;
     __syncthreads();                     // the CTA's partials are stored
     if (threadIdx.x == 0) {
@@ -82,45 +151,12 @@ DKV_DEV void q8_merge_splits(const Q8AttnArgs& a, size_t bhr, int b, int h, int 
     }
     __syncthreads();
     if (!is_last) return;
-    const int ns = a.n_splits;
-    const float* parts = a.part + bhr * ns * (size_t)RB * PS;
-    for (int i = threadIdx.x; i < R * (D / 2); i += blockDim.x) {
-        const int r = i / (D / 2), e = i % (D / 2) * 2;
-        float M = -INFINITY, L = 0.f, x0 = 0.f, x1 = 0.f;
-        for (int q0 = 0; q0 < ns; q0 += kMergeQ) {
-            float2 ml[kMergeQ], y[kMergeQ];
-#pragma unroll
-            for (int k = 0; k < kMergeQ; ++k) {
-                ml[k] = make_float2(-INFINITY, 0.f);
-                y[k] = make_float2(0.f, 0.f);
-                if (q0 + k < ns) {
-                    const float* at = parts + ((size_t)(q0 + k) * RB + r) * PS;
-                    ml[k] = __ldcg(reinterpret_cast<const float2*>(at));
-                    y[k] = __ldcg(reinterpret_cast<const float2*>(at + 4 + e));
-                }
-            }
-            float m = M;
-#pragma unroll
-            for (int k = 0; k < kMergeQ; ++k) m = fmaxf(m, ml[k].x);
-            if (m == -INFINITY) continue;
-            const float al = M == -INFINITY ? 0.f : q8_ex2(M - m);
-            M = m;
-            L *= al;
-            x0 *= al;
-            x1 *= al;
-#pragma unroll
-            for (int k = 0; k < kMergeQ; ++k) {
-                if (ml[k].x == -INFINITY) continue;        // (its O was never written)
-                const float w = q8_ex2(ml[k].x - m);
-                L += ml[k].y * w;
-                x0 += y[k].x * w;
-                x1 += y[k].y * w;
-            }
-        }
-        q8_store2<D>(a, b, h, rbase + r, n_tok, e, L == 0.f ? 0.f : x0 / L, L == 0.f ? 0.f : x1 / L);
-        if (e == 0 && a.stats)
-            a.stats[((size_t)b * a.v.n_kv + h) * (a.T * a.group) + rbase + r] =
-                make_float2(M, L == 0.f || (rbase + r) / a.group >= n_tok ? 0.f : 1.f / L);
+    const float* parts = a.part + bhr * a.n_splits * (size_t)RB * PS;
+    const int nt = blockDim.x, i0 = threadIdx.x;
+    if (a.n_splits <= 4) {
+        for (int i = i0; i < R * (D / 2); i += 4 * nt) q8_merge_items<D, RB, 2, 4, 4>(a, parts, b, h, rbase, R, n_tok, i, nt);
+    } else {
+        for (int i = i0; i < R * (D / 2); i += nt) q8_merge_items<D, RB, 2, 1, 16>(a, parts, b, h, rbase, R, n_tok, i, nt);
     }
 }
 

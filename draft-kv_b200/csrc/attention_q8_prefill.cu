@@ -40,7 +40,7 @@ constexpr int kQpThreads = kQpSoft + kQpConv + 32;
 constexpr int kQpNst = 2;               // K and V ring depth
 constexpr int kQpTmemCols = 512;        // per query tile t: S at 256 t (P over it), O at 256 t + 128
 constexpr int kQpSplit = 16384;         // most keys a split has (page ids staged in shared memory)
-constexpr int kQpMinSplit = 2048;
+constexpr int kQpMinSplit = 512;
 constexpr float kQpLazy = 8.f;
 constexpr int kQpBias = 6;
 constexpr int kQpDown = -20;            // V block exponents below the largest that probabilities carry
@@ -134,7 +134,6 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
         }
         for (int r = threadIdx.x; r < R; r += kQpThreads)
             *reinterpret_cast<float2*>(a.part + ((bhr * a.n_splits + s) * kQpRows + r) * PS) = make_float2(-INFINITY, 0.f);
-        q8_merge_splits<D, kQpRows>(a, bhr, b, h, r0, R, n_tok);
         return;
     }
     if (threadIdx.x == 0) {
@@ -547,7 +546,21 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
         tc_fence_after();
         tmem_dealloc(tmem, kQpTmemCols);
     }
-    if (!alone) q8_merge_splits<D, kQpRows>(a, bhr, b, h, r0, R, n_tok);
+}
+
+// The splits' partial rows merged into outputs, D / 4 threads a row (a launch of
+// its own: the 256 rows of a block, by the CTA that ends last, took 35 to 60 us).
+constexpr int kQpMergeThreads = 256;
+template <int D>
+__global__ void __launch_bounds__(kQpMergeThreads) q8_prefill_merge_kernel(Q8AttnArgs a) {
+    constexpr int PS = D + 4, ROWS = kQpMergeThreads * 4 / D;          // rows a CTA
+    pdl_trigger();
+    pdl_wait();
+    const int h = blockIdx.y, b = blockIdx.z, row0 = blockIdx.x * ROWS, rb = row0 / kQpRows, r0 = rb * kQpRows;
+    const int n_tok = a.n_rows ? min(a.n_rows[b], a.T) : a.T;
+    const size_t bhr = ((size_t)b * a.v.n_kv + h) * a.n_rb + rb;
+    q8_merge_items<D, kQpRows, 4, 1, 8>(a, a.part + bhr * a.n_splits * (size_t)kQpRows * PS, b, h, r0,
+                                        min(kQpRows, a.T * a.group - r0), n_tok, (row0 - r0) * (D / 4) + threadIdx.x, 0);
 }
 
 // Keys per split: the whole capacity up to 16384 keys; where the row blocks
@@ -568,7 +581,7 @@ size_t prefill_layout(dkv_dims dims, int group, int T, int capacity, Q8AttnArgs*
         a->split = split;
         a->n_splits = ns;
         a->n_rb = n_rb;
-        a->tickets = ar->take<unsigned>(kQ8Tickets);
+        ar->take<unsigned>(kQ8Tickets);                    // (zero for other calls over the same buffer)
         a->part = ar->take<float>(part);
     }
     return kQ8Tickets * sizeof(unsigned) + align_up(part * sizeof(float), 256) + 1024;
@@ -583,17 +596,23 @@ size_t attn_q8_prefill_work(dkv_dims dims, int group, int T, int capacity) {
 int attn_q8_prefill(Q8AttnArgs& a, dkv_dims dims, void* work, size_t work_bytes, cudaStream_t st) {
     Arena ar(work, work_bytes);
     prefill_layout(dims, a.group, a.T, a.v.capacity(), &a, &ar);
-    DKV_REQUIRE(a.tickets && a.part, "dkv_q8_attn: work buffer");
-    const size_t n_tk = (size_t)dims.batch * dims.n_kv * a.n_rb;
-    DKV_REQUIRE((a.n_splits == 1 || n_tk <= kQ8Tickets) && n_tk * a.n_splits <= 0x7fffffffu, "dkv_q8_attn: batch x heads x row blocks too large");
+    DKV_REQUIRE(a.part, "dkv_q8_attn: work buffer");
+    const size_t ctas = (size_t)dims.batch * dims.n_kv * a.n_rb * a.n_splits;
+    DKV_REQUIRE(ctas <= 0x7fffffffu, "dkv_q8_attn: batch x heads x row blocks too large");
     ProfScope ps(DKV_PROF_ATTN_FULL, 0.0, st);
-    const dim3 grid((unsigned)(n_tk * a.n_splits));
+    const dim3 grid((unsigned)ctas);
     if (dims.d == 128) {
         DKV_CUDA(allow_smem_max_once<q8_prefill_kernel<128>>());
         DKV_CUDA(launch_pdl(q8_prefill_kernel<128>, grid, dim3(kQpThreads), QpGeo<128>::SMEM, st, a));
     } else {
         DKV_CUDA(allow_smem_max_once<q8_prefill_kernel<64>>());
         DKV_CUDA(launch_pdl(q8_prefill_kernel<64>, grid, dim3(kQpThreads), QpGeo<64>::SMEM, st, a));
+    }
+    if (a.n_splits > 1) {
+        const int rows = kQpMergeThreads * 4 / dims.d;
+        const dim3 mg((unsigned)((a.T * a.group + rows - 1) / rows), (unsigned)dims.n_kv, (unsigned)dims.batch);
+        DKV_CUDA(dims.d == 128 ? launch_pdl(q8_prefill_merge_kernel<128>, mg, dim3(kQpMergeThreads), 0, st, a)
+                               : launch_pdl(q8_prefill_merge_kernel<64>, mg, dim3(kQpMergeThreads), 0, st, a));
     }
     return DKV_OK;
 }
