@@ -358,14 +358,22 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
             constexpr int LPR = D / 4, RPI = 32 / LPR;            // lanes a row, rows a step
             const int li = lane % LPR;
             uint8_t* qt = sm + t * Geo::QT;
-#pragma unroll 4
-            for (int i = 0; i < LPR; ++i) {
-                const int wr = i * RPI + lane / LPR, row = (warp & 3) * 32 + wr, qr = r0 + t * kQpTile + row;
-                const bool there = t * kQpTile + row < R && qr / G < n_tok;
-                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (there)
-                    x = q8_ld(reinterpret_cast<const float4*>(
+            constexpr int B = 16;                                 // rows in flight a lane
+#pragma unroll 1
+            for (int i0 = 0; i0 < LPR; i0 += B) {
+            float4 xs[B];
+#pragma unroll
+            for (int k = 0; k < B; ++k) {
+                const int row = (warp & 3) * 32 + (i0 + k) * RPI + lane / LPR, qr = r0 + t * kQpTile + row;
+                xs[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (t * kQpTile + row < R && qr / G < n_tok)
+                    xs[k] = q8_ld(reinterpret_cast<const float4*>(
                         a.q + (((size_t)b * a.T + qr / G) * v.n_kv * G + h * G + qr % G) * D + 4 * li));
+            }
+#pragma unroll
+            for (int k = 0; k < B; ++k) {
+                const int i = i0 + k, row = (warp & 3) * 32 + i * RPI + lane / LPR;
+                const float4 x = xs[k];
                 float am = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
 #pragma unroll
                 for (int o = 1; o < LPR; o <<= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
@@ -378,6 +386,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
                 uint8_t* at = qt + (u >> 3) * 16384 + row * 128 + in;
                 *reinterpret_cast<uint32_t*>(at + (((u & 7) ^ (row & 7)) << 4)) = h2(x.x * f, x.y * f);
                 *reinterpret_cast<uint32_t*>(at + ((((u + 2) & 7) ^ (row & 7)) << 4)) = h2(x.z * f, x.w * f);
+            }
             }
             fence_async_shared();
             named_sync(1, kQpSoft + 32);
