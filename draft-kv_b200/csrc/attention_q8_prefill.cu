@@ -159,39 +159,52 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
-    // per 16-key group of the key range: page id and scales; keys of a bad page are not seen
-    const int n_grp = (kend - k0 + 15) / 16;
-    for (int i = threadIdx.x; i < ntiles * 8; i += kQpThreads) {
-        const int pid = i < n_grp ? q8_ld(v.row(b) + ((k0 + i * 16) >> v.page_shift)) : -1;
-        const bool ok = v.ok(pid);
-        float2 sc = make_float2(1.f, 1.f);
-        int ev = kQ8ExpMin;
-        if (ok) {
-            sc = q8_ld(reinterpret_cast<const float2*>(v.scale + v.scale_at(pid, h, 0)));
-            ev = min(max(q8_scale_exp(sc.y), kQ8ExpMin), kQ8ExpMax);
-            atomicMax(&emax_s, ev);
-        } else if (i < n_grp) {
-            atomicOr(a.err, kErrQ8Page);
-            atomicOr(&bad_s[i >> 5], 1u << (i & 31));
+    // Converters and the MMA warp, while the others load Q: per 16-key group of the
+    // key range, page id and scales (all of a thread's loads in two rounds); keys of
+    // a bad page are not seen.  The MMA warp meets the softmax warps after this.
+    if (warp >= 8) {
+        constexpr int NS = kQpThreads - kQpSoft, PER = (kQpSplit / 16 + NS - 1) / NS;
+        const int first = threadIdx.x - kQpSoft, n_grp = (kend - k0 + 15) / 16;
+        int pid[PER];
+        float2 sc[PER];
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const int i = first + k * NS;
+            pid[k] = i < n_grp ? q8_ld(v.row(b) + ((k0 + i * 16) >> v.page_shift)) : -1;
         }
-        page_s[i] = ok ? pid : -1;
-        kf_s[i] = sc.x;
-        ev_s[i] = (int8_t)ev;
+#pragma unroll
+        for (int k = 0; k < PER; ++k)
+            sc[k] = v.ok(pid[k]) ? q8_ld(reinterpret_cast<const float2*>(v.scale + v.scale_at(pid[k], h, 0))) : make_float2(1.f, 1.f);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const int i = first + k * NS;
+            if (i >= ntiles * 8) break;
+            const bool there = v.ok(pid[k]);
+            const int ev = there ? min(max(q8_scale_exp(sc[k].y), kQ8ExpMin), kQ8ExpMax) : kQ8ExpMin;
+            if (there) {
+                atomicMax(&emax_s, ev);
+            } else if (i < n_grp) {
+                atomicOr(a.err, kErrQ8Page);
+                atomicOr(&bad_s[i >> 5], 1u << (i & 31));
+            }
+            page_s[i] = there ? pid[k] : -1;
+            kf_s[i] = sc[k].x;
+            ev_s[i] = (int8_t)ev;
+        }
+        named_sync(2, NS);
+        for (int i = first; i < ntiles * 8; i += NS) {
+            const int dv = max((int)ev_s[i] - emax_s, kQpDown);
+            dv_s[i] = (float)dv;
+            iv_s[i] = q8_pow2(-dv);
+        }
+        named_sync(2, NS);
     }
-    __syncthreads();
-    const int evm = emax_s;
-    for (int i = threadIdx.x; i < ntiles * 8; i += kQpThreads) {
-        const int dv = max((int)ev_s[i] - evm, kQpDown);
-        dv_s[i] = (float)dv;
-        iv_s[i] = q8_pow2(-dv);
-    }
-    __syncthreads();
 
     bool ok = true;
     if (warp >= 8 && warp < 12) {
         // ---------------- converters: warp w takes groups 2 w and 2 w + 1 of a tile
         constexpr int NJ = D / 32;                                // 512-byte blocks a group and side
-        const int w = warp - 8, g = lane >> 2, t = lane & 3;
+        const int w = warp - 8, g = lane >> 2, t = lane & 3, evm = emax_s;
         uint4 kr[2][NJ], vr[2][NJ];
         auto load = [&](int j, int i, uint4 (&r)[2][NJ]) {
 #pragma unroll
@@ -304,7 +317,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
                          sw128_desc(k_s + (kk >> 2) * 16384 + (kk & 3) * 32), idS, kk != 0 ? 1u : 0u);
             tc_commit(&s_full[t]);
         };
-        named_sync(1, kQpSoft + 32);      // Q is in shared memory
+        named_sync(1, kQpSoft + 32);      // Q is in shared memory, and the softmax warps may read the scales
         for (int j = 0; j < ntiles && ok; ++j) {
             if (!wait_all(&k_full[j % kQpNst], (uint32_t)((j / kQpNst) & 1)) ||
                 (j >= 1 && !wait_all(&v_full[(j - 1) % kQpNst], (uint32_t)(((j - 1) / kQpNst) & 1)))) {
@@ -510,6 +523,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
         float* mypart = alone ? nullptr : a.part + ((bhr * a.n_splits + s) * kQpRows + cr) * PS;
         if (l != l && m == -INFINITY) m = 0.f;     // NaN scores have no max: give the row one, so that its NaN comes out
         const bool live = ok && m != -INFINITY;
+        const int evm = emax_s;
         // O is in units of 2^(evm - bias), l in units of 2^-bias.  (Apart from the
         // sum: 2^evm / l may be too small for fp32 where their result is not.)
         const float un = alone ? q8_pow2(evm) : q8_pow2(evm - kQpBias);
