@@ -26,6 +26,7 @@
 // tile against 128 * 2 d bytes.
 // Every mbarrier wait is bounded (error word 0x80).
 #include <algorithm>
+#include <type_traits>
 
 #include "attention_q8.cuh"
 #include "prefill_common.cuh"
@@ -367,39 +368,48 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
         float c = 1.f;                                            // scores = S * c * (K scale), log2 units
         {
             // the warp's 32 rows of Q as f16 of q * log2 e / sqrt(d) * 2^-x, x the
-            // row's exponent: D / 4 lanes a row, 16 bytes each
-            constexpr int LPR = D / 4, RPI = 32 / LPR;            // lanes a row, rows a step
-            const int li = lane % LPR;
+            // row's exponent.  8 lanes a row: of each 64-dim half a lane makes one
+            // 16-byte unit, li, from the four pairs it consists of.  The loads of 16
+            // rows go out together
+            constexpr int B = 4, CH = Geo::CH;                    // 4-row steps a round, 64-dim halves
+            const int li = lane & 7, from = 32 * (li & 1) + 2 * (li >> 1);
             uint8_t* qt = sm + t * Geo::QT;
-            constexpr int B = 16;                                 // rows in flight a lane
 #pragma unroll 1
-            for (int i0 = 0; i0 < LPR; i0 += B) {
-            float4 xs[B];
+            for (int i0 = 0; i0 < 8; i0 += B) {
+                float2 x[B][CH][4];
 #pragma unroll
-            for (int k = 0; k < B; ++k) {
-                const int row = (warp & 3) * 32 + (i0 + k) * RPI + lane / LPR, qr = r0 + t * kQpTile + row;
-                xs[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (t * kQpTile + row < R && qr / G < n_tok)
-                    xs[k] = q8_ld(reinterpret_cast<const float4*>(
-                        a.q + (((size_t)b * a.T + qr / G) * v.n_kv * G + h * G + qr % G) * D + 4 * li));
-            }
+                for (int k = 0; k < B; ++k) {
+                    const int row = (warp & 3) * 32 + (i0 + k) * 4 + (lane >> 3), qr = r0 + t * kQpTile + row;
+                    const bool there = t * kQpTile + row < R && qr / G < n_tok;
+                    const float* at = a.q + (((size_t)b * a.T + qr / G) * v.n_kv * G + h * G + qr % G) * D + from;
 #pragma unroll
-            for (int k = 0; k < B; ++k) {
-                const int i = i0 + k, row = (warp & 3) * 32 + i * RPI + lane / LPR;
-                const float4 x = xs[k];
-                float am = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+                    for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
-                for (int o = 1; o < LPR; o <<= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
-                const int ex = min(max((int)(__float_as_uint(am * a.scale) >> 23) - 127, -100), 126);
-                const float f = a.scale * q8_pow2(-ex);
-                const int mx = __shfl_sync(0xffffffffu, ex, (lane % RPI) * LPR);
-                if (lane / RPI == i) c = q8_pow2(mx);             // (this thread's own row: lane = i * RPI + ..)
-                // dims 4 li .. + 3 are two pairs: block li / 8, half li / 4 % 2, t = 2 li % 4, + 1
-                const int blk = li >> 3, u = (blk >> 1) * 8 + (blk & 1) + 2 * ((2 * li) & 3), in = ((li >> 2) & 1) * 8 + ((li >> 1) & 1) * 4;
-                uint8_t* at = qt + (u >> 3) * 16384 + row * 128 + in;
-                *reinterpret_cast<uint32_t*>(at + (((u & 7) ^ (row & 7)) << 4)) = h2(x.x * f, x.y * f);
-                *reinterpret_cast<uint32_t*>(at + ((((u + 2) & 7) ^ (row & 7)) << 4)) = h2(x.z * f, x.w * f);
-            }
+                        for (int p = 0; p < 4; ++p)
+                            x[k][ch][p] = there ? q8_ld(reinterpret_cast<const float2*>(at + ch * 64 + p * 8)) : make_float2(0.f, 0.f);
+                }
+#pragma unroll
+                for (int k = 0; k < B; ++k) {
+                    const int row = (warp & 3) * 32 + (i0 + k) * 4 + (lane >> 3);
+                    float am = 0.f;
+#pragma unroll
+                    for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+                        for (int p = 0; p < 4; ++p) am = pf_max3(am, fabsf(x[k][ch][p].x), fabsf(x[k][ch][p].y));
+#pragma unroll
+                    for (int o = 1; o < 8; o <<= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
+                    const int ex = min(max((int)(__float_as_uint(am * a.scale) >> 23) - 127, -100), 126);
+                    const float f = a.scale * q8_pow2(-ex);
+                    const int mx = __shfl_sync(0xffffffffu, ex, (lane & 3) * 8);
+                    if ((lane >> 2) == i0 + k) c = q8_pow2(mx);   // (this thread's own row)
+#pragma unroll
+                    for (int ch = 0; ch < CH; ++ch) {
+                        const float2(&y)[4] = x[k][ch];
+                        *reinterpret_cast<uint4*>(qt + ch * 16384 + row * 128 + ((li ^ (row & 7)) << 4)) =
+                            make_uint4(h2(y[0].x * f, y[0].y * f), h2(y[1].x * f, y[1].y * f), h2(y[2].x * f, y[2].y * f),
+                                       h2(y[3].x * f, y[3].y * f));
+                    }
+                }
             }
             fence_async_shared();
             named_sync(1, kQpSoft + 32);
@@ -530,28 +540,50 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
         const float f = alone && live ? 1.f / l : 1.f;
         const size_t out_at = (((size_t)b * a.T + gr / G) * v.n_kv * G + h * G + gr % G) * D;
         if (__all_sync(0xffffffffu, ok)) {
+            // through the drained K and V rings (a part of each warp's own), so that
+            // whole rows are stored: a lane's 16-byte chunk ch of row r at ch ^ r
+            const bool wide = !alone || a.out_dtype == DKV_F32;
+            uint8_t* stg = sm + Geo::K0 + warp * (32 * D * 4);
 #pragma unroll 1
             for (int c0 = 0; c0 < D; c0 += 32) {
                 uint32_t o[32];
                 tmem_ld32(ob + c0, o);
                 tmem_wait_ld();
-                if (!mine) continue;
 #pragma unroll
                 for (int e = 0; e < 32; ++e) o[e] = live ? __float_as_uint(__uint_as_float(o[e]) * f * un) : 0u;
-                if (!alone || a.out_dtype == DKV_F32) {
-                    if (!alone && !live) continue;
-                    float* to = alone ? reinterpret_cast<float*>(a.out) + out_at + c0 : mypart + 4 + c0;
+                if (wide) {
 #pragma unroll
                     for (int e = 0; e < 32; e += 4)
-                        *reinterpret_cast<uint4*>(to + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                        *reinterpret_cast<uint4*>(stg + lane * D * 4 + ((((c0 + e) / 4) ^ (lane & (D / 4 - 1))) << 4)) =
+                            make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
                 } else {
-                    uint16_t* to = reinterpret_cast<uint16_t*>(a.out) + out_at + c0;
                     auto bf2 = [&](int e) { return pack_bf2(__uint_as_float(o[e]), __uint_as_float(o[e + 1])); };
 #pragma unroll
                     for (int e = 0; e < 32; e += 8)
-                        *reinterpret_cast<uint4*>(to + e) = make_uint4(bf2(e), bf2(e + 2), bf2(e + 4), bf2(e + 6));
+                        *reinterpret_cast<uint4*>(stg + lane * D * 2 + ((((c0 + e) / 8) ^ (lane & (D / 8 - 1))) << 4)) =
+                            make_uint4(bf2(e), bf2(e + 2), bf2(e + 4), bf2(e + 6));
                 }
             }
+            __syncwarp();
+            const unsigned rows = __ballot_sync(0xffffffffu, mine);
+            auto copy_rows = [&](auto lanes_a_row, auto dest) {
+                constexpr int LP = decltype(lanes_a_row)::value;      // 16-byte chunks a row
+                const int ch = lane % LP;
+#pragma unroll 4
+                for (int i = 0; i < LP; ++i) {
+                    const int r = i * (32 / LP) + lane / LP;
+                    const size_t at = __shfl_sync(0xffffffffu, out_at, r);
+                    if ((rows >> r) & 1u)
+                        *reinterpret_cast<uint4*>(dest(r, at) + ch * 16) =
+                            *reinterpret_cast<const uint4*>(stg + r * LP * 16 + ((ch ^ (r & (LP - 1))) << 4));
+                }
+            };
+            if (!alone)
+                copy_rows(std::integral_constant<int, D / 4>{}, [&](int r, size_t) { return reinterpret_cast<uint8_t*>(mypart + (r - lane) * PS + 4); });
+            else if (wide)
+                copy_rows(std::integral_constant<int, D / 4>{}, [&](int, size_t at) { return reinterpret_cast<uint8_t*>(a.out) + at * 4; });
+            else
+                copy_rows(std::integral_constant<int, D / 8>{}, [&](int, size_t at) { return reinterpret_cast<uint8_t*>(a.out) + at * 2; });
         }
         if (!alone && cr < R)
             *reinterpret_cast<float2*>(mypart) = make_float2(live ? m : -INFINITY, live ? l * q8_pow2(-kQpBias) : 0.f);
