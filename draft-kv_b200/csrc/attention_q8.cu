@@ -104,7 +104,6 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
         fence_async_shared();
     }
     __syncwarp();
-    pdl_trigger();
     pdl_wait();            // queries and the new entries come from earlier kernels
 
     // one round of loads: the first page ids (any entry of the table row may be
@@ -528,6 +527,7 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
                 }
             }
     }
+    pdl_trigger();
     __syncthreads();
     const size_t bhr = ((size_t)b * v.n_kv + h) * a.n_rb + rb;
     const bool alone = a.n_splits == 1;
@@ -586,7 +586,6 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
 constexpr int kMassThreads = 256, kMassKeys = 4;
 __global__ void __launch_bounds__(kMassThreads) q8_mass_kernel(Q8AttnArgs a, float* mass) {
     __shared__ float2 st_s[kQ8MaxRows + 1];
-    pdl_trigger();
     pdl_wait();
     const int h = blockIdx.y, b = blockIdx.z, R = a.T * a.group;
     const int n = a.n_keys(b), e0 = a.first(b), key0 = blockIdx.x * kMassThreads * kMassKeys + threadIdx.x;
@@ -618,6 +617,7 @@ __global__ void __launch_bounds__(kMassThreads) q8_mass_kernel(Q8AttnArgs a, flo
             if (s1.y != 0.f && key <= l1) sum[k] += q8_ex2(x.y - s1.x) * s1.y;
         }
     }
+    pdl_trigger();
 #pragma unroll
     for (int k = 0; k < kMassKeys; ++k)
         if (key0 + k * kMassThreads < n) mass[bh * cap + key0 + k * kMassThreads] = old[k] + sum[k];

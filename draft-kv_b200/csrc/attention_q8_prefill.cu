@@ -117,7 +117,6 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
     const size_t bhr = ((size_t)b * v.n_kv + h) * a.n_rb + rb;
     const bool alone = a.n_splits == 1;
 
-    pdl_trigger();
     pdl_wait();
     const int e0 = a.first(b);
     const int n_tok = a.n_rows ? min(a.n_rows[b], a.T) : a.T;
@@ -589,6 +588,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
             *reinterpret_cast<float2*>(mypart) = make_float2(live ? m : -INFINITY, live ? l * q8_pow2(-kQpBias) : 0.f);
     }
 
+    pdl_trigger();
     const bool all_ok = __syncthreads_and(ok) != 0;
     if (!all_ok && warp == 12 && lane == 0) {
         // a wait ran out: the MMAs still in flight end before the memory is let go
@@ -609,7 +609,6 @@ constexpr int kQpMergeThreads = 256;
 template <int D>
 __global__ void __launch_bounds__(kQpMergeThreads) q8_prefill_merge_kernel(Q8AttnArgs a) {
     constexpr int PS = D + 4, ROWS = kQpMergeThreads * 4 / D;          // rows a CTA
-    pdl_trigger();
     pdl_wait();
     const int h = blockIdx.y, b = blockIdx.z, row0 = blockIdx.x * ROWS, rb = row0 / kQpRows, r0 = rb * kQpRows;
     const int n_tok = a.n_rows ? min(a.n_rows[b], a.T) : a.T;

@@ -124,7 +124,6 @@ template <bool VEC>
 __global__ void __launch_bounds__(kQ8Threads) q8_append_kernel(Q8AppendArgs a) {
     extern __shared__ __align__(16) float stage[];
     __shared__ float red[32];
-    pdl_trigger();
     pdl_wait();
     const Q8View& v = a.v;
     const int b = blockIdx.z >> 1, i = blockIdx.z & 1, h = blockIdx.y;
@@ -195,6 +194,7 @@ __global__ void __launch_bounds__(kQ8Threads) q8_append_kernel(Q8AppendArgs a) {
         const int p0 = a.pos0 ? a.pos0[b] : e0;
         for (int r = lo + threadIdx.x; r < hi; r += kQ8Threads) a.pos[m0 + r] = p0 + base + r - e0;
     }
+    pdl_trigger();
     amax = block_max(amax, red);
     float* sc = v.scale + v.scale_at(pid, h, i);
     const int e_old = lo > 0 ? min(max(q8_scale_exp(*sc), kQ8ExpMin), kQ8ExpMax) : kQ8ExpMin;
@@ -331,7 +331,6 @@ __global__ void __launch_bounds__(kSelThreads) q8_select_kernel(Q8EvictArgs a, i
     const uint32_t rank = cluster > 1 ? cluster_rank() : 0u;
     const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     for (int i = tid; i < 3 * kSelBins; i += kSelThreads) sel_sm[i] = 0u;
-    pdl_trigger();
     pdl_wait();
     int n;
     const int keep = evict_keep(a, b, &n);
@@ -450,6 +449,7 @@ __global__ void __launch_bounds__(kSelThreads) q8_select_kernel(Q8EvictArgs a, i
         cluster_arrive_all();                      // (waited for at the end: shared memory outlives its readers)
     }
 
+    pdl_trigger();
     if (i0 < i1) {
         // A warp a contiguous part of the slice, 32 groups of 32 entries at a time:
         // lane g holds, as bits, which entries of group g lie below the key and at
@@ -602,7 +602,6 @@ __global__ void __launch_bounds__(gather_threads(D, TILES)) q8_gather_kernel(Q8E
     const Q8View& v = a.v;
     const int b = blockIdx.z >> 1, side = blockIdx.z & 1, h = blockIdx.y, pg = blockIdx.x, tid = threadIdx.x;
     const int wi = tid >> 5, lane = tid & 31;
-    pdl_trigger();
     pdl_wait();
     const int src = tid < TILES * 16 ? a.kept[(((size_t)b * v.n_kv + h) * a.out_pages + pg) * v.page + tid] : -1;
     const int pid = q8_ld(a.out_table + (size_t)b * a.out_pages + pg);
@@ -698,6 +697,7 @@ __global__ void __launch_bounds__(gather_threads(D, TILES)) q8_gather_kernel(Q8E
     if (tid < TILES * 16) factors[tid] = shift_of(er, e);
     if (tid == 0) v.scale[v.scale_at(pid, h, side)] = q8_pow2(e);
     __syncthreads();
+    pdl_trigger();
     uint8_t* out = v.side(pid, h, side);
 #pragma unroll
     for (int x = 0; x < FR; ++x) {
