@@ -581,40 +581,62 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
 
 // mass[b][h][j] += sum over the call's rows of p_j: the scores of the pass
 // above under the merged (max, sum), rows in order (no atomics).
-// A thread takes kMassKeys keys, kMassThreads apart, whose loads are in flight
-// together.
+// A thread takes kMassKeys keys, kMassThreads apart, W rows of each at a time (8:
+// a sector a load pair; rows of 2 scores: 2), whose loads are in flight together.
+// (Two rows at a time, each sector fetched four times: 42 rows over 3 x 6 x 36337
+// entries 75 us; so, 38 us.)
 constexpr int kMassThreads = 256, kMassKeys = 4;
+template <int W>
 __global__ void __launch_bounds__(kMassThreads) q8_mass_kernel(Q8AttnArgs a, float* mass) {
-    __shared__ float2 st_s[kQ8MaxRows + 1];
+    __shared__ float2 st_s[kQ8MaxRows + 8];        // (max, 1 / sum) of a row
+    __shared__ int last_s[kQ8MaxRows + 8];         // a row's scores exist up to its own entry
     pdl_wait();
     const int h = blockIdx.y, b = blockIdx.z, R = a.T * a.group;
     const int n = a.n_keys(b), e0 = a.first(b), key0 = blockIdx.x * kMassThreads * kMassKeys + threadIdx.x;
     if ((int)(blockIdx.x * kMassThreads * kMassKeys) >= n) return;
     const size_t bh = (size_t)b * a.v.n_kv + h, cap = a.v.capacity();
     float old[kMassKeys], sum[kMassKeys];
-    float2 x0[kMassKeys];
     const float* sc = a.scores + (bh * cap + key0) * a.s_ld;
+    constexpr int V = W == 2 ? 2 : 4;              // scores a load
+    float x[kMassKeys][W];
+    auto load = [&](int r) {
+#pragma unroll
+        for (int k = 0; k < kMassKeys; ++k)
+#pragma unroll
+            for (int w = 0; w < W; w += V) {
+                const float* at = sc + (size_t)k * kMassThreads * a.s_ld + r + w;
+                if (key0 + k * kMassThreads >= n || r + w >= a.s_ld) continue;
+                if (V == 2) {
+                    const float2 y = __ldcg(reinterpret_cast<const float2*>(at));
+                    x[k][w] = y.x, x[k][w + 1] = y.y;
+                } else {
+                    const float4 y = __ldcg(reinterpret_cast<const float4*>(at));
+                    x[k][w] = y.x, x[k][w + 1] = y.y, x[k][w + V - 2] = y.z, x[k][w + V - 1] = y.w;
+                }
+            }
+    };
 #pragma unroll
     for (int k = 0; k < kMassKeys; ++k) {
-        const int key = key0 + k * kMassThreads;
         sum[k] = 0.f;
-        old[k] = key < n ? mass[bh * cap + key] : 0.f;
-        x0[k] = key < n ? __ldcg(reinterpret_cast<const float2*>(sc + (size_t)k * kMassThreads * a.s_ld))
-                        : make_float2(0.f, 0.f);
-    }
-    for (int r = threadIdx.x; r <= R; r += kMassThreads) st_s[r] = r < R ? a.stats[bh * R + r] : make_float2(0.f, 0.f);
-    __syncthreads();
-    for (int r = 0; r < R; r += 2) {
-        const float2 s0 = st_s[r], s1 = st_s[r + 1];
-        const int l0 = e0 + r / a.group, l1 = e0 + (r + 1) / a.group;     // a row's scores exist up to its own entry
+        old[k] = key0 + k * kMassThreads < n ? mass[bh * cap + key0 + k * kMassThreads] : 0.f;
 #pragma unroll
-        for (int k = 0; k < kMassKeys; ++k) {
-            const int key = key0 + k * kMassThreads;
-            if (key >= n) continue;
-            const float2 x = r == 0 ? x0[k]
-                                    : __ldcg(reinterpret_cast<const float2*>(sc + (size_t)k * kMassThreads * a.s_ld + r));
-            if (s0.y != 0.f && key <= l0) sum[k] += q8_ex2(x.x - s0.x) * s0.y;
-            if (s1.y != 0.f && key <= l1) sum[k] += q8_ex2(x.y - s1.x) * s1.y;
+        for (int w = 0; w < W; ++w) x[k][w] = 0.f;
+    }
+    load(0);
+    for (int r = threadIdx.x; r < kQ8MaxRows + 8; r += kMassThreads) {
+        st_s[r] = r < R ? a.stats[bh * R + r] : make_float2(0.f, 0.f);
+        last_s[r] = e0 + r / a.group;
+    }
+    __syncthreads();
+    for (int r = 0; r < R; r += W) {
+        if (r > 0) load(r);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float2 st = st_s[r + w];
+            const int last = last_s[r + w];
+#pragma unroll
+            for (int k = 0; k < kMassKeys; ++k)
+                if (st.y != 0.f && key0 + k * kMassThreads <= last) sum[k] += q8_ex2(x[k][w] - st.x) * st.y;
         }
     }
     pdl_trigger();
@@ -651,7 +673,7 @@ int split_count(dkv_dims dims, int capacity, int split_keys) {
 size_t decode_work(dkv_dims dims, int R, int capacity, int split_keys, bool mass, Q8AttnArgs* a, Arena* ar) {
     const int rb = row_block(R), n_rb = (R + rb - 1) / rb, ns = split_count(dims, capacity, split_keys);
     const size_t bh = (size_t)dims.batch * dims.n_kv;
-    const size_t part = bh * n_rb * ns * rb * (dims.d + 4), s_ld = (size_t)(R + 1) / 2 * 2;
+    const size_t part = bh * n_rb * ns * rb * (dims.d + 4), s_ld = R <= 2 ? 2 : (size_t)(R + 3) / 4 * 4;
     if (a) {
         a->tickets = ar->take<unsigned>(kQ8Tickets);
         a->part = ar->take<float>(part);
@@ -738,9 +760,19 @@ extern "C" int dkv_q8_attn(const dkv_q8_cache* cache, dkv_dims dims, int layer, 
     else
         e = plo ? launch_decode_rows<64, true>(a, R, grid, st) : launch_decode_rows<64, false>(a, R, grid, st);
     DKV_CUDA(e);
-    if (mass)
-        DKV_CUDA(launch_pdl(q8_mass_kernel, dim3((unsigned)((cap + kMassThreads * kMassKeys - 1) / (kMassThreads * kMassKeys)), (unsigned)dims.n_kv,
-                                 (unsigned)dims.batch),
-                            dim3(kMassThreads), 0, st, a, mass));
+    if (mass) {
+        const dim3 mg((unsigned)((cap + kMassThreads * kMassKeys - 1) / (kMassThreads * kMassKeys)), (unsigned)dims.n_kv,
+                      (unsigned)dims.batch);
+        // (after more than one wave an early start takes SMs from the CTAs that are
+        // still to come: 42 rows over 3 x 6 x 36337 entries 257 us, 242 us without)
+        if ((size_t)grid.x * grid.y * grid.z <= 2 * 148)
+            DKV_CUDA(a.s_ld == 2 ? launch_pdl(q8_mass_kernel<2>, mg, dim3(kMassThreads), 0, st, a, mass)
+                                 : launch_pdl(q8_mass_kernel<8>, mg, dim3(kMassThreads), 0, st, a, mass));
+        else if (a.s_ld == 2)
+            q8_mass_kernel<2><<<mg, kMassThreads, 0, st>>>(a, mass);
+        else
+            q8_mass_kernel<8><<<mg, kMassThreads, 0, st>>>(a, mass);
+        DKV_LAUNCHED();
+    }
     return DKV_OK;
 }
