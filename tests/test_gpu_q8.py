@@ -259,6 +259,15 @@ def test_attention_split_over_keys(split, T, group):
     check_attention(mk, r, q, e0, out_dtype=torch.float32, split_keys=split, with_mass=True)
 
 
+def test_mass_behind_several_waves():
+    """32 splits x 2 heads x 2 sequences x 3 row blocks are more CTAs than the GPU holds."""
+    mk = Made(2, 1, 2, 64, 16, 256, seed=8)
+    rng = np.random.default_rng(6)
+    r = mk.fill([4000, 2100], rng, spread=0.5)
+    q = rng.standard_normal((2, 11, 6, 64)).astype(np.float32)
+    check_attention(mk, r, q, [3989, 2089], with_mass=True, split_keys=128, out_dtype=torch.float32)
+
+
 @pytest.mark.parametrize("d,group", [(64, 3), (128, 4), (128, 1)])
 def test_verify_rows_equal_decode_rows_bit_for_bit(d, group):
     mk = Made(2, 1, 2, d, 16, 80, seed=5)
@@ -397,6 +406,17 @@ def test_prompt_attention_over_key_splits(d, page):
     check_attention(mk, r, q, [e0])
     r0 = mk.cache.attention(0, torch.from_numpy(q).cuda(), i32([-T]))
     assert (r0 == 0).all()
+
+
+@pytest.mark.parametrize("d,out_dtype", [(64, torch.float32), (128, torch.bfloat16)])
+def test_prompt_row_blocks_over_key_splits(d, out_dtype):
+    """Two row blocks, four key splits of which the short sequence reaches one, tokens that are not there."""
+    mk = Made(2, 1, 2, d, 32, 64, seed=3)
+    rng = np.random.default_rng(d)
+    T, e0 = 130, [1500, 3]
+    r = mk.fill([x + T for x in e0], rng, spread=0.5)
+    q = rng.standard_normal((2, T, 6, d)).astype(np.float32)
+    check_attention(mk, r, q, e0, n_rows=[130, 77], out_dtype=out_dtype)
 
 
 def test_prompt_rows_that_see_nothing_or_are_not_there():
