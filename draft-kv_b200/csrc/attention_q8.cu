@@ -645,6 +645,15 @@ __global__ void __launch_bounds__(kMassThreads) q8_mass_kernel(Q8AttnArgs a, flo
         if (key0 + k * kMassThreads < n) mass[bh * cap + key0 + k * kMassThreads] = old[k] + sum[k];
 }
 
+// Query rows a CTA: 16, or 8 where the rows come in an odd number of eights (at
+// d = 64, where a block of 16 takes 1.6 times one of 8, up to three of them; at
+// d = 128 1.9 times).  4 x 8 heads, 32768 entries: 20 rows of d 128 128 us in
+// eights, 155 in sixteens; of d 64 77 and 81; 56 rows of d 64 169 and 157.
+int row_block(int R, int d) {
+    const int e = (R + 7) / 8;
+    return e % 2 && (d == 128 || e <= 3) ? 8 : 16;
+}
+
 template <int D, int NT, bool PLO, bool PAIR>
 cudaError_t launch_decode(const Q8AttnArgs& a, dim3 grid, cudaStream_t st) {
     const cudaError_t e = allow_smem_max_once<q8_decode_kernel<D, NT, PLO, PAIR>>();
@@ -654,11 +663,9 @@ cudaError_t launch_decode(const Q8AttnArgs& a, dim3 grid, cudaStream_t st) {
 template <int D, bool PLO>
 cudaError_t launch_decode_rows(const Q8AttnArgs& a, int R, dim3 grid, cudaStream_t st) {
     return R <= 4 ? launch_decode<D, 1, PLO, true>(a, grid, st)
-                  : R <= 8 ? launch_decode<D, 1, PLO, false>(a, grid, st) : launch_decode<D, 2, PLO, false>(a, grid, st);
+                  : row_block(R, D) == 8 ? launch_decode<D, 1, PLO, false>(a, grid, st)
+                                      : launch_decode<D, 2, PLO, false>(a, grid, st);
 }
-
-// Query rows a CTA: 8 or 16.
-int row_block(int R) { return R <= 8 ? 8 : 16; }
 
 // Splits of the key axis.  Where the caller names no length: one wave of two
 // CTAs an SM over (sequence, head, split), and at least 128 KB of codes a split
@@ -671,7 +678,7 @@ int split_count(dkv_dims dims, int capacity, int split_keys) {
 }
 
 size_t decode_work(dkv_dims dims, int R, int capacity, int split_keys, bool mass, Q8AttnArgs* a, Arena* ar) {
-    const int rb = row_block(R), n_rb = (R + rb - 1) / rb, ns = split_count(dims, capacity, split_keys);
+    const int rb = row_block(R, dims.d), n_rb = (R + rb - 1) / rb, ns = split_count(dims, capacity, split_keys);
     const size_t bh = (size_t)dims.batch * dims.n_kv;
     const size_t part = bh * n_rb * ns * rb * (dims.d + 4), s_ld = R <= 2 ? 2 : (size_t)(R + 3) / 4 * 4;
     if (a) {

@@ -292,7 +292,7 @@ DKV_API int dkv_q8_read(const dkv_q8_cache* cache, dkv_dims dims, int b, int lay
  * the other rows, bit for bit.  split_keys (a multiple of 128): the keys go to
  * ceil(capacity / split_keys) splits; 0: a rule on (batch, n_kv, capacity).
  * Above 64 rows the splits are chosen by a rule.
- * Up to 64 rows, batch * n_kv * ceil(T * group / 16) is at most 16384 where the
+ * Up to 64 rows, batch * n_kv * ceil(T * group / 8) is at most 16384 where the
  * keys are split.
  * The first 64 KB of the work buffer must be zero when first used and are left
  * so; any call may use it, but no two that may run at the same time (two

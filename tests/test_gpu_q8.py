@@ -285,6 +285,22 @@ def test_verify_rows_equal_decode_rows_bit_for_bit(d, group):
         assert torch.equal(few, whole[:, 2:5])
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("T,group", [(5, 4), (9, 4), (11, 5)])
+def test_row_blocks_of_either_size(d, T, group):
+    """20, 36 and 55 rows come in blocks of 8 or of 16: against the definition, and row by row as one-token calls."""
+    mk = Made(2, 1, 2, d, 32, 20, seed=T)
+    rng = np.random.default_rng(T * d)
+    e0 = [500, 90]
+    r = mk.fill([x + T for x in e0], rng, spread=0.5)
+    q = rng.standard_normal((2, T, 2 * group, d)).astype(np.float32)
+    out = check_attention(mk, r, q, e0, out_dtype=torch.float32, with_mass=True)
+    for t in range(T):
+        one = mk.cache.attention(0, torch.from_numpy(q[:, t:t + 1].copy()).cuda(), i32([x + t for x in e0]),
+                                 out_dtype=torch.float32)
+        assert torch.equal(one[:, 0], out[:, t])
+
+
 def test_rows_that_see_nothing_and_rows_that_are_not_there():
     """entry0 below zero empties rows (zeros); tokens past n_rows keep their output."""
     mk = Made(3, 1, 2, 64, 16, 4, seed=9)
