@@ -68,7 +68,8 @@ DKV_DEV uint32_t movm_trans(uint32_t x) {
     return y;
 }
 // Page ids and scales of a warp's next tiles, one tile a lane; the K scale of a
-// tile that must not be seen (bad page id, past the end) is negative.
+// tile that must not be seen (bad page id, past the end) is negative, its V scale
+// the smallest.
 struct QdMeta {
     int pid;
     float ks, vs;
@@ -94,6 +95,7 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
     __shared__ float ms[RB], ls[RB];
     __shared__ float gw[RB * kQdKG];
     __shared__ int failed;
+    __shared__ int8_t own_eo[kQdKG][RB];
     const Q8View& v = a.v;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint8_t* ring = ring_all + (size_t)warp * kQdDepth * kQdUnit;
@@ -151,7 +153,7 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
         return -1;
     };
     auto load_scale = [&](int pid, float& ks, float& vs) {
-        float2 sc = make_float2(-1.f, 1.f);
+        float2 sc = make_float2(-1.f, q8_pow2(kQ8ExpMin));
         if (pid >= 0) sc = q8_ld(reinterpret_cast<const float2*>(v.scale + v.scale_at(pid, h, 0)));
         ks = sc.x;
         vs = sc.y;
@@ -187,7 +189,7 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
         }
         __syncwarp();
     };
-    QdMeta cur{-1, -1.f, 1.f}, nxt{-1, -1.f, 1.f};
+    QdMeta cur{-1, -1.f, q8_pow2(kQ8ExpMin)}, nxt = cur;
     cur.pid = check_pid(0, first_pid);
     const int prologue = min(mine, kQdDepth);
     for (int u = 0; u < prologue; ++u) issue(u, u, cur.pid);     // (kQdDepth <= UPB)
@@ -256,7 +258,12 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
     // thr: the score that forces m up
     float m[NT][2], thr[NT][2], l[NT][2];
     float o[NT][KS][4];
-    int eo = kQ8ExpMin;                                // O is in units of 2^(eo - kQdBias)
+    // O is in units of 2^(eo - kQdBias), eo the largest V exponent so far; for a row
+    // that sees no more when it grows (the growth may be more than fp32 spans) in the
+    // units of own_eo
+    int eo = kQ8ExpMin;
+    if (lane < RB) own_eo[warp][lane] = (int8_t)-128;
+    __syncwarp();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         m[nt][0] = m[nt][1] = l[nt][0] = l[nt][1] = 0.f;
@@ -425,24 +432,28 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
                 }
             }
         }
-        int ev = q8_scale_exp(vs[0]);
-#pragma unroll
-        for (int tt = 1; tt < TPU; ++tt) ev = max(ev, q8_scale_exp(vs[tt]));
-        if (ev > eo) {                                 // (uniform) larger V values: O to their units
+        // (past the last unit: over stale bytes, unused)
+        if (AHEAD) products(ring + slot1 * kQdUnit + lane * 16, sn);
+        // (uniform) larger V values in a tile: O to their units, tile by
+        // tile, so that a row's probabilities are rounded under the exponents of the
+        // tiles it sees.  (A row that does not see this tile sees none behind it.)
+        auto raise = [&](int tt, int ev) {
             const float dn = q8_pow2(max(eo - ev, -126));
-            eo = ev;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int md = 0; md < KS; ++md)
+                for (int c = 0; c < 2; ++c) {
+                    const bool seen = whole || key0 + tt * 16 <= lim[nt][c];
+                    int8_t& own = own_eo[warp][nt * 8 + 2 * qc + c];
+                    if (!seen && qr == 0 && own < kQ8ExpMin) own = (int8_t)eo;
+                    const float f = seen ? dn : 1.f;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[nt][md][e] *= dn;
-        }
-        // (past the last unit: over stale bytes, unused)
-        if (AHEAD) products(ring + slot1 * kQdUnit + lane * 16, sn);
-#pragma unroll
-        for (int tt = 0; tt < TPU; ++tt) {
-            const float vf = q8_pow2(max(q8_scale_exp(vs[tt]) - eo + kQdBias, -126));
+                    for (int md = 0; md < KS; ++md) o[nt][md][c] *= f, o[nt][md][c + 2] *= f;
+                }
+            eo = ev;
+        };
+        auto weigh = [&](int tt, int ev) {
+            const float vf = q8_pow2(max(ev - eo + kQdBias, -126));
             uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -492,6 +503,20 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
                     }
                 }
             }
+        };
+        bool larger = false;
+#pragma unroll
+        for (int tt = 0; tt < TPU; ++tt) larger = larger || q8_scale_exp(vs[tt]) > eo;
+        if (TPU == 1 || larger) {                      // (rare for d = 64: its tiles overlap below)
+#pragma unroll
+            for (int tt = 0; tt < TPU; ++tt) {
+                const int ev = q8_scale_exp(vs[tt]);
+                if (ev > eo) raise(tt, ev);
+                weigh(tt, ev);
+            }
+        } else {
+#pragma unroll
+            for (int tt = 0; tt < TPU; ++tt) weigh(tt, q8_scale_exp(vs[tt]));
         }
         // the slot's bytes are in registers: refill it
         __syncwarp();
@@ -505,11 +530,12 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
     // ---- this warp's (max, sum, O) of every row to its drained ring
     {
         float* mine_f = reinterpret_cast<float*>(ring);        // [RB][max, sum, -, -, O]
-        const float un = q8_pow2(eo), bias = q8_pow2(-kQdBias);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
+                const int own = own_eo[warp][nt * 8 + 2 * qc + c];
+                const float un = q8_pow2((own < kQ8ExpMin ? eo : own) - kQdBias);
                 float ll = l[nt][c];
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) ll += __shfl_xor_sync(0xffffffffu, ll, off);
@@ -522,8 +548,8 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
                 }
 #pragma unroll
                 for (int md = 0; md < KS; ++md) {
-                    to[4 + 16 * md + qr] = o[nt][md][c] * un * bias;
-                    to[4 + 16 * md + qr + 8] = o[nt][md][c + 2] * un * bias;
+                    to[4 + 16 * md + qr] = o[nt][md][c] * un;
+                    to[4 + 16 * md + qr + 8] = o[nt][md][c + 2] * un;
                 }
             }
     }

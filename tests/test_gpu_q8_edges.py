@@ -1,0 +1,128 @@
+"""The 8-bit paged cache on the GPU where its blocks, tiles and scales are
+least even: what a row of attention may depend on, values of any size, rows and
+blocks of zeros.  Against the 64-bit restatement (tests/q8_reference.py)."""
+import numpy as np
+import pytest
+
+from tests import q8_reference as ref
+from tests.test_gpu_q8 import Made, clean_error_word, device_error, i32  # noqa: F401 (clean_error_word: a fixture)
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def fill(mk, k, v, n):
+    """Writes k, v [batch, rows, kv, d] (fp32) from the start, n[b] rows; returns the reference."""
+    r = mk.reference()
+    mk.cache.write(0, torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda(), i32([0] * mk.batch), n_rows=i32(n))
+    r.append(0, k, v, [0] * mk.batch, n)
+    return r
+
+
+def row_error(mk, r, b, h, n, q, got, out_dtype, see=None, prompt=False):
+    """Largest error of output rows got [rows, d] of queries q [rows, d] over entries
+    `see` (all n) of one head, in units of the bound.
+
+    An output is sum p v.  Weights are off by the factor 1 +- 2 delta (scores,
+    sums and merges: attention_tolerance with vmax 1), so the sum by 2 delta
+    sum p |v|.  What enters the product is p 2^(e - E) in f16 beside codes of at
+    most 448, e the block's exponent and E the largest of the blocks in sight:
+    one f16 number for bf16 outputs (half a step, 2^-11 of it), two for fp32
+    (2^-22), and below f16's normal numbers half a step of 2^-24 beside weights
+    that enter times 2^6: 2^-31 of 448 2^E for each key.  Then one rounding to
+    the output's type.  Prompt calls with bf16 outputs: queries are one f16
+    number too, see prompt_tolerance."""
+    see = np.arange(n) if see is None else see
+    kk, vv = (x[see] for x in r.entries(b, 0, h, n))
+    s = q.astype(np.float64) @ kk.T / np.sqrt(mk.d)
+    bound = (np.abs(q.astype(np.float64)) @ np.abs(kk).T).max() / np.sqrt(mk.d)
+    p = np.exp(s - s.max(-1, keepdims=True))
+    p /= p.sum(-1, keepdims=True)
+    want = p @ vv
+    top = 448 * 2.0 ** max(int(r.exp[mk.table_np[b, 0, e // mk.page], h, 1]) for e in see)
+    delta = ref.attention_tolerance(mk.d, n, bound, 1.0, 0.0)[1] + (2.0 ** -11 if out_dtype is BF16 else 2.0 ** -22)
+    if prompt and out_dtype is BF16:
+        delta += 2 * 2.0 ** -11 * bound
+    tol = delta * (p @ np.abs(vv)) + len(see) * 2.0 ** -31 * top + torch.finfo(out_dtype).eps / 2 * np.abs(want) \
+        + torch.finfo(out_dtype).smallest_normal
+    return float((np.abs(got.double().cpu().numpy() - want) / tol).max())
+
+
+# ----------------------------------------------- up to 64 rows: tiles of a unit
+@pytest.mark.parametrize("d,page", [(64, 16), (64, 64), (128, 16)])
+@pytest.mark.parametrize("size", [1.0, 1e-2, 1e-4, 1e-6, 2.0 ** -30, 2.0 ** -100])
+def test_small_values_in_a_half_filled_unit(d, page, size):
+    """Lengths whose last 32 entries hold one tile of 16, or a part of it."""
+    lengths = [1, 5, 12, 16, 33, 37, 48, 64]
+    mk = Made(len(lengths), 1, 2, d, page, 128 // page, seed=d)
+    rng = np.random.default_rng(page)
+    k, v = (rng.standard_normal((len(lengths), 64, 2, d)).astype(np.float32) for _ in range(2))
+    r = fill(mk, k, (v * np.float32(size)).astype(np.float32), lengths)
+    for group in (1, 3, 6):
+        q = rng.standard_normal((len(lengths), 1, 2 * group, d)).astype(np.float32)
+        for dt in (BF16, F32):
+            out = mk.cache.attention(0, torch.from_numpy(q).cuda(), i32([n - 1 for n in lengths]), out_dtype=dt)
+            for b, n in enumerate(lengths):
+                for h in range(2):
+                    at = slice(h * group, (h + 1) * group)
+                    err = row_error(mk, r, b, h, n, q[b, 0, at], out[b, 0, at], dt)
+                    assert err <= 1, (n, group, dt, err)
+
+
+def test_small_values_beside_a_bad_page():
+    mk = Made(1, 1, 1, 64, 16, 6, seed=6)
+    rng = np.random.default_rng(0)
+    k, v = (rng.standard_normal((1, 90, 1, 64)).astype(np.float32) for _ in range(2))
+    r = fill(mk, k, (v * 1e-8).astype(np.float32), [90])
+    q = rng.standard_normal((1, 1, 2, 64)).astype(np.float32)
+    for page in (2, 3):
+        mk.table[0, 0, page] = -1
+        for dt in (BF16, F32):
+            out = mk.cache.attention(0, torch.from_numpy(q).cuda(), i32([89]), out_dtype=dt)
+            assert device_error() == 0x400
+            see = np.r_[0:16 * page, 16 * page + 16:90]
+            assert row_error(mk, r, 0, 0, 90, q[0, 0], out[0, 0], dt, see) <= 1
+        mk.table[0, 0, page] = int(mk.table_np[0, 0, page])
+
+
+@pytest.mark.parametrize("d,page", [(64, 16), (64, 32), (128, 16)])
+@pytest.mark.parametrize("step", [0, 10, -10, 40, 200, -200])
+def test_rows_do_not_depend_on_tiles_they_do_not_see(d, page, step):
+    """Verify calls from a unit's first tile into its second and beyond, V of
+    neighbouring tiles 2^step apart (at 200 from one end of the scales to the
+    other): every row equals the one-token call at its entry bit for bit."""
+    mk = Made(2, 1, 1, d, page, 1280 // page, seed=5)
+    rng = np.random.default_rng(d + page)
+    k, v = (rng.standard_normal((2, 1280, 1, d)).astype(np.float32) for _ in range(2))
+    size = np.ldexp(1.0, (np.arange(1280) // 16 % 2) * step - (step // 2 if step > 100 else 0)
+                    + (-step // 2 if step < -100 else 0))
+    fill(mk, k, (v * size[None, :, None, None]).astype(np.float32), [1280, 1280])
+    for e0, T, group in (([10, 1194], 9, 1), ([1194, 26], 9, 3), ([10, 1178], 17, 1), ([15, 31], 2, 2), ([8, 1000], 21, 3)):
+        q = torch.from_numpy((rng.standard_normal((2, T, group, d)) * 2).astype(np.float32)).cuda()
+        for dt in (BF16, F32):
+            whole = mk.cache.attention(0, q, i32(e0), out_dtype=dt)
+            assert torch.isfinite(whole).all()
+            for t in range(T):
+                one = mk.cache.attention(0, q[:, t:t + 1].contiguous(), i32([x + t for x in e0]), out_dtype=dt)
+                assert torch.equal(one[:, 0], whole[:, t]), (e0, T, group, dt, t)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("group,T", [(1, 64), (4, 16), (1, 8)])
+def test_rows_do_not_depend_on_far_larger_values_behind_them(d, group, T):
+    """From entry 256 on V is 2^200 larger: the rows before it, in one call with
+    rows behind it, give what they give alone."""
+    mk = Made(1, 1, 1, d, 16, 80, seed=5)
+    rng = np.random.default_rng(d)
+    k, v = (rng.standard_normal((1, 320, 1, d)).astype(np.float32) for _ in range(2))
+    v = np.ldexp(v, np.where(np.arange(320) < 256, -100, 100)[None, :, None, None]).astype(np.float32)
+    r = fill(mk, k, v, [320])
+    q = rng.standard_normal((1, T, group, d)).astype(np.float32)
+    e0 = 259 - T
+    for dt in (BF16, F32):
+        whole = mk.cache.attention(0, torch.from_numpy(q).cuda(), i32([e0]), out_dtype=dt)
+        for t in range(T):
+            one = mk.cache.attention(0, torch.from_numpy(q[:, t:t + 1].copy()).cuda(), i32([e0 + t]), out_dtype=dt)
+            assert torch.equal(one[:, 0], whole[:, t]), (dt, t)
+            assert row_error(mk, r, 0, 0, e0 + t + 1, q[0, t], whole[0, t], dt) <= 1, (dt, t)
