@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
         am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 1));
         am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 2));
         // am = 1.m * 2^ex; an infinite row keeps its infinities
-        const int ex = min(max((int)(__float_as_uint(am) >> 23) - 127, -100), 126);
+        const int ex = min(max((int)(__float_as_uint(am) >> 23) - 127, -126), 126);
         const float down = q8_pow2(-ex);
 #pragma unroll
         for (int kk = 0; kk < KS; ++kk) {

@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
                         for (int p = 0; p < 4; ++p) am = pf_max3(am, fabsf(x[k][ch][p].x), fabsf(x[k][ch][p].y));
 #pragma unroll
                     for (int o = 1; o < 8; o <<= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
-                    const int ex = min(max((int)(__float_as_uint(am * a.scale) >> 23) - 127, -100), 126);
+                    const int ex = min(max((int)(__float_as_uint(am * a.scale) >> 23) - 127, -126), 126);
                     const float f = a.scale * q8_pow2(-ex);
                     const int mx = __shfl_sync(0xffffffffu, ex, (lane & 3) * 8);
                     if ((lane >> 2) == i0 + k) c = q8_pow2(mx);   // (this thread's own row)
@@ -421,6 +421,9 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
         // this row's last key; rows that are not there see every key
         const int lim = mine ? min(e0 + gr / G, kend - 1) : kend - 1;
         float m = -INFINITY, l = 0.f;
+        // a score's factor; not zero (a row of zeros against a block of zeros), which
+        // would make NaN of the -infinity of what is not seen
+        auto factor = [&](float kscale) { return fmaxf(c * kscale, 1.175494351e-38f); };
         for (int j = 0; j < ntiles; ++j) {
             if (!__all_sync(0xffffffffu, mbar_wait(&s_full[t], (uint32_t)(j & 1), a.err))) {
                 ok = false;
@@ -466,10 +469,9 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
                     }
                 }
                 const float4 f = kf[half];
-                mn = pf_max3(mn, fmaxf(mx[0], mx[1]) * f.x, fmaxf(mx[2], mx[3]) * f.y);
-                mn = pf_max3(mn, fmaxf(mx[4], mx[5]) * f.z, fmaxf(mx[6], mx[7]) * f.w);
+                mn = pf_max3(mn, fmaxf(mx[0], mx[1]) * factor(f.x), fmaxf(mx[2], mx[3]) * factor(f.y));
+                mn = pf_max3(mn, fmaxf(mx[4], mx[5]) * factor(f.z), fmaxf(mx[6], mx[7]) * factor(f.w));
             }
-            mn *= c;
             float alpha = 1.f;
             if (mn > m + kQpLazy) {
                 alpha = pf_ex2(m - mn);                           // 0 from -infinity
@@ -486,8 +488,8 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
                 const float4 f = kf[k], dv = *reinterpret_cast<const float4*>(dv_s + j * 8 + 4 * k);
                 const float4 iv = *reinterpret_cast<const float4*>(iv_s + j * 8 + 4 * k);
                 uint64_t cg[4], og[4], sum2[4] = {0ull, 0ull, 0ull, 0ull};
-                cg[0] = pf_pack2(c * f.x, c * f.x), cg[1] = pf_pack2(c * f.y, c * f.y);
-                cg[2] = pf_pack2(c * f.z, c * f.z), cg[3] = pf_pack2(c * f.w, c * f.w);
+                const float fx = factor(f.x), fy = factor(f.y), fz = factor(f.z), fw = factor(f.w);
+                cg[0] = pf_pack2(fx, fx), cg[1] = pf_pack2(fy, fy), cg[2] = pf_pack2(fz, fz), cg[3] = pf_pack2(fw, fw);
                 og[0] = pf_pack2(off + dv.x, off + dv.x), og[1] = pf_pack2(off + dv.y, off + dv.y);
                 og[2] = pf_pack2(off + dv.z, off + dv.z), og[3] = pf_pack2(off + dv.w, off + dv.w);
                 tmem_wait_ld();

@@ -126,3 +126,40 @@ def test_rows_do_not_depend_on_far_larger_values_behind_them(d, group, T):
             one = mk.cache.attention(0, torch.from_numpy(q[:, t:t + 1].copy()).cuda(), i32([e0 + t]), out_dtype=dt)
             assert torch.equal(one[:, 0], whole[:, t]), (dt, t)
             assert row_error(mk, r, 0, 0, e0 + t + 1, q[0, t], whole[0, t], dt) <= 1, (dt, t)
+
+
+# ------------------------------------------------------------- prompt chunks
+def check_rows(mk, r, q, e0, out, out_dtype, prompt=True):
+    for b in range(mk.batch):
+        for h in range(mk.kv):
+            G = q.shape[2] // mk.kv
+            for t in range(q.shape[1]):
+                at = slice(h * G, (h + 1) * G)
+                err = row_error(mk, r, b, h, e0[b] + t + 1, q[b, t, at], out[b, t, at], out_dtype, prompt=prompt)
+                assert err <= 1, (b, h, t, err)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("T", [3, 100])
+def test_rows_and_blocks_of_zeros(d, T):
+    """Queries of zero, tiny ones, keys of zero: equal weights over what is seen,
+    also where 2^-100 (a zero query's exponent) meets 2^-120 (a zero block's)."""
+    mk = Made(1, 1, 1, d, 16, 16, seed=2)
+    rng = np.random.default_rng(d)
+    k, v = (rng.standard_normal((1, 200, 1, d)).astype(np.float32) for _ in range(2))
+    k[:, :48] = 0
+    k[:, 64:96] *= np.float32(2.0 ** -110)
+    v[:, 16:32] = 0
+    r = fill(mk, k, v, [200])
+    q = rng.standard_normal((1, T, 2, d)).astype(np.float32)
+    q[:, ::3] = 0
+    q[:, 1::3] *= np.float32(2.0 ** -90)
+    for e0 in (0, 30, 200 - T):
+        out = mk.cache.attention(0, torch.from_numpy(q).cuda(), i32([e0]), out_dtype=BF16)
+        check_rows(mk, r, q, [e0], out, BF16)
+    # keys near fp32's largest under queries near its smallest
+    k = (rng.standard_normal((1, 200, 1, d)) * 2.0 ** 120).astype(np.float32)
+    r = fill(mk, k, v, [200])
+    q = (rng.standard_normal((1, T, 2, d)) * 2.0 ** -120).astype(np.float32)
+    out = mk.cache.attention(0, torch.from_numpy(q).cuda(), i32([200 - T]), out_dtype=BF16)
+    check_rows(mk, r, q, [200 - T], out, BF16)
