@@ -15,12 +15,13 @@
 // order in which a lane's bytes lie: dims are permuted alike in Q and K, keys
 // alike in S, P and V (qp_key: a tile's column c belongs to the 16-token group
 // (c >> 6) * 4 + ((c >> 2) & 3)).
-// Block scales never touch the operands: K's multiplies the fp32 score, V's
-// (over the largest of the CTA's key range) is added to the exponent of the
-// probability that enters the product, and divided out of the row sum again; V
-// blocks more than 2^20 smaller are brought to that scale (their values lie 2^-20
-// and more below the range's largest; what is rounded off, 2^-37 below).
-// Rounding: queries are one f16 number each (2^-12 of the row's largest),
+// Block scales never touch the operands: K's multiplies the fp32 score, V's is added
+// to the exponent of the probability that enters the product (over the largest of
+// the key tiles so far, to which O is brought when it grows; in a row's last tiles
+// over the largest that the row itself sees, so that no row's precision depends on
+// keys it does not see), and divided out of the row sum again.  Weights of blocks
+// more than 2^40 below that are zeros in f16 whatever they are.
+// Rounding: queries are one f16 number each (2^-11 of the row's largest),
 // probabilities too, biased by 2^6 so that f16 keeps 2^-30 of the max; max, sum
 // and O are fp32.
 // Bound by the softmax warps: a key tile takes 4100 cycles at d = 128, of which
@@ -28,7 +29,7 @@
 // tiles), and a CTA 12000 more for its start and its end.  512 tokens of 2
 // sequences of up to 8192 entries, 8 heads, group 4: 161 us (98.7 GFLOP, 58 us at
 // the measured matrix rate; the shorter sequence's SMs idle at the end); 4096
-// tokens from the start: 178 us.
+// tokens from the start: 184 us.
 // Every mbarrier wait is bounded (error word 0x80).
 #include <algorithm>
 #include <type_traits>
@@ -49,7 +50,7 @@ constexpr int kQpSplit = 16384;         // most keys a split has (page ids stage
 constexpr int kQpMinSplit = 512;
 constexpr float kQpLazy = 8.f;
 constexpr int kQpBias = 6;
-constexpr int kQpDown = -20;            // V block exponents below the largest that probabilities carry
+constexpr int kQpDown = -40;            // V block exponents below the largest that probabilities carry
 
 // Element i (0..7) of a row's 16-byte unit u (of the d / 8) is dim
 // 32 (2 (u >> 3) + (u & 1)) + 16 (i >> 2) + 8 ((i >> 1) & 1) + 2 ((u & 7) >> 1) + (i & 1):
@@ -82,12 +83,44 @@ DKV_DEV uint32_t pack_bf2(float lo, float hi) {
     __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&v);
 }
-// Four codes times f (a power of two up to 1), rounded to codes again.
-DKV_DEV uint32_t rescaled(uint32_t w, float f) {
-    uint32_t lo, hi;
-    q8_decode4(w, lo, hi);
-    const float2 a = __half22float2(*reinterpret_cast<__half2*>(&lo)), b = __half22float2(*reinterpret_cast<__half2*>(&hi));
-    return q8_encode2(a.x * f, a.y * f) | (q8_encode2(b.x * f, b.y * f) << 16);
+// V exponent of a group below a row's unit, as probabilities carry it (all whole
+// numbers; a group that the row does not see may lie above: its probabilities are 0).
+DKV_DEV float qp_below(float ev, float unit) { return fmaxf(fminf(ev, unit) - unit, (float)kQpDown); }
+
+// A score's factor: the row's times the K scale, and not zero (a row of zeros against
+// a block of zeros), which would make NaN of the -infinity of what is not seen.
+DKV_DEV float qp_factor(float row, float kscale) { return fmaxf(row * kscale, 1.175494351e-38f); }
+
+// The second softmax pass (below) of a tile in which a row of the warp sees less than
+// what the tile's V exponents are counted from: under the row's own unit.  A call of
+// its own, since the loop around it fills the instruction cache (inlined but not
+// taken, it cost 512 tokens over 8192 entries 6 us of 161 at d 128, 14 of 141 at d 64).
+// Returns the tile's row sum.
+__device__ __noinline__ float qp_weigh_apart(uint32_t sb, const float* kf, const float* ev, float c, float off, float unit) {
+    float l = 0.f;
+#pragma unroll 1
+    for (int cc = 0; cc < 4; ++cc) {
+        uint32_t x[32], pk[16];
+        tmem_ld32(sb + 32 * cc, x);
+        tmem_wait_ld();
+#pragma unroll
+        for (int gi = 0; gi < 4; ++gi) {
+            const int g = (cc >> 1) * 4 + gi;
+            const float below = qp_below(ev[g], unit), f = qp_factor(c, kf[g]);
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+                if (((e >> 2) & 3) != gi) continue;
+                const float p0 = pf_ex2(fmaf(__uint_as_float(x[e]), f, off + below));
+                const float p1 = pf_ex2(fmaf(__uint_as_float(x[e + 1]), f, off + below));
+                sum += p0 + p1;
+                pk[e / 2] = h2(p0, p1);
+            }
+            l += sum * q8_pow2(-(int)below);
+        }
+        tmem_st16(sb + 16 * cc, pk);
+    }
+    return l;
 }
 
 template <int D>
@@ -100,12 +133,10 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
     __shared__ __align__(8) uint64_t s_full[2], p_full[2], o_done, drain;
     __shared__ uint32_t tmem_slot;
     __shared__ int32_t page_s[kQpSplit / 16];
-    // per 16-key group: K scale, V exponent below the largest (at least kQpDown), 2^-that, and what of
-    // the V scale is left for the operand (1 but for far smaller blocks)
-    __shared__ __align__(16) float kf_s[kQpSplit / 16], dv_s[kQpSplit / 16], iv_s[kQpSplit / 16];
-    __shared__ int8_t ev_s[kQpSplit / 16];
+    // per 16-key group: K scale, V exponent, that below the largest of the tiles so far, 2^-that
+    __shared__ __align__(16) float kf_s[kQpSplit / 16], ev_s[kQpSplit / 16], dv_s[kQpSplit / 16], iv_s[kQpSplit / 16];
+    __shared__ float top_s[kQpSplit / kQpKeys];                      // largest V exponent of the tiles so far
     __shared__ uint32_t bad_s[kQpSplit / kQpKeys / 4];               // 8 bits a key tile: 16-key groups not to be seen
-    __shared__ int emax_s;
 
     const Q8View& v = a.v;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -156,7 +187,6 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
         mbar_init(&drain, 1);
         fence_barrier_init();
         fence_async_shared();
-        emax_s = kQ8ExpMin;
     }
     for (int i = threadIdx.x; i < (ntiles + 3) / 4; i += kQpThreads) bad_s[i] = 0u;
     if (warp == 12) tmem_alloc(&tmem_slot, kQpTmemCols);
@@ -186,21 +216,40 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
             if (i >= ntiles * 8) break;
             const bool there = v.ok(pid[k]);
             const int ev = there ? min(max(q8_scale_exp(sc[k].y), kQ8ExpMin), kQ8ExpMax) : kQ8ExpMin;
-            if (there) {
-                atomicMax(&emax_s, ev);
-            } else if (i < n_grp) {
+            if (!there && i < n_grp) {
                 atomicOr(a.err, kErrQ8Page);
                 atomicOr(&bad_s[i >> 5], 1u << (i & 31));
             }
             page_s[i] = there ? pid[k] : -1;
             kf_s[i] = sc[k].x;
-            ev_s[i] = (int8_t)ev;
+            ev_s[i] = (float)ev;
+        }
+        named_sync(2, NS);
+        if (warp == 8) {
+            constexpr int PL = kQpSplit / kQpKeys / 32;           // tiles a lane, in order
+            float top[PL], run = (float)kQ8ExpMin;
+#pragma unroll
+            for (int k = 0; k < PL; ++k) {
+                const int j = lane * PL + k;
+                for (int i = 0; i < 8 && j < ntiles; ++i) run = fmaxf(run, ev_s[j * 8 + i]);
+                top[k] = run;
+            }
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const float y = __shfl_up_sync(0xffffffffu, run, o);
+                if (lane >= o) run = fmaxf(run, y);
+            }
+            float before = __shfl_up_sync(0xffffffffu, run, 1);
+            if (lane == 0) before = (float)kQ8ExpMin;
+#pragma unroll
+            for (int k = 0; k < PL; ++k)
+                if (lane * PL + k < ntiles) top_s[lane * PL + k] = fmaxf(top[k], before);
         }
         named_sync(2, NS);
         for (int i = first; i < ntiles * 8; i += NS) {
-            const int dv = max((int)ev_s[i] - emax_s, kQpDown);
-            dv_s[i] = (float)dv;
-            iv_s[i] = q8_pow2(-dv);
+            const float dv = qp_below(ev_s[i], top_s[i >> 3]);
+            dv_s[i] = dv;
+            iv_s[i] = q8_pow2(-(int)dv);
         }
         named_sync(2, NS);
     }
@@ -209,7 +258,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
     if (warp >= 8 && warp < 12) {
         // ---------------- converters: warp w takes groups 2 w and 2 w + 1 of a tile
         constexpr int NJ = D / 32;                                // 512-byte blocks a group and side
-        const int w = warp - 8, g = lane >> 2, t = lane & 3, evm = emax_s;
+        const int w = warp - 8, g = lane >> 2, t = lane & 3;
         uint4 kr[2][NJ], vr[2][NJ];
         auto load = [&](int j, int i, uint4 (&r)[2][NJ]) {
 #pragma unroll
@@ -245,21 +294,17 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
         // V: rows are dims 32 x + 8 q' + g; unit 2 t + (w & 1) of key half w >> 1 holds 4 tokens of each group
         auto put_v = [&](int j, uint8_t* dst) {
             // rare: bytes of tokens that are not there become zeros (their weight is
-            // 0, but 0 x NaN would not be), and blocks more than 2^20 below the
-            // largest are brought to that scale (rounded to e4m3 again)
+            // 0, but 0 x NaN would not be)
 #pragma unroll
             for (int gb = 0; gb < 2; ++gb) {
-                const int grp = j * 8 + 2 * w + gb, left = kend - k0 - grp * 16;
-                const int rest = (int)ev_s[grp] - evm - kQpDown;
-                if (left < 16 || rest < 0) {
+                const int left = kend - k0 - (j * 8 + 2 * w + gb) * 16;
+                if (left < 16) {
                     const uint32_t vm = (2 * t < left ? 0xffu : 0u) | (2 * t + 1 < left ? 0xff00u : 0u) |
                                         (2 * t + 8 < left ? 0xff0000u : 0u) | (2 * t + 9 < left ? 0xff000000u : 0u);
-                    const float f = q8_pow2(max(min(rest, 0), -126));
 #pragma unroll
                     for (int x = 0; x < NJ; ++x) {
                         uint4& r = vr[gb][x];
-                        r.x = rescaled(r.x & vm, f), r.y = rescaled(r.y & vm, f);
-                        r.z = rescaled(r.z & vm, f), r.w = rescaled(r.w & vm, f);
+                        r.x &= vm, r.y &= vm, r.z &= vm, r.w &= vm;
                     }
                 }
             }
@@ -420,10 +465,8 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
         }
         // this row's last key; rows that are not there see every key
         const int lim = mine ? min(e0 + gr / G, kend - 1) : kend - 1;
-        float m = -INFINITY, l = 0.f;
-        // a score's factor; not zero (a row of zeros against a block of zeros), which
-        // would make NaN of the -infinity of what is not seen
-        auto factor = [&](float kscale) { return fmaxf(c * kscale, 1.175494351e-38f); };
+        float m = -INFINITY, l = 0.f, unit = (float)kQ8ExpMin;
+        auto factor = [&](float kscale) { return qp_factor(c, kscale); };
         for (int j = 0; j < ntiles; ++j) {
             if (!__all_sync(0xffffffffu, mbar_wait(&s_full[t], (uint32_t)(j & 1), a.err))) {
                 ok = false;
@@ -432,6 +475,8 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
             tc_fence_after();
             const int lc = lim - (k0 + j * kQpKeys);              // last live column
             const uint32_t bad = (bad_s[j >> 2] >> ((j & 3) * 8)) & 0xffu;
+            float to = top_s[j];                                  // O's unit with this tile
+            bool apart = false;                                   // a row has a smaller one
             if (__any_sync(0xffffffffu, lc < kQpKeys - 1 || bad != 0u)) {
                 // a row's last tiles, or a bad page: -infinity over what is not seen
                 // (kept out of the loops below: their code has to stay small)
@@ -448,6 +493,11 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
                     tmem_st32(sb + 32 * cc, x);
                 }
                 tmem_wait_st();
+                to = unit;                                        // the groups this row sees count
+#pragma unroll 1
+                for (int i = 0; i < 8; ++i)
+                    if (16 * i <= lc) to = fmaxf(to, ev_s[j * 8 + i]);
+                apart = __any_sync(0xffffffffu, to != top_s[j]) != 0;
             }
             // pass 1: the largest score, group by group (one factor a group)
             float mn = -INFINITY;
@@ -477,54 +527,64 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
                 alpha = pf_ex2(m - mn);                           // 0 from -infinity
                 m = mn;
             }
-            // pass 2: probabilities 2^(s - m + bias + dv), as f16 pairs into columns read before
-            const float off = m == -INFINITY ? 0.f : (float)kQpBias - m;
-            l *= alpha;
-            uint32_t sr[2][32];
-#pragma unroll 1
-            for (int k = 0; k < 2; ++k) {
-                tmem_ld32(sb + 64 * k, sr[0]);
-                tmem_ld32(sb + 64 * k + 32, sr[1]);
-                const float4 f = kf[k], dv = *reinterpret_cast<const float4*>(dv_s + j * 8 + 4 * k);
-                const float4 iv = *reinterpret_cast<const float4*>(iv_s + j * 8 + 4 * k);
-                uint64_t cg[4], og[4], sum2[4] = {0ull, 0ull, 0ull, 0ull};
-                const float fx = factor(f.x), fy = factor(f.y), fz = factor(f.z), fw = factor(f.w);
-                cg[0] = pf_pack2(fx, fx), cg[1] = pf_pack2(fy, fy), cg[2] = pf_pack2(fz, fz), cg[3] = pf_pack2(fw, fw);
-                og[0] = pf_pack2(off + dv.x, off + dv.x), og[1] = pf_pack2(off + dv.y, off + dv.y);
-                og[2] = pf_pack2(off + dv.z, off + dv.z), og[3] = pf_pack2(off + dv.w, off + dv.w);
-                tmem_wait_ld();
-                uint32_t pk[32];
-#pragma unroll
-                for (int h3 = 0; h3 < 2; ++h3) {
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        const int gi = (e >> 2) & 3;
-                        float d0, d1;
-                        pf_unpack2(pf_fma2(pf_pack2(__uint_as_float(sr[h3][e]), __uint_as_float(sr[h3][e + 1])), cg[gi], og[gi]),
-                                   d0, d1);
-                        const float p0 = pf_ex2(d0), p1 = pf_ex2(d1);
-                        sum2[gi] = pf_add2(sum2[gi], pf_pack2(p0, p1));
-                        pk[h3 * 16 + e / 2] = h2(p0, p1);
-                    }
-                }
-                tmem_st32(sb + 32 * k, pk);
-                const float ivs[4] = {iv.x, iv.y, iv.z, iv.w};
-#pragma unroll
-                for (int gi = 0; gi < 4; ++gi) {
-                    float a0, a1;
-                    pf_unpack2(sum2[gi], a0, a1);
-                    l += (a0 + a1) * ivs[gi];
-                }
+            float shrink = alpha;                                 // O's factor: in units of 2^(unit - bias)
+            if (to > unit) {
+                shrink *= q8_pow2((int)fmaxf(unit - to, -126.f));
+                unit = to;
             }
-            if (j >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {
+            if (j >= 1 && __any_sync(0xffffffffu, shrink != 1.f)) {
 #pragma unroll 1
                 for (int c0 = 0; c0 < D; c0 += 32) {
                     uint32_t o[32];
                     tmem_ld32(ob + c0, o);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink);
                     tmem_st32(ob + c0, o);
+                }
+            }
+            // pass 2: probabilities 2^(s - m + bias + dv), as f16 pairs into columns read before
+            const float off = m == -INFINITY ? 0.f : (float)kQpBias - m;
+            l *= alpha;
+            if (apart) {
+                l += qp_weigh_apart(sb, kf_s + j * 8, ev_s + j * 8, c, off, unit);
+            } else {
+                uint32_t sr[2][32];
+#pragma unroll 1
+                for (int k = 0; k < 2; ++k) {
+                    tmem_ld32(sb + 64 * k, sr[0]);
+                    tmem_ld32(sb + 64 * k + 32, sr[1]);
+                    const float4 f = kf[k];
+                    const float4 dv = *reinterpret_cast<const float4*>(dv_s + j * 8 + 4 * k);
+                    const float4 iv = *reinterpret_cast<const float4*>(iv_s + j * 8 + 4 * k);
+                    uint64_t cg[4], og[4], sum2[4] = {0ull, 0ull, 0ull, 0ull};
+                    const float fx = factor(f.x), fy = factor(f.y), fz = factor(f.z), fw = factor(f.w);
+                    cg[0] = pf_pack2(fx, fx), cg[1] = pf_pack2(fy, fy), cg[2] = pf_pack2(fz, fz), cg[3] = pf_pack2(fw, fw);
+                    og[0] = pf_pack2(off + dv.x, off + dv.x), og[1] = pf_pack2(off + dv.y, off + dv.y);
+                    og[2] = pf_pack2(off + dv.z, off + dv.z), og[3] = pf_pack2(off + dv.w, off + dv.w);
+                    tmem_wait_ld();
+                    uint32_t pk[32];
+#pragma unroll
+                    for (int h3 = 0; h3 < 2; ++h3) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) {
+                            const int gi = (e >> 2) & 3;
+                            float d0, d1;
+                            pf_unpack2(pf_fma2(pf_pack2(__uint_as_float(sr[h3][e]), __uint_as_float(sr[h3][e + 1])), cg[gi], og[gi]),
+                                       d0, d1);
+                            const float p0 = pf_ex2(d0), p1 = pf_ex2(d1);
+                            sum2[gi] = pf_add2(sum2[gi], pf_pack2(p0, p1));
+                            pk[h3 * 16 + e / 2] = h2(p0, p1);
+                        }
+                    }
+                    tmem_st32(sb + 32 * k, pk);
+                    const float ivs[4] = {iv.x, iv.y, iv.z, iv.w};
+#pragma unroll
+                    for (int gi = 0; gi < 4; ++gi) {
+                        float a0, a1;
+                        pf_unpack2(sum2[gi], a0, a1);
+                        l += (a0 + a1) * ivs[gi];
+                    }
                 }
             }
             tmem_wait_st();
@@ -539,10 +599,9 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
         float* mypart = alone ? nullptr : a.part + ((bhr * a.n_splits + s) * kQpRows + cr) * PS;
         if (l != l && m == -INFINITY) m = 0.f;     // NaN scores have no max: give the row one, so that its NaN comes out
         const bool live = ok && m != -INFINITY;
-        const int evm = emax_s;
-        // O is in units of 2^(evm - bias), l in units of 2^-bias.  (Apart from the
-        // sum: 2^evm / l may be too small for fp32 where their result is not.)
-        const float un = alone ? q8_pow2(evm) : q8_pow2(evm - kQpBias);
+        // O is in units of 2^(unit - bias), l in units of 2^-bias.  (Apart from the
+        // sum: 2^unit / l may be too small for fp32 where their result is not.)
+        const float un = q8_pow2((int)unit - (alone ? 0 : kQpBias));
         const float f = alone && live ? 1.f / l : 1.f;
         const size_t out_at = (((size_t)b * a.T + gr / G) * v.n_kv * G + h * G + gr % G) * D;
         if (__all_sync(0xffffffffu, ok)) {

@@ -163,3 +163,41 @@ def test_rows_and_blocks_of_zeros(d, T):
     q = (rng.standard_normal((1, T, 2, d)) * 2.0 ** -120).astype(np.float32)
     out = mk.cache.attention(0, torch.from_numpy(q).cuda(), i32([200 - T]), out_dtype=BF16)
     check_rows(mk, r, q, [200 - T], out, BF16)
+
+
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 16), (128, 64)])
+@pytest.mark.parametrize("step", [24, 60, 200])
+def test_prompt_rows_before_far_larger_values(d, page, step):
+    """V grows by 2^step at entry 48 (inside the first tile of 128 keys), or at
+    200: rows before it keep the precision of what they see."""
+    T = 280
+    rng = np.random.default_rng(d + step)
+    for at in (48, 200):
+        mk = Made(1, 1, 1, d, page, 320 // page, seed=2)
+        k, v = (rng.standard_normal((1, T, 1, d)).astype(np.float32) for _ in range(2))
+        at -= at % page
+        v = np.ldexp(v, np.where(np.arange(T) < at, -step // 2, step - step // 2)[None, :, None, None]).astype(np.float32)
+        r = fill(mk, k, v, [T])
+        q = rng.standard_normal((1, T, 1, d)).astype(np.float32)
+        out = mk.cache.attention(0, torch.from_numpy(q).cuda(), i32([0]), out_dtype=BF16)
+        check_rows(mk, r, q, [0], out, BF16)
+
+
+def test_prompt_rows_before_far_larger_values_over_key_splits():
+    """The same where the keys are split (512 a split) and where a bad page lies between."""
+    T, e0, d = 100, 1000, 128
+    rng = np.random.default_rng(1)
+    for at, bad in ((1056, None), (992, 30), (512, None), (96, 61)):
+        mk = Made(1, 1, 1, d, 16, 80, seed=2)
+        k, v = (rng.standard_normal((1, e0 + T, 1, d)).astype(np.float32) for _ in range(2))
+        v = np.ldexp(v, np.where(np.arange(e0 + T) < at, -60, 40)[None, :, None, None]).astype(np.float32)
+        r = fill(mk, k, v, [e0 + T])
+        if bad is not None:
+            mk.table[0, 0, bad] = -1
+        q = rng.standard_normal((1, T, 2, d)).astype(np.float32)
+        out = mk.cache.attention(0, torch.from_numpy(q).cuda(), i32([e0]), out_dtype=BF16)
+        assert device_error() == (0 if bad is None else 0x400)
+        for t in range(0, T, 7):
+            see = np.arange(e0 + t + 1)
+            see = see if bad is None else see[see // 16 != bad]
+            assert row_error(mk, r, 0, 0, e0 + t + 1, q[0, t], out[0, t], BF16, see, prompt=True) <= 1, (at, t)
