@@ -726,8 +726,8 @@ size_t decode_work(dkv_dims dims, int R, int capacity, int split_keys, bool mass
 size_t attn_q8_work_upto(dkv_dims dims, int group, int max_T, int capacity, bool mass) {
     const int T1 = std::min(max_T, std::max(1, kQ8MaxRows / group));
     size_t w = dkv_q8_attn_work_bytes(dims, group, T1, capacity, 0, mass ? 1 : 0);
-    // (rows of a prompt chunk count in blocks of 256: one T of each block count)
-    for (long long R = kQ8MaxRows + 1; R <= (long long)max_T * group; R = (R + 255) / 256 * 256 + 1)
+    // (rows of a prompt chunk count in blocks of 128 or 256: one T of each block count)
+    for (long long R = kQ8MaxRows + 1; R <= (long long)max_T * group; R = (R + 127) / 128 * 128 + 1)
         w = std::max(w, attn_q8_prefill_work(dims, 1, (int)std::min(R, 1ll << 24), capacity));
     return w;
 }

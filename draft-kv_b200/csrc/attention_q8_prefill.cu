@@ -21,9 +21,11 @@
 // over the largest that the row itself sees, so that no row's precision depends on
 // keys it does not see), and divided out of the row sum again.  Weights of blocks
 // more than 2^40 below that are zeros in f16 whatever they are.
-// Rounding: queries are one f16 number each (2^-11 of the row's largest),
-// probabilities too, biased by 2^6 so that f16 keeps 2^-30 of the max; max, sum
-// and O are fp32.
+// Rounding, bf16 outputs: queries are one f16 number each (2^-11 of the row's
+// largest), probabilities too, biased by 2^6 so that f16 keeps 2^-30 of the max;
+// max, sum and O are fp32.  fp32 outputs (WIDE): both are two f16 numbers, as in
+// calls of up to 64 rows; products double, and one query tile a CTA does not
+// overlap with another (512 tokens over 2 x 8192 entries 420 us).
 // Bound by the softmax warps: a key tile takes 4100 cycles at d = 128, of which
 // the tensor cores work half and the exp2 units half (each 2050 for both query
 // tiles), and a CTA 12000 more for its start and its end.  512 tokens of 2
@@ -41,7 +43,9 @@ namespace dkv {
 
 namespace {
 
-constexpr int kQpTile = 128, kQpRows = 256, kQpKeys = 128;
+constexpr int kQpTile = 128, kQpKeys = 128;
+// Query rows a CTA: two tiles, or one whose queries' lower parts take the second's place
+constexpr int qp_rows(bool wide) { return wide ? kQpTile : 2 * kQpTile; }
 constexpr int kQpSoft = 256, kQpConv = 128;
 constexpr int kQpThreads = kQpSoft + kQpConv + 32;
 constexpr int kQpNst = 2;               // K and V ring depth
@@ -79,6 +83,11 @@ DKV_DEV uint32_t h2(float lo, float hi) {
     __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&v);
 }
+// What h = h2(lo, hi) leaves of its numbers.
+DKV_DEV uint32_t h2_rest(float lo, float hi, uint32_t h) {
+    const float2 x = __half22float2(*reinterpret_cast<__half2*>(&h));
+    return h2(lo - x.x, hi - x.y);
+}
 DKV_DEV uint32_t pack_bf2(float lo, float hi) {
     __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&v);
@@ -91,16 +100,18 @@ DKV_DEV float qp_below(float ev, float unit) { return fmaxf(fminf(ev, unit) - un
 // a block of zeros), which would make NaN of the -infinity of what is not seen.
 DKV_DEV float qp_factor(float row, float kscale) { return fmaxf(row * kscale, 1.175494351e-38f); }
 
-// The second softmax pass (below) of a tile in which a row of the warp sees less than
-// what the tile's V exponents are counted from: under the row's own unit.  A call of
-// its own, since the loop around it fills the instruction cache (inlined but not
+// The second softmax pass (below) a group at a time, under the row's own unit: tiles
+// in which a row of the warp sees less than what the tile's V exponents are counted
+// from, and WIDE's, whose probabilities' lower parts go 256 columns further.  A call
+// of its own, since the loop around it fills the instruction cache (inlined but not
 // taken, it cost 512 tokens over 8192 entries 6 us of 161 at d 128, 14 of 141 at d 64).
 // Returns the tile's row sum.
-__device__ __noinline__ float qp_weigh_apart(uint32_t sb, const float* kf, const float* ev, float c, float off, float unit) {
+template <bool WIDE>
+__device__ __noinline__ float qp_weigh_groups(uint32_t sb, const float* kf, const float* ev, float c, float off, float unit) {
     float l = 0.f;
 #pragma unroll 1
     for (int cc = 0; cc < 4; ++cc) {
-        uint32_t x[32], pk[16];
+        uint32_t x[32], pk[16], lo[16];
         tmem_ld32(sb + 32 * cc, x);
         tmem_wait_ld();
 #pragma unroll
@@ -115,18 +126,22 @@ __device__ __noinline__ float qp_weigh_apart(uint32_t sb, const float* kf, const
                 const float p1 = pf_ex2(fmaf(__uint_as_float(x[e + 1]), f, off + below));
                 sum += p0 + p1;
                 pk[e / 2] = h2(p0, p1);
+                if (WIDE) lo[e / 2] = h2_rest(p0, p1, pk[e / 2]);
             }
             l += sum * q8_pow2(-(int)below);
         }
         tmem_st16(sb + 16 * cc, pk);
+        if (WIDE) tmem_st16(sb + 256 + 16 * cc, lo);
     }
     return l;
 }
 
-template <int D>
+// WIDE (fp32 outputs): queries and probabilities are two f16 numbers each; the CTA
+// has one query tile, the lower parts take the other's shared and tensor memory.
+template <int D, bool WIDE>
 __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_constant__ Q8AttnArgs a) {
     using Geo = QpGeo<D>;
-    constexpr int PS = D + 4;
+    constexpr int PS = D + 4, ROWS = qp_rows(WIDE), TILES = ROWS / kQpTile;
     extern __shared__ uint8_t qp_raw[];
     uint8_t* sm = qp_raw + ((1024u - (smem_u32(qp_raw) & 1023u)) & 1023u);
     __shared__ __align__(8) uint64_t k_full[kQpNst], k_empty[kQpNst], v_full[kQpNst], v_empty[kQpNst];
@@ -149,7 +164,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
     const int rb = a.n_rb - 1 - (int)(blockIdx.x / v.n_kv / a.n_splits % a.n_rb);
     const int b = (int)(blockIdx.x / v.n_kv / a.n_splits / a.n_rb);
     const int G = a.group;
-    const int r0 = rb * kQpRows, R = min(kQpRows, a.T * G - r0);
+    const int r0 = rb * ROWS, R = min(ROWS, a.T * G - r0);
     const size_t bhr = ((size_t)b * v.n_kv + h) * a.n_rb + rb;
     const bool alone = a.n_splits == 1;
 
@@ -169,7 +184,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
             return;
         }
         for (int r = threadIdx.x; r < R; r += kQpThreads)
-            *reinterpret_cast<float2*>(a.part + ((bhr * a.n_splits + s) * kQpRows + r) * PS) = make_float2(-INFINITY, 0.f);
+            *reinterpret_cast<float2*>(a.part + ((bhr * a.n_splits + s) * ROWS + r) * PS) = make_float2(-INFINITY, 0.f);
         return;
     }
     if (threadIdx.x == 0) {
@@ -357,6 +372,11 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
             for (int ks = 0; ks < kQpKeys / 16; ++ks)
                 tc_mma_ts(base + 128, base + ks * 8, sw128_desc(v_s + (ks >> 2) * (D * 128) + (ks & 3) * 32), idO,
                           (i | ks) != 0 ? 1u : 0u);
+            if (WIDE) {
+#pragma unroll
+                for (int ks = 0; ks < kQpKeys / 16; ++ks)
+                    tc_mma_ts(base + 128, base + 256 + ks * 8, sw128_desc(v_s + (ks >> 2) * (D * 128) + (ks & 3) * 32), idO, 1u);
+            }
         };
         auto issue_s = [&](int t, int j) {
             const uint32_t k_s = k_s0 + (j % kQpNst) * Geo::KVB;
@@ -365,6 +385,12 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
             for (int kk = 0; kk < D / 16; ++kk)
                 tc_mma_i(tmem + (uint32_t)(t * 256), sw128_desc(qt + (kk >> 2) * 16384 + (kk & 3) * 32),
                          sw128_desc(k_s + (kk >> 2) * 16384 + (kk & 3) * 32), idS, kk != 0 ? 1u : 0u);
+            if (WIDE) {
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk)
+                    tc_mma_i(tmem, sw128_desc(q_s + Geo::QT + (kk >> 2) * 16384 + (kk & 3) * 32),
+                             sw128_desc(k_s + (kk >> 2) * 16384 + (kk & 3) * 32), idS, 1u);
+            }
             tc_commit(&s_full[t]);
         };
         named_sync(1, kQpSoft + 32);      // Q is in shared memory, and the softmax warps may read the scales
@@ -374,7 +400,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
                 ok = false;
                 break;
             }
-            for (int t = 0; t < 2; ++t) {
+            for (int t = 0; t < TILES; ++t) {
                 if (j >= 1 && !wait_all(&p_full[t], (uint32_t)((j - 1) & 1))) {
                     ok = false;
                     break;
@@ -396,7 +422,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
         if (ok) {
             const int i = ntiles - 1;
             ok = wait_all(&v_full[i % kQpNst], (uint32_t)((i / kQpNst) & 1));
-            for (int t = 0; t < 2 && ok; ++t) {
+            for (int t = 0; t < TILES && ok; ++t) {
                 if (!wait_all(&p_full[t], (uint32_t)(i & 1))) {
                     ok = false;
                     break;
@@ -409,8 +435,9 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
             __syncwarp();
         }
     } else {
-        // ---------------- softmax: row rt of query tile t = TMEM lane rt; CTA row cr
-        const int t = warp >> 2, rt = threadIdx.x & 127, cr = t * kQpTile + rt, gr = r0 + cr;
+        // ---------------- softmax: row rt of query tile t = TMEM lane rt; CTA row cr.
+        // (WIDE: tile 0 alone; warps 4-7 load the queries' lower parts and are done)
+        const int half = warp >> 2, t = WIDE ? 0 : half, rt = threadIdx.x & 127, cr = t * kQpTile + rt, gr = r0 + cr;
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t sb = lanes + (uint32_t)(t * 256), ob = sb + 128;
         const bool mine = cr < R && gr / G < n_tok;
@@ -422,7 +449,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
             // rows go out together
             constexpr int B = 4, CH = Geo::CH;                    // 4-row steps a round, 64-dim halves
             const int li = lane & 7, from = 32 * (li & 1) + 2 * (li >> 1);
-            uint8_t* qt = sm + t * Geo::QT;
+            uint8_t* qt = sm + half * Geo::QT;
 #pragma unroll 1
             for (int i0 = 0; i0 < 8; i0 += B) {
                 float2 x[B][CH][4];
@@ -453,10 +480,15 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
                     if ((lane >> 2) == i0 + k) c = q8_pow2(mx);   // (this thread's own row)
 #pragma unroll
                     for (int ch = 0; ch < CH; ++ch) {
-                        const float2(&y)[4] = x[k][ch];
+                        uint32_t u[4];
+#pragma unroll
+                        for (int p = 0; p < 4; ++p) {
+                            const float y0 = x[k][ch][p].x * f, y1 = x[k][ch][p].y * f;
+                            u[p] = h2(y0, y1);
+                            if (WIDE && half) u[p] = h2_rest(y0, y1, u[p]);
+                        }
                         *reinterpret_cast<uint4*>(qt + ch * 16384 + row * 128 + ((li ^ (row & 7)) << 4)) =
-                            make_uint4(h2(y[0].x * f, y[0].y * f), h2(y[1].x * f, y[1].y * f), h2(y[2].x * f, y[2].y * f),
-                                       h2(y[3].x * f, y[3].y * f));
+                            make_uint4(u[0], u[1], u[2], u[3]);
                     }
                 }
             }
@@ -467,7 +499,8 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
         const int lim = mine ? min(e0 + gr / G, kend - 1) : kend - 1;
         float m = -INFINITY, l = 0.f, unit = (float)kQ8ExpMin;
         auto factor = [&](float kscale) { return qp_factor(c, kscale); };
-        for (int j = 0; j < ntiles; ++j) {
+        const bool idle = WIDE && half;
+        for (int j = 0; j < ntiles && !idle; ++j) {
             if (!__all_sync(0xffffffffu, mbar_wait(&s_full[t], (uint32_t)(j & 1), a.err))) {
                 ok = false;
                 break;
@@ -546,8 +579,8 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
             // pass 2: probabilities 2^(s - m + bias + dv), as f16 pairs into columns read before
             const float off = m == -INFINITY ? 0.f : (float)kQpBias - m;
             l *= alpha;
-            if (apart) {
-                l += qp_weigh_apart(sb, kf_s + j * 8, ev_s + j * 8, c, off, unit);
+            if (WIDE || apart) {
+                l += qp_weigh_groups<WIDE>(sb, kf_s + j * 8, ev_s + j * 8, c, off, unit);
             } else {
                 uint32_t sr[2][32];
 #pragma unroll 1
@@ -591,12 +624,12 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
             tc_fence_before();
             mbar_arrive(&p_full[t]);
         }
-        if (ok) {
+        if (ok && !idle) {
             ok = __all_sync(0xffffffffu, mbar_wait(&o_done, 0u, a.err));
             tc_fence_after();
         }
         // ---- the row's output (one split) or its partial (max, sum, O)
-        float* mypart = alone ? nullptr : a.part + ((bhr * a.n_splits + s) * kQpRows + cr) * PS;
+        float* mypart = alone ? nullptr : a.part + ((bhr * a.n_splits + s) * ROWS + cr) * PS;
         if (l != l && m == -INFINITY) m = 0.f;     // NaN scores have no max: give the row one, so that its NaN comes out
         const bool live = ok && m != -INFINITY;
         // O is in units of 2^(unit - bias), l in units of 2^-bias.  (Apart from the
@@ -604,10 +637,10 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
         const float un = q8_pow2((int)unit - (alone ? 0 : kQpBias));
         const float f = alone && live ? 1.f / l : 1.f;
         const size_t out_at = (((size_t)b * a.T + gr / G) * v.n_kv * G + h * G + gr % G) * D;
-        if (__all_sync(0xffffffffu, ok)) {
+        if (__all_sync(0xffffffffu, ok) && !idle) {
             // through the drained K and V rings (a part of each warp's own), so that
             // whole rows are stored: a lane's 16-byte chunk ch of row r at ch ^ r
-            const bool wide = !alone || a.out_dtype == DKV_F32;
+            const bool wide = WIDE || !alone;
             uint8_t* stg = sm + Geo::K0 + warp * (32 * D * 4);
 #pragma unroll 1
             for (int c0 = 0; c0 < D; c0 += 32) {
@@ -650,7 +683,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
             else
                 copy_rows(std::integral_constant<int, D / 8>{}, [&](int, size_t at) { return reinterpret_cast<uint8_t*>(a.out) + at * 2; });
         }
-        if (!alone && cr < R)
+        if (!alone && cr < R && !idle)
             *reinterpret_cast<float2*>(mypart) = make_float2(live ? m : -INFINITY, live ? l * q8_pow2(-kQpBias) : 0.f);
     }
 
@@ -670,17 +703,17 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
 }
 
 // The splits' partial rows merged into outputs, D / 4 threads a row (a launch of
-// its own: the 256 rows of a block, by the CTA that ends last, took 35 to 60 us).
+// its own: 256 rows of a block, by the CTA that ends last, took 35 to 60 us).
 constexpr int kQpMergeThreads = 256;
-template <int D>
+template <int D, int BLOCK>              // rows a block of the partials
 __global__ void __launch_bounds__(kQpMergeThreads) q8_prefill_merge_kernel(Q8AttnArgs a) {
     constexpr int PS = D + 4, ROWS = kQpMergeThreads * 4 / D;          // rows a CTA
     pdl_wait();
-    const int h = blockIdx.y, b = blockIdx.z, row0 = blockIdx.x * ROWS, rb = row0 / kQpRows, r0 = rb * kQpRows;
+    const int h = blockIdx.y, b = blockIdx.z, row0 = blockIdx.x * ROWS, rb = row0 / BLOCK, r0 = rb * BLOCK;
     const int n_tok = a.n_rows ? min(a.n_rows[b], a.T) : a.T;
     const size_t bhr = ((size_t)b * a.v.n_kv + h) * a.n_rb + rb;
-    q8_merge_items<D, kQpRows, 4, 1, 8>(a, a.part + bhr * a.n_splits * (size_t)kQpRows * PS, b, h, r0,
-                                        min(kQpRows, a.T * a.group - r0), n_tok, (row0 - r0) * (D / 4) + threadIdx.x, 0);
+    q8_merge_items<D, BLOCK, 4, 1, 8>(a, a.part + bhr * a.n_splits * (size_t)BLOCK * PS, b, h, r0,
+                                      min(BLOCK, a.T * a.group - r0), n_tok, (row0 - r0) * (D / 4) + threadIdx.x, 0);
 }
 
 // Keys per split: the whole capacity up to 16384 keys; where the row blocks
@@ -694,10 +727,10 @@ int prefill_split(dkv_dims dims, int n_rb, int capacity) {
     return std::min((keys + kQpKeys - 1) / kQpKeys * kQpKeys, kQpSplit);
 }
 
-size_t prefill_layout(dkv_dims dims, int group, int T, int capacity, Q8AttnArgs* a, Arena* ar) {
-    const int R = T * group, n_rb = (R + kQpRows - 1) / kQpRows;
+size_t prefill_layout(dkv_dims dims, int group, int T, int capacity, bool wide, Q8AttnArgs* a, Arena* ar) {
+    const int R = T * group, rows = qp_rows(wide), n_rb = (R + rows - 1) / rows;
     const int split = prefill_split(dims, n_rb, capacity), ns = std::max(1, (capacity + split - 1) / split);
-    const size_t part = ns == 1 ? 0 : (size_t)dims.batch * dims.n_kv * n_rb * ns * kQpRows * (dims.d + 4);
+    const size_t part = ns == 1 ? 0 : (size_t)dims.batch * dims.n_kv * n_rb * ns * rows * (dims.d + 4);
     if (a) {
         a->split = split;
         a->n_splits = ns;
@@ -708,34 +741,38 @@ size_t prefill_layout(dkv_dims dims, int group, int T, int capacity, Q8AttnArgs*
     return kQ8Tickets * sizeof(unsigned) + align_up(part * sizeof(float), 256) + 1024;
 }
 
+template <int D, bool WIDE>
+int launch_prefill(const Q8AttnArgs& a, dkv_dims dims, cudaStream_t st) {
+    const size_t ctas = (size_t)dims.batch * dims.n_kv * a.n_rb * a.n_splits;
+    DKV_REQUIRE(ctas <= 0x7fffffffu, "dkv_q8_attn: batch x heads x row blocks too large");
+    constexpr auto kernel = q8_prefill_kernel<D, WIDE>;
+    DKV_CUDA(allow_smem_max_once<kernel>());
+    DKV_CUDA(launch_pdl(kernel, dim3((unsigned)ctas), dim3(kQpThreads), QpGeo<D>::SMEM, st, a));
+    if (a.n_splits > 1) {
+        constexpr int rows = kQpMergeThreads * 4 / D;
+        const dim3 mg((unsigned)((a.T * a.group + rows - 1) / rows), (unsigned)dims.n_kv, (unsigned)dims.batch);
+        constexpr auto merge = q8_prefill_merge_kernel<D, qp_rows(WIDE)>;
+        DKV_CUDA(launch_pdl(merge, mg, dim3(kQpMergeThreads), 0, st, a));
+    }
+    return DKV_OK;
+}
+
 }  // namespace
 
+// (for either type of outputs)
 size_t attn_q8_prefill_work(dkv_dims dims, int group, int T, int capacity) {
-    return prefill_layout(dims, group, T, capacity, nullptr, nullptr);
+    return std::max(prefill_layout(dims, group, T, capacity, false, nullptr, nullptr),
+                    prefill_layout(dims, group, T, capacity, true, nullptr, nullptr));
 }
 
 int attn_q8_prefill(Q8AttnArgs& a, dkv_dims dims, void* work, size_t work_bytes, cudaStream_t st) {
+    const bool wide = a.out_dtype == DKV_F32;
     Arena ar(work, work_bytes);
-    prefill_layout(dims, a.group, a.T, a.v.capacity(), &a, &ar);
+    prefill_layout(dims, a.group, a.T, a.v.capacity(), wide, &a, &ar);
     DKV_REQUIRE(a.part, "dkv_q8_attn: work buffer");
-    const size_t ctas = (size_t)dims.batch * dims.n_kv * a.n_rb * a.n_splits;
-    DKV_REQUIRE(ctas <= 0x7fffffffu, "dkv_q8_attn: batch x heads x row blocks too large");
     ProfScope ps(DKV_PROF_ATTN_FULL, 0.0, st);
-    const dim3 grid((unsigned)ctas);
-    if (dims.d == 128) {
-        DKV_CUDA(allow_smem_max_once<q8_prefill_kernel<128>>());
-        DKV_CUDA(launch_pdl(q8_prefill_kernel<128>, grid, dim3(kQpThreads), QpGeo<128>::SMEM, st, a));
-    } else {
-        DKV_CUDA(allow_smem_max_once<q8_prefill_kernel<64>>());
-        DKV_CUDA(launch_pdl(q8_prefill_kernel<64>, grid, dim3(kQpThreads), QpGeo<64>::SMEM, st, a));
-    }
-    if (a.n_splits > 1) {
-        const int rows = kQpMergeThreads * 4 / dims.d;
-        const dim3 mg((unsigned)((a.T * a.group + rows - 1) / rows), (unsigned)dims.n_kv, (unsigned)dims.batch);
-        DKV_CUDA(dims.d == 128 ? launch_pdl(q8_prefill_merge_kernel<128>, mg, dim3(kQpMergeThreads), 0, st, a)
-                               : launch_pdl(q8_prefill_merge_kernel<64>, mg, dim3(kQpMergeThreads), 0, st, a));
-    }
-    return DKV_OK;
+    if (dims.d == 128) return wide ? launch_prefill<128, true>(a, dims, st) : launch_prefill<128, false>(a, dims, st);
+    return wide ? launch_prefill<64, true>(a, dims, st) : launch_prefill<64, false>(a, dims, st);
 }
 
 }  // namespace dkv

@@ -220,7 +220,9 @@ class Q8KVCache(PagedKVCache):
         by default); tokens t >= n_rows[b] are skipped and their rows of `out`
         left as they were (zeros when `out` is made here).  mass (T * n_heads /
         n_kv <= 64): every seen entry's softmax weights are added to it.  A row
-        of up to 64 equals the one-token call at that entry bit for bit.  `work`:
+        of up to 64 equals the one-token call at that entry bit for bit.  With
+        fp32 outputs queries and weights keep 22 bits; with bf16 outputs weights
+        keep 11, and queries too where T * n_heads / n_kv > 64.  `work`:
         uint8 scratch of `dkv_q8_attn_work_bytes`, the first 64 KB zero when
         first used, for a caller that keeps its own; by default the cache has one
         per stream, and a captured call one of its own."""

@@ -201,3 +201,60 @@ def test_prompt_rows_before_far_larger_values_over_key_splits():
             see = np.arange(e0 + t + 1)
             see = see if bad is None else see[see // 16 != bad]
             assert row_error(mk, r, 0, 0, e0 + t + 1, q[0, t], out[0, t], BF16, see, prompt=True) <= 1, (at, t)
+
+
+WIDE = [   # batch, kv, group, d, page, pages, T, entries before the call, n_rows
+    (1, 1, 1, 64, 16, 5, 65, [0], None), (2, 2, 4, 128, 16, 20, 17, [300, 0], None), (1, 1, 1, 64, 32, 10, 301, [3], None),
+    (2, 1, 3, 128, 64, 6, 100, [250, 7], [100, 31]), (3, 1, 2, 64, 16, 40, 129, [500, 128, -20], None),
+    (1, 1, 2, 128, 16, 80, 70, [1200], None), (2, 1, 4, 64, 16, 320, 40, [5000, 17], [40, 0]),
+]
+
+
+@pytest.mark.parametrize("shape", WIDE, ids=lambda s: f"b{s[0]}kv{s[1]}g{s[2]}d{s[3]}p{s[4]}T{s[6]}")
+@pytest.mark.parametrize("size", [1.0, 1e-20])
+def test_prompt_calls_with_fp32_outputs_hold_their_bits(shape, size):
+    """More than 64 rows a head, fp32 outputs: queries and weights as two f16
+    numbers each, as calls of up to 64 rows hold them."""
+    batch, kv, group, d, page, pages, T, e0, n_rows = shape
+    mk = Made(batch, 1, kv, d, page, pages, seed=T)
+    rng = np.random.default_rng(d + T)
+    n = [max(x + T, 1) for x in e0]
+    k, v = (rng.standard_normal((batch, max(n), kv, d)).astype(np.float32) for _ in range(2))
+    v *= np.exp(rng.standard_normal((batch, max(n), kv, 1))).astype(np.float32)
+    r = fill(mk, k, (v * np.float32(size)).astype(np.float32), n)
+    q = (rng.standard_normal((batch, T, kv * group, d)) * 1.5).astype(np.float32)
+    out = torch.full(q.shape, 5.0, device="cuda")
+    mk.cache.attention(0, torch.from_numpy(q).cuda(), i32(e0), n_rows=None if n_rows is None else i32(n_rows), out=out)
+    for b in range(batch):
+        live = T if n_rows is None else n_rows[b]
+        assert (out[b, live:] == 5).all()
+        for t in range(0, live, 3):
+            if e0[b] + t < 0:
+                assert (out[b, t] == 0).all()
+                continue
+            for h in range(kv):
+                at = slice(h * group, (h + 1) * group)
+                err = row_error(mk, r, b, h, e0[b] + t + 1, q[b, t, at], out[b, t, at], F32, prompt=True)
+                assert err <= 1, (b, t, h, err)
+
+
+def test_prompt_calls_with_fp32_outputs_where_scales_differ():
+    """fp32 outputs over blocks 2^24 and 2^60 apart, zeros and a bad page."""
+    T, d = 200, 64
+    rng = np.random.default_rng(6)
+    mk = Made(1, 1, 1, d, 16, 16, seed=2)
+    k, v = (rng.standard_normal((1, T, 1, d)).astype(np.float32) for _ in range(2))
+    v = np.ldexp(v, np.array([-60, -36, 0, -3, 24, 0, 8, -50, 3, 30, 0, 0, 0])[np.arange(T) // 16][None, :, None, None])
+    k[:, 32:48], v[:, 64:80] = 0, 0
+    r = fill(mk, k.astype(np.float32), v.astype(np.float32), [T])
+    q = rng.standard_normal((1, T, 2, d)).astype(np.float32)
+    q[:, ::9] = 0
+    for bad in (None, 3):
+        if bad is not None:
+            mk.table[0, 0, bad] = -1
+        out = mk.cache.attention(0, torch.from_numpy(q).cuda(), i32([0]), out_dtype=F32)
+        assert device_error() == (0 if bad is None else 0x400)
+        for t in range(T):
+            see = np.arange(t + 1)
+            see = see if bad is None else see[see // 16 != bad]
+            assert row_error(mk, r, 0, 0, t + 1, q[0, t], out[0, t], F32, see, prompt=True) <= 1, t
