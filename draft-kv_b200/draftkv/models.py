@@ -283,8 +283,8 @@ class DeviceDecoder:
         if cache.pool is None:
             raise TypeError("a cache over external storage has no block allocator: use forward_raw")
         n = cache.length
-        if any(c != n for c in cache.counts[0]):
-            raise ValueError("the layers hold different numbers of entries (evict all of them alike)")
+        if any(c != n for c in cache.counts[0]) or len(set(cache._gone[0])) > 1:
+            raise ValueError("the layers hold different entries (evict all of them alike)")
         if cache.next_pos[0] != start_pos:
             raise ValueError(f"the cache continues at position {cache.next_pos[0]}, start_pos {start_pos}")
         T = int(toks.shape[0])

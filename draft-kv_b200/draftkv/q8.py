@@ -62,6 +62,7 @@ class Q8KVCache(PagedKVCache):
         self.next_pos = [0] * batch          # position of the next token (entries + evicted)
         # per sequence and layer: entries from here on are the last positions of every head
         self._floor = [[0] * n_layers for _ in range(batch)]
+        self._gone = [[0] * n_layers for _ in range(batch)]     # entries evicted since the sequence was empty
 
     @staticmethod
     def _check_shape(d_head: int, block_size: int) -> None:
@@ -364,16 +365,35 @@ class Q8KVCache(PagedKVCache):
         """Rollback to n_pos entries (paged.py:144-162); the scale of a partly
         emptied block stays until the block is written from its start again.
         After an eviction a sequence can go back through its recent entries (or
-        to none): before them the heads hold different positions."""
-        floor = max(self._floor[b])
-        if 0 < n_pos < floor:
-            raise ValueError(f"entries before {floor} of sequence {b} hold other positions in each head")
-        if n_pos <= 0:
-            self._floor[b] = [0] * self.n_layers
-        before = self.counts[b][0]
+        to none): before them the heads hold different positions.  Layers of
+        which different numbers were evicted can only go back together while
+        they hold equally many entries: otherwise entry n_pos is another position
+        in each."""
+        n_pos, counts = max(n_pos, 0), self.counts[b]
+        self._check_rollback(b, n_pos)
+        if n_pos >= max(counts):
+            return
+        if n_pos == 0:
+            self._floor[b], self._gone[b] = [0] * self.n_layers, [0] * self.n_layers
+        before = counts[0]
         super().truncate_seq(b, n_pos)
-        left = self.counts[b][0]
+        left = counts[0]
         self.next_pos[b] = self.next_pos[b] - (before - left) if left else 0
+
+    def _check_rollback(self, b: int, n_pos: int) -> None:
+        counts, floor = self.counts[b], max(self._floor[b])
+        if not 0 < n_pos < max(counts):
+            return
+        if len(set(counts)) > 1 and len(set(self._gone[b])) > 1:
+            raise ValueError(f"the layers of sequence {b} hold different positions (evict all of them alike)")
+        if n_pos < floor:
+            raise ValueError(f"entries before {floor} of sequence {b} hold other positions in each head")
+
+    def truncate(self, n_pos: int) -> None:
+        """Every sequence, or where one cannot go back to n_pos none."""
+        for b in range(self.batch):
+            self._check_rollback(b, n_pos)
+        super().truncate(n_pos)
 
     def set_length(self, b: int, n: int) -> None:
         self.next_pos[b] += n - self.counts[b][0]
@@ -424,6 +444,7 @@ class Q8KVCache(PagedKVCache):
                 self.table_host[b, L, :len(ids)] = table[b, :len(ids)]
                 self.counts[b][L] = m[b]
                 if n[b] > m[b]:
+                    self._gone[b][L] += n[b] - m[b]
                     self._floor[b][L] = max(self._floor[b][L] - (n[b] - m[b]), m[b] - recent)
             self._dirty = True
         return out
