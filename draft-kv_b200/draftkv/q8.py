@@ -302,14 +302,13 @@ class Q8KVCache(PagedKVCache):
     # ---------------------------------------------------- cache protocol
     def append(self, layer: int, k, v, pos) -> None:
         """Rows (numpy [rows, n_kv, d]) of sequence 0 at its end; positions must
-        follow each other (after an eviction they run ahead of the entries)."""
+        go on where the layer's end (after an eviction ahead of the entries)."""
         k, v = np.asarray(k, np.float32), np.asarray(v, np.float32)
         pos = np.asarray(pos).reshape(-1)
         n, start = k.shape[0], self.counts[0][layer]
         if n == 0:
             return
-        if not np.array_equal(pos, np.arange(pos[0], pos[0] + n)) or pos[0] < start \
-                or (pos[0] != start and not self.track_mass):
+        if not np.array_equal(pos, start + self._gone[0][layer] + np.arange(n)):
             raise ValueError("appended positions must be consecutive and continue the cache's")
         self._ensure_layer(0, layer, start + n)
         kv = torch.from_numpy(np.ascontiguousarray(np.stack([k, v])[:, None])).to(self.device)

@@ -122,3 +122,22 @@ def test_rollback_of_a_batch_is_all_or_nothing():
     c.truncate(37)
     assert c.counts == [[37, 37], [37, 37]] and c.next_pos == [37, 77]
     c.pool.check_invariants()
+
+
+def test_appends_continue_the_layer_s_positions():
+    c = HostCache()
+    for start in (1, 5):
+        with pytest.raises(ValueError):
+            put(c, 0, start, 3)
+    for L in (0, 1):
+        put(c, L, 0, 80)
+    c.evict(8, sink=0, recent=4)
+    for start in (8, 10, 79, 81):              # positions the cache has seen, or a gap
+        with pytest.raises(ValueError):
+            put(c, 0, start, 2)
+    put(c, 0, 80, 2)
+    with pytest.raises(ValueError):
+        put(c, 1, 82, 1)                       # layer 1 goes on at 80 whatever layer 0 holds
+    put(c, 1, 80, 2)
+    assert c.next_pos == [82] and c.counts == [[10, 10]]
+    assert (c.positions(1)[:, -3:] == [79, 80, 81]).all()
