@@ -402,7 +402,8 @@ class Q8KVCache(PagedKVCache):
         """Prunes every sequence to at most max(budget, sink + recent) entries a
         layer by accumulated attention mass, per KV head.  New blocks are taken
         from the pool before the old ones return to it (BlockPoolExhausted leaves
-        the cache as it was).  Returns {layer: kept entry indices [batch, n_kv,
+        the cache as it was; where a call fails later, the layers before it are
+        pruned, and it and those behind it are as they were).  Returns {layer: kept entry indices [batch, n_kv,
         .] on the device} of the layers that were pruned."""
         if not self.track_mass:
             raise ValueError("evict needs track_mass=True")
@@ -426,14 +427,18 @@ class Q8KVCache(PagedKVCache):
         out = {}
         for L, n, m, pages in plan:
             new = [self.pool.allocate_many(p) for p in pages]
-            out_pages = max(max(pages), 1)
-            table = torch.full((self.batch, out_pages), -1, dtype=torch.int32)
-            for b, ids in enumerate(new):
-                table[b, :len(ids)] = torch.tensor(ids, dtype=torch.int32)
-            dev = self.device
-            out[L], _, _ = self.evict_rows(
-                L, torch.tensor(n, dtype=torch.int32).to(dev), torch.tensor(m, dtype=torch.int32).to(dev), table.to(dev),
-                self.mass[L], self.pos_t[L], sink, recent, self.mass[-1], self.pos_t[-1])
+            try:
+                table = torch.full((self.batch, max(max(pages), 1)), -1, dtype=torch.int32)
+                for b, ids in enumerate(new):
+                    table[b, :len(ids)] = torch.tensor(ids, dtype=torch.int32)
+                dev = self.device
+                out[L], _, _ = self.evict_rows(
+                    L, torch.tensor(n, dtype=torch.int32).to(dev), torch.tensor(m, dtype=torch.int32).to(dev), table.to(dev),
+                    self.mass[L], self.pos_t[L], sink, recent, self.mass[-1], self.pos_t[-1])
+            except BaseException:
+                for blk in reversed([blk for ids in new for blk in ids]):
+                    self.pool.free(blk)
+                raise
             self.mass[L], self.mass[-1] = self.mass[-1], self.mass[L]
             self.pos_t[L], self.pos_t[-1] = self.pos_t[-1], self.pos_t[L]
             for b, ids in enumerate(new):

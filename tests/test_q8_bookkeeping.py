@@ -9,7 +9,7 @@ import pytest
 from tests import q8_reference as ref
 
 torch = pytest.importorskip("torch")
-from draftkv import Q8KVCache  # noqa: E402
+from draftkv import BlockPoolExhausted, Q8KVCache  # noqa: E402
 
 
 class HostCache(Q8KVCache):
@@ -141,3 +141,25 @@ def test_appends_continue_the_layer_s_positions():
     put(c, 1, 80, 2)
     assert c.next_pos == [82] and c.counts == [[10, 10]]
     assert (c.positions(1)[:, -3:] == [79, 80, 81]).all()
+
+
+def test_a_failed_eviction_returns_its_blocks():
+    c = HostCache(batch=2)
+    for L in (0, 1):
+        put(c, L, 0, 80)
+    before = state(c)
+    c.fail = True
+    with pytest.raises(RuntimeError):
+        c.evict(40, sink=0, recent=4)
+    assert state(c) == before
+    c.pool.check_invariants()
+    c.fail = False
+    c.evict(40, sink=0, recent=4)
+    assert c.counts[0] == [40, 40] and c.blocks_in_use == 6
+    small = HostCache(n_blocks=10)
+    for L in (0, 1):
+        put(small, L, 0, 80)
+    before = state(small)
+    with pytest.raises(BlockPoolExhausted):
+        small.evict(40, sink=0, recent=4)
+    assert state(small) == before
