@@ -183,6 +183,8 @@ class DraftKVEngine:
         lens = [len(p) - 1 for p in prompts]
         L = max(lens) if lens else 0
         CH = max(self.prefill_chunk, self.prefill_tokens // max(B, 1)) if L >= 1024 else 64
+        if isinstance(st.full, Q8KVCache):
+            st.full.truncate(0)         # a cache that was used: no evicted entries, positions from 0
         if isinstance(st.full, Q8KVCache) and st.full.track_mass:
             CH = max(1, min(CH, MASS_ROWS // m.n_rep))      # every prompt token adds to the mass
         tok = torch.zeros((B, max(L, 1)), dtype=torch.int32)
