@@ -121,7 +121,8 @@ class Q8KVCache(PagedKVCache):
         self._struct = _lib.Q8CacheS(self.codes.data_ptr(), self.scale.data_ptr(), self.table_dev.data_ptr(),
                                      self.codes.shape[0], self.block_size, self.max_pages)
         self._dims = _lib.DimsS(self.n_layers, self.n_heads, self.d_head, self.batch)
-        self._work: dict = {}
+        self._work: dict = {}            # scratch by stream (threads with streams of their own do not meet)
+        self._work_bytes: dict = {}      # its size by call
 
     def struct(self) -> "_lib.Q8CacheS":
         self.sync_table()
@@ -151,21 +152,19 @@ class Q8KVCache(PagedKVCache):
         when made and left so by each call.  A call that is being captured gets
         one of its own, cleared by the graph itself: graphs may be replayed side
         by side."""
-        capturing = torch.cuda.is_current_stream_capturing()
-        key = (T, group, split_keys, note_mass, stream)
-        w = None if capturing else self._work.get(key)
-        if w is None:
+        key = (T, group, split_keys, note_mass)
+        n = self._work_bytes.get(key)
+        if n is None:
             n = max(int(_lib.load().dkv_q8_attn_work_bytes(self._dims, group, T, self.capacity_tokens, split_keys,
                                                            1 if note_mass else 0)), WORK_ZERO_BYTES)
-            if not capturing:
-                w = next((t for k, t in self._work.items() if k[4] == stream), None)
-            if w is None or w.numel() < n:
-                w = torch.empty(n, dtype=torch.uint8, device=self.device)
-                w[:WORK_ZERO_BYTES].zero_()
-                if not capturing:        # (the smaller one goes)
-                    self._work = {k: t for k, t in self._work.items() if k[4] != stream}
-            if not capturing:
-                self._work[key] = w
+            self._work_bytes[key] = n
+        capturing = torch.cuda.is_current_stream_capturing()
+        w = None if capturing else self._work.get(stream)
+        if w is None or w.numel() < n:
+            w = torch.empty(n, dtype=torch.uint8, device=self.device)
+            w[:WORK_ZERO_BYTES].zero_()
+            if not capturing:            # (the smaller one goes)
+                self._work[stream] = w
         return w
 
     def _stream(self) -> int:

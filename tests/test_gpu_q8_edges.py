@@ -258,3 +258,47 @@ def test_prompt_calls_with_fp32_outputs_where_scales_differ():
             see = np.arange(t + 1)
             see = see if bad is None else see[see // 16 != bad]
             assert row_error(mk, r, 0, 0, t + 1, q[0, t], out[0, t], F32, see, prompt=True) <= 1, t
+
+
+# ------------------------------------------------------------------- scratch
+def test_threads_with_streams_of_their_own_share_a_cache():
+    """Several threads, a stream each, call one cache with sizes it has not seen:
+    the scratch of one must not be in another's way."""
+    import sys
+    import threading
+    mk = Made(1, 1, 1, 64, 16, 70, seed=4)
+    rng = np.random.default_rng(4)
+    k, v = (rng.standard_normal((1, 1100, 1, 64)).astype(np.float32) for _ in range(2))
+    fill(mk, k, v, [1100])
+    calls = [(T, split) for T in range(1, 60) for split in (0, 128, 256)]
+    q = {T: torch.randn((1, T, 1, 64), device="cuda") for T in range(1, 60)}
+    e0 = {T: i32([1100 - T]) for T in q}
+    want = {c: mk.cache.attention(0, q[c[0]], e0[c[0]], split_keys=c[1]) for c in calls}
+    from draftkv import Q8KVCache
+    shared = Q8KVCache.from_storage(mk.codes, mk.scale, mk.table)
+    torch.cuda.synchronize()
+    wrong, start = [], threading.Barrier(4)
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                start.wait()
+                for c in calls[i::2] + calls[::2]:
+                    got = shared.attention(0, q[c[0]], e0[c[0]], split_keys=c[1])
+                    torch.cuda.current_stream().synchronize()
+                    if not torch.equal(got, want[c]):
+                        wrong.append(c)
+        except Exception as e:
+            wrong.append(e)
+
+    interval = sys.getswitchinterval()
+    sys.setswitchinterval(1e-6)
+    try:
+        threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+    finally:
+        sys.setswitchinterval(interval)
+    assert not wrong, wrong[:3]
