@@ -738,7 +738,7 @@ using namespace dkv;
 extern "C" size_t dkv_q8_attn_work_bytes(dkv_dims dims, int group, int T, int capacity, int split_keys, int note_mass) {
     if (dims.batch < 1 || dims.n_kv < 1 || group < 1 || T < 1 || capacity < 1) return 0;
     const long long R = (long long)T * group;
-    if (R > (1 << 24) || capacity > (1 << 30)) return 0;
+    if (R > (1 << 24) || capacity > (1 << 30) || (split_keys > 0 && split_keys % 128)) return 0;
     if (R > kQ8MaxRows) return attn_q8_prefill_work(dims, group, T, capacity);
     return decode_work(dims, (int)R, capacity, split_keys, note_mass != 0, nullptr, nullptr);
 }

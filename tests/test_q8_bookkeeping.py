@@ -163,3 +163,12 @@ def test_a_failed_eviction_returns_its_blocks():
     with pytest.raises(BlockPoolExhausted):
         small.evict(40, sink=0, recent=4)
     assert state(small) == before
+
+
+def test_scratch_of_refused_calls_has_no_size():
+    """Split lengths that the call refuses ask for no scratch (one of 1 would mean a split an entry)."""
+    from draftkv import _lib
+    size = _lib.load(require_device=False).dkv_q8_attn_work_bytes
+    dims = _lib.DimsS(1, 2, 64, 1)
+    assert [size(dims, 4, 1, 1 << 20, s, 0) for s in (1, 100, 129)] == [0, 0, 0]
+    assert size(dims, 4, 1, 1 << 20, 128, 0) > size(dims, 4, 1, 1 << 20, 1024, 0) > 65536
