@@ -2,8 +2,9 @@
 // verify), and the attention mass that eviction goes by.
 //
 // softmax(q K^T / sqrt(d)) V per row, row t of sequence b over entries
-// 0 .. entry0[b] + t.  Memory-bound: 2 d bytes an entry and KV head, read once
-// for all rows.  Keys are the rows of the tensor-core products (m16n8k16):
+// 0 .. entry0[b] + t.  Memory-bound up to a block of 8 or 16 rows: 2 d bytes an
+// entry and KV head, read (from HBM or L2) and widened once for each such block of
+// query rows.  Keys are the rows of the tensor-core products (m16n8k16):
 // S^T = K Q^T and O^T += V^T P^T, 8 query rows as columns, so that the few
 // rows of a decode step waste little.  The cache's bytes are stored in operand
 // order, so a lane's 16-byte shared-memory load is an operand after
@@ -26,9 +27,10 @@
 // fixed by its index alone and a row's arithmetic does not depend on the other
 // rows of the call, so a verify row equals the decode step at that entry bit for
 // bit.
-// Measured (d 128, group 4, bf16): a fixed 11 us (launch, first bytes, two
-// merges) and then 6.9 TB/s; a warp needs about 1900 cycles a unit, so one CTA
-// alone streams 27 GB/s, which bounds ragged batches.  6 warps with units of
+// Measured (d 128, group 4, bf16): 262144 entries of 8 heads (537 MB) in 92 us,
+// 5.8 TB/s, of which about 10 us are launch, first bytes and two merges; a warp
+// needs about 1900 cycles a unit, so one CTA alone streams 27 GB/s, which bounds
+// ragged batches.  6 warps with units of
 // 8 KB (half the overhead a byte) were slower: 262144 entries 95 for 90 us.
 //
 // The running max is raised lazily: only when a score exceeds it by more than
@@ -258,10 +260,10 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
     // thr: the score that forces m up
     float m[NT][2], thr[NT][2], l[NT][2];
     float o[NT][KS][4];
-    // O is in units of 2^(eo - kQdBias), eo the largest V exponent so far; for a row
-    // that sees no more when it grows (the growth may be more than fp32 spans) in the
-    // units of own_eo
-    int eo = kQ8ExpMin;
+    // O is in units of 2^(eo - kQdBias), eo the largest V exponent so far or one below
+    // (probabilities, at most 2^8, then enter as p * 2^(bias + 1)); for a row that sees
+    // no more when it grows (the growth may be more than fp32 spans) in those of own_eo
+    int eo = q8_scale_exp(__shfl_sync(0xffffffffu, cur.vs, 0));
     if (lane < RB) own_eo[warp][lane] = (int8_t)-128;
     __syncwarp();
 #pragma unroll
@@ -432,8 +434,6 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
                 }
             }
         }
-        // (past the last unit: over stale bytes, unused)
-        if (AHEAD) products(ring + slot1 * kQdUnit + lane * 16, sn);
         // (uniform) larger V values in a tile: O to their units, tile by
         // tile, so that a row's probabilities are rounded under the exponents of the
         // tiles it sees.  (A row that does not see this tile sees none behind it.)
@@ -506,12 +506,15 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
         };
         bool larger = false;
 #pragma unroll
-        for (int tt = 0; tt < TPU; ++tt) larger = larger || q8_scale_exp(vs[tt]) > eo;
-        if (TPU == 1 || larger) {                      // (rare for d = 64: its tiles overlap below)
+        for (int tt = 0; tt < TPU; ++tt) larger = larger || q8_scale_exp(vs[tt]) > eo + 1;
+        if (TPU == 1 && larger) raise(0, q8_scale_exp(vs[0]));
+        // (past the last unit: over stale bytes, unused)
+        if (AHEAD) products(ring + slot1 * kQdUnit + lane * 16, sn);
+        if (TPU > 1 && larger) {                       // (rare: below the tiles overlap)
 #pragma unroll
             for (int tt = 0; tt < TPU; ++tt) {
                 const int ev = q8_scale_exp(vs[tt]);
-                if (ev > eo) raise(tt, ev);
+                if (ev > eo + 1) raise(tt, ev);
                 weigh(tt, ev);
             }
         } else {
@@ -671,13 +674,14 @@ __global__ void __launch_bounds__(kMassThreads) q8_mass_kernel(Q8AttnArgs a, flo
         if (key0 + k * kMassThreads < n) mass[bh * cap + key0 + k * kMassThreads] = old[k] + sum[k];
 }
 
-// Query rows a CTA: 16, or 8 where the rows come in an odd number of eights (at
-// d = 64, where a block of 16 takes 1.6 times one of 8, up to three of them; at
-// d = 128 1.9 times).  4 x 8 heads, 32768 entries: 20 rows of d 128 128 us in
-// eights, 155 in sixteens; of d 64 77 and 81; 56 rows of d 64 169 and 157.
+// Query rows a CTA: 16, or 8 where the rows come in an odd number of eights, up to
+// three of them at d = 64 (where a block of 16 takes 1.6 times one of 8), up to five
+// at d = 128.  4 x 8 heads, 32768 entries, bf16 outputs, in eights and in sixteens:
+// d 128 20 rows 130 and 145 us, 36 rows 211 and 212 (fp32 228 and 234), 56 rows 293
+// and 276; d 64 20 rows 81 and 86, 36 rows 129 and 124.
 int row_block(int R, int d) {
     const int e = (R + 7) / 8;
-    return e % 2 && (d == 128 || e <= 3) ? 8 : 16;
+    return e % 2 && e <= (d == 128 ? 5 : 3) ? 8 : 16;
 }
 
 template <int D, int NT, bool PLO, bool PAIR>
