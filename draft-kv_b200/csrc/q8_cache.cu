@@ -207,7 +207,8 @@ __global__ void __launch_bounds__(kQ8Threads) q8_append_kernel(Q8AppendArgs a) {
 }
 
 // [n][n_kv][2][d] fp32 of entries [0, n) of one sequence: one CTA per
-// (16-token tile, head), a thread per 16-byte fragment of K and V.
+// (16-token tile, head), a thread an element at a time (byte loads: for reading
+// back and tests, no path of a forward).
 __global__ void q8_read_kernel(Q8View v, int b, int n, float* dst, uint32_t* err) {
     const int tile = blockIdx.x, h = blockIdx.y, d = v.d;
     const int pid = v.row(b)[(tile * 16) >> v.page_shift];
