@@ -110,3 +110,29 @@ def test_engine_starts_over_in_a_cache_that_was_used():
     cache.truncate(50)                            # nothing was evicted in this run
     m.forward(np.array([1]), cache, 50)
     cache.pool.check_invariants()
+
+
+def test_bounded_decoding_in_the_pool_it_needs():
+    """A loop that prunes at 64 entries to 32 runs in the blocks of 64 entries a
+    layer and one layer's 32 kept ones; one block less is refused."""
+    from draftkv import BlockPoolExhausted, Q8KVCache
+    m, vocab = small_llama()
+    prompt = W.tokens(50, vocab, seed=2)
+
+    def run(n_blocks):
+        cache = Q8KVCache(m.n_layers, m.n_kv_heads, m.d_head, block_size=16, n_blocks=n_blocks, max_blocks_per_seq=4,
+                          track_mass=True)
+        logits = m.forward(np.array(prompt), cache, 0)
+        for _ in range(100):
+            token = int(logits[-1].argmax())
+            if cache.length >= 64:
+                cache.evict(32, sink=4, recent=8)
+            logits = m.forward(np.array([token]), cache, cache.next_pos[0])
+        return cache
+
+    cache = run(m.n_layers * 4 + 2)
+    assert cache.next_pos == [150] and 32 <= cache.length <= 64
+    assert (cache.positions(0)[:, -8:] == np.arange(142, 150)).all() and (cache.positions(1)[:, :4] == np.arange(4)).all()
+    cache.pool.check_invariants()
+    with pytest.raises(BlockPoolExhausted):
+        run(m.n_layers * 4 + 1)
