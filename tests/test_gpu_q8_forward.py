@@ -136,3 +136,25 @@ def test_bounded_decoding_in_the_pool_it_needs():
     cache.pool.check_invariants()
     with pytest.raises(BlockPoolExhausted):
         run(m.n_layers * 4 + 1)
+
+
+def test_batches_add_up_the_mass_of_their_own_sequences():
+    """Two sequences decoded together with the mass, against each alone (key splits,
+    and so the last bits, depend on the batch)."""
+    from draftkv import DraftKVEngine, Q8KVCache
+    m, vocab = small_llama()
+    prompts = [W.tokens(70, vocab, seed=s) for s in (5, 6)]
+
+    def run(ps):
+        cache = Q8KVCache(m.n_layers, m.n_kv_heads, m.d_head, block_size=32, n_blocks=30, batch=len(ps),
+                          max_blocks_per_seq=5, track_mass=True)
+        toks = DraftKVEngine(m, seed=0, full_cache_factory=lambda: cache).generate_baseline_batch(ps, 0, 0.0)
+        return toks, [x[:, :, :70].cpu().numpy() for x in cache.mass[:m.n_layers]]
+
+    both, mass = run(prompts)
+    for b, p in enumerate(prompts):
+        one, alone = run([p])
+        assert both[b] == one[0]
+        for L in range(m.n_layers):
+            assert np.abs(mass[L][b] - alone[L][0]).max() < TOL["bf16"] * alone[L].max()
+            assert np.abs(mass[L][b].sum() - m.n_rep * m.n_kv_heads * 69) < 1e-3 * 69     # 69 tokens, weights of sum 1
