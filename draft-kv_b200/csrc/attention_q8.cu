@@ -530,9 +530,9 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
     }
     __syncwarp();
 
-    // ---- this warp's (max, sum, O) of every row to its drained ring
+    // ---- this warp's (max, sum, O over the sum) of every row to its drained ring
     {
-        float* mine_f = reinterpret_cast<float*>(ring);        // [RB][max, sum, -, -, O]
+        float* mine_f = reinterpret_cast<float*>(ring);        // [RB][max, sum, -, -, O / sum]
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -542,6 +542,9 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
                 float ll = l[nt][c];
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) ll += __shfl_xor_sync(0xffffffffu, ll, off);
+                // O goes on over the sum (1 and more where a key was seen): an average of
+                // V, which fp32 holds whatever V is
+                const float inv = ll == 0.f ? 0.f : 1.f / ll;
                 // no key seen: -infinity (a row with NaN scores has a NaN sum, to be merged)
                 const float mm = thr[nt][c] == -INFINITY && ll == ll ? -INFINITY : m[nt][c];
                 float* to = mine_f + (nt * 8 + 2 * qc + c) * PS;
@@ -551,8 +554,8 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
                 }
 #pragma unroll
                 for (int md = 0; md < KS; ++md) {
-                    to[4 + 16 * md + qr] = o[nt][md][c] * un;
-                    to[4 + 16 * md + qr + 8] = o[nt][md][c + 2] * un;
+                    to[4 + 16 * md + qr] = o[nt][md][c] * inv * un;
+                    to[4 + 16 * md + qr + 8] = o[nt][md][c + 2] * inv * un;
                 }
             }
     }
@@ -570,10 +573,13 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
 #pragma unroll
         for (int g = 0; g < kQdKG; ++g) {
             const float mg = group_row(g, r)[0];
-            const float w = mg == -INFINITY ? 0.f : q8_ex2(mg - M);
-            if (w != 0.f) L += group_row(g, r)[1] * w;
+            const float w = mg == -INFINITY ? 0.f : group_row(g, r)[1] * q8_ex2(mg - M);
+            L += w;
             gw[r * kQdKG + g] = w;
         }
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+        for (int g = 0; g < kQdKG; ++g) gw[r * kQdKG + g] *= inv;
         if (failed) M = -INFINITY, L = 0.f;            // a failed split counts as empty
         ms[r] = M;
         ls[r] = L;
@@ -593,8 +599,7 @@ __global__ void __launch_bounds__(kQdThreads, 16 / kQdKG) q8_decode_kernel(const
             }
         }
         if (alone) {
-            const float L = ls[r];
-            q8_store2<D>(a, b, h, rbase + r, n_tok, e, L == 0.f ? 0.f : x0 / L, L == 0.f ? 0.f : x1 / L);
+            q8_store2<D>(a, b, h, rbase + r, n_tok, e, x0, x1);
         } else {
             *reinterpret_cast<float2*>(mypart + (size_t)r * PS + 4 + e) = make_float2(x0, x1);
         }
@@ -674,14 +679,14 @@ __global__ void __launch_bounds__(kMassThreads) q8_mass_kernel(Q8AttnArgs a, flo
         if (key0 + k * kMassThreads < n) mass[bh * cap + key0 + k * kMassThreads] = old[k] + sum[k];
 }
 
-// Query rows a CTA: 16, or 8 where the rows come in an odd number of eights, up to
-// three of them at d = 64 (where a block of 16 takes 1.6 times one of 8), up to five
-// at d = 128.  4 x 8 heads, 32768 entries, bf16 outputs, in eights and in sixteens:
-// d 128 20 rows 130 and 145 us, 36 rows 211 and 212 (fp32 228 and 234), 56 rows 293
-// and 276; d 64 20 rows 81 and 86, 36 rows 129 and 124.
+// Query rows a CTA: 16, or 8 where the rows come in an odd number of eights (at
+// d = 64, where a block of 16 takes 1.5 times one of 8, up to three of them).
+// 4 x 8 heads, 32768 entries, bf16 outputs, in eights and in sixteens: d 128 20 rows
+// 127 and 150 us, 36 rows 207 and 219, 56 rows 287 and 287 (fp32 309 and 322); d 64
+// 20 rows 80 and 81, 36 rows 127 and 117.
 int row_block(int R, int d) {
     const int e = (R + 7) / 8;
-    return e % 2 && e <= (d == 128 ? 5 : 3) ? 8 : 16;
+    return e % 2 && (d == 128 || e <= 3) ? 8 : 16;
 }
 
 template <int D, int NT, bool PLO, bool PAIR>

@@ -19,7 +19,7 @@ struct Q8AttnArgs {
     int out_dtype;
     int split, n_splits, n_rb;   // keys per split (prompt chunks), splits, row blocks per (sequence, head)
     float scale;                 // log2 e / sqrt(d)
-    float* part;                 // [batch][n_kv][n_rb][n_splits][rows a block][d + 4]: max, sum, -, -, O
+    float* part;                 // [batch][n_kv][n_rb][n_splits][rows a block][d + 4]: max, sum, -, -, O / sum
     unsigned* tickets;           // [batch][n_kv][n_rb]
     float* scores;               // [batch][n_kv][capacity][s_ld] (log2 units) or null
     float2* stats;               // [batch][n_kv][T * group] (max in log2 units, 1 / sum)
@@ -61,7 +61,8 @@ DKV_DEV void q8_store2(const Q8AttnArgs& a, int b, int h, int gr, int n_tok, int
 }
 // Rows r = i / (D / E), E elements from E (i % (D / E)) on, for items i = i0 + u *
 // stride (u < U): online over the splits in order, Q of them at a time, the loads
-// of all U items of a step in flight together.
+// of all U items of a step in flight together.  What is carried is the average so
+// far (sums of V near fp32's largest would overflow).
 template <int D, int RB, int E, int U, int Q>
 DKV_DEV void q8_merge_items(const Q8AttnArgs& a, const float* parts, int b, int h, int rbase, int R, int n_tok, int i0,
                             int stride) {
@@ -100,18 +101,23 @@ DKV_DEV void q8_merge_items(const Q8AttnArgs& a, const float* parts, int b, int 
 #pragma unroll
             for (int k = 0; k < Q; ++k) m = fmaxf(m, ml[u][k].x);
             if (m == -INFINITY) continue;
-            const float al = M[u] == -INFINITY ? 0.f : q8_ex2(M[u] - m);
+            float w[Q];
+            const float before = M[u] == -INFINITY ? 0.f : L[u] * q8_ex2(M[u] - m);
             M[u] = m;
-            L[u] *= al;
+            L[u] = before;
 #pragma unroll
-            for (int e = 0; e < E; ++e) x[u][e] *= al;
+            for (int k = 0; k < Q; ++k) {
+                w[k] = ml[u][k].x == -INFINITY ? 0.f : ml[u][k].y * q8_ex2(ml[u][k].x - m);
+                L[u] += w[k];
+            }
+            const float inv = 1.f / L[u];                  // (a split with a key has a sum of 1 or more, or NaN)
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[u][e] *= before * inv;
 #pragma unroll
             for (int k = 0; k < Q; ++k) {
                 if (ml[u][k].x == -INFINITY) continue;     // (its O was never written)
-                const float w = q8_ex2(ml[u][k].x - m);
-                L[u] += ml[u][k].y * w;
 #pragma unroll
-                for (int e = 0; e < E; ++e) x[u][e] += y[u][k][e] * w;
+                for (int e = 0; e < E; ++e) x[u][e] += y[u][k][e] * (w[k] * inv);
             }
         }
     }
@@ -122,15 +128,15 @@ DKV_DEV void q8_merge_items(const Q8AttnArgs& a, const float* parts, int b, int 
         const bool none = L[u] == 0.f;
 #pragma unroll
         for (int e = 0; e < E; e += 2)
-            q8_store2<D>(a, b, h, rbase + r, n_tok, at + e, none ? 0.f : x[u][e] / L[u], none ? 0.f : x[u][e + 1] / L[u]);
+            q8_store2<D>(a, b, h, rbase + r, n_tok, at + e, x[u][e], x[u][e + 1]);
         if (at == 0 && a.stats)
             a.stats[((size_t)b * a.v.n_kv + h) * (a.T * a.group) + rbase + r] =
                 make_float2(M[u], none || (rbase + r) / a.group >= n_tok ? 0.f : 1.f / L[u]);
     }
 }
 
-// After a CTA has stored its split's partial rows (max in log2 units, sum,
-// unnormalised O; an empty split has max -infinity and no O) of row block
+// After a CTA has stored its split's partial rows (max in log2 units, sum, O over
+// the sum; an empty split has max -infinity and no O) of row block
 // `bhr`, the last CTA to arrive merges all splits and writes the outputs (and
 // the rows' stats).  A thread merges an element pair on its own, 16 loads of
 // partials in flight: several splits of one item, or with few splits several

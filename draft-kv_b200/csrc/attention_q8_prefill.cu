@@ -628,14 +628,14 @@ __global__ void __launch_bounds__(kQpThreads, 1) q8_prefill_kernel(const __grid_
             ok = __all_sync(0xffffffffu, mbar_wait(&o_done, 0u, a.err));
             tc_fence_after();
         }
-        // ---- the row's output (one split) or its partial (max, sum, O)
+        // ---- the row's output (one split) or its partial (max, sum, O over the sum)
         float* mypart = alone ? nullptr : a.part + ((bhr * a.n_splits + s) * ROWS + cr) * PS;
         if (l != l && m == -INFINITY) m = 0.f;     // NaN scores have no max: give the row one, so that its NaN comes out
         const bool live = ok && m != -INFINITY;
         // O is in units of 2^(unit - bias), l in units of 2^-bias.  (Apart from the
         // sum: 2^unit / l may be too small for fp32 where their result is not.)
-        const float un = q8_pow2((int)unit - (alone ? 0 : kQpBias));
-        const float f = alone && live ? 1.f / l : 1.f;
+        const float un = q8_pow2((int)unit);
+        const float f = live ? 1.f / l : 1.f;
         const size_t out_at = (((size_t)b * a.T + gr / G) * v.n_kv * G + h * G + gr % G) * D;
         if (__all_sync(0xffffffffu, ok) && !idle) {
             // through the drained K and V rings (a part of each warp's own), so that

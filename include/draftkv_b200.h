@@ -292,8 +292,7 @@ DKV_API int dkv_q8_read(const dkv_q8_cache* cache, dkv_dims dims, int b, int lay
  * numbers each (22 bits), K and V enter exactly, the rest is fp32.  bf16
  * outputs: the weights are one f16 number (11 bits; they keep 2^-30 of the
  * largest under the largest V scale in a row's sight), above 64 rows the queries
- * too.  Values of V whose weighted sum before the division passes fp32 (2^128
- * over up to 256 times the entries) overflow.
+ * too.
  * Up to 64 query rows (T * group) a row's result does not depend on T or on
  * the other rows, bit for bit.  split_keys (a multiple of 128): the keys go to
  * ceil(capacity / split_keys) splits; 0: a rule on (batch, n_kv, capacity).

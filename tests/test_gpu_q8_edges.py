@@ -302,3 +302,24 @@ def test_threads_with_streams_of_their_own_share_a_cache():
     finally:
         sys.setswitchinterval(interval)
     assert not wrong, wrong[:3]
+
+
+# -------------------------------------------------- values near fp32's largest
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 32)])
+@pytest.mark.parametrize("T,n", [(1, 1), (1, 700), (9, 300), (20, 1200), (80, 80), (100, 1200), (70, 40)])
+def test_values_near_fp32_s_largest(d, page, T, n):
+    """V up to 448 2^119, over one warp, several, key splits and prompt chunks:
+    averages of finite values are finite."""
+    mk = Made(1, 1, 1, d, page, 1280 // page, seed=3)
+    rng = np.random.default_rng(T + n)
+    n = max(n, T)
+    k = (rng.standard_normal((1, n, 1, d)) * 0.3).astype(np.float32)
+    v = np.ldexp(1 + rng.random((1, n, 1, d)) * 0.7, 127).astype(np.float32) * np.sign(rng.standard_normal((1, n, 1, 1))).astype(np.float32)
+    r = fill(mk, k, v, [n])
+    q = rng.standard_normal((1, T, 2, d)).astype(np.float32)
+    mass = torch.zeros((1, 1, mk.cap), device="cuda") if T * 2 <= 64 else None
+    for dt in (BF16, F32):
+        for split in (0, 128) if T * 2 <= 64 else (0,):
+            out = mk.cache.attention(0, torch.from_numpy(q).cuda(), i32([n - T]), out_dtype=dt, split_keys=split, mass=mass)
+            assert torch.isfinite(out).all()
+            check_rows(mk, r, q, [n - T], out, dt, prompt=T * 2 > 64)
