@@ -78,7 +78,7 @@ struct QdMeta {
 };
 
 // NT: tiles of 8 query rows; PLO: probabilities as two f16 numbers (fp32
-// outputs; one keeps 2^-12 of a weight, a sixteenth of a bf16 output's
+// outputs; one holds a weight to 2^-11, an eighth of a bf16 output's
 // rounding).  PAIR (up to 4 rows): columns 4..7 of the score product hold the
 // queries' lower parts, so one product gives both sums; the same numbers are
 // multiplied and added as without, so a row's bits do not depend on it.
